@@ -12,7 +12,7 @@ import ctypes
 import os
 from typing import Optional
 
-import torch  # noqa: F401  (must be loaded before the HIP library)
+import torch  # (must be loaded before the HIP library)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GSPLAT_HIP_LIB", os.path.join(_HERE, "lib", "libgsplat_hip.so"))
@@ -26,6 +26,8 @@ STATUS_LOOKBACK_TIMEOUT = 1               # GSPLAT_STATUS_LOOKBACK_TIMEOUT
 HANDOFF_PAIRS = 128                       # GSPLAT_HANDOFF_PAIRS
 TIME_FORWARD, TIME_BACKWARD = 0, 1        # GSPLAT_TIME_FORWARD / _BACKWARD
 TRACE_MAX = 1024                          # GSPLAT_TRACE_MAX
+MAX_TOP = 64                              # GSPLAT_MAX_TOP
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GSPLAT_F32 / _BF16 / _F16
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -67,9 +69,33 @@ class Slice(ctypes.Structure):
                 ("render_workspace", _vp), ("render_workspace_bytes", _sz), ("slots", _i32)]
 
 
+class LookupMeta(ctypes.Structure):
+    """Mirror of ``gsplat_lookup_meta``."""
+
+    _fields_ = [("rows", _i64), ("num_codes", _i32), ("width", _i32), ("stride", _i64), ("dtype", _i32),
+                ("code_bytes", _i32), ("factor", ctypes.c_float)]
+
+
+class ProbsMeta(ctypes.Structure):
+    """Mirror of ``gsplat_probs_meta``."""
+
+    _fields_ = [("rows", _i64), ("num_codes", _i32), ("top", _i32), ("stride", _i64), ("dtype", _i32),
+                ("code_bytes", _i32), ("temperature", ctypes.c_float)]
+
+
+class BalanceMeta(ctypes.Structure):
+    """Mirror of ``gsplat_balance_meta``."""
+
+    _fields_ = [("rows", _i64), ("batch", _i32), ("num_codes", _i32), ("choices", _i32), ("dtype", _i32),
+                ("stride", _i64), ("code_bytes", _i32)]
+
+
 _PM = ctypes.POINTER(RasterMeta)
 _PP = ctypes.POINTER(ProjectMeta)
 _PS = ctypes.POINTER(Slice)
+_PL = ctypes.POINTER(LookupMeta)
+_PQ = ctypes.POINTER(ProbsMeta)
+_PB = ctypes.POINTER(BalanceMeta)
 
 # name -> (restype, argtypes); every name here is declared in gsplat_hip.h.
 SIGNATURES = {
@@ -121,6 +147,15 @@ SIGNATURES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _sz, _vp],
     ),
+    "gsplat_hip_lookup_forward": (ctypes.c_int, [_PL] + [_vp] * 5),
+    "gsplat_hip_lookup_backward_workspace_bytes": (_sz, [_PL]),
+    "gsplat_hip_lookup_backward": (ctypes.c_int, [_PL] + [_vp] * 7 + [_sz, _vp]),
+    "gsplat_hip_code_probs_workspace_bytes": (_sz, [_PQ]),
+    "gsplat_hip_code_probs_forward": (ctypes.c_int, [_PQ] + [_vp] * 8 + [_sz, _vp]),
+    "gsplat_hip_code_probs_backward": (ctypes.c_int, [_PQ] + [_vp] * 10),
+    "gsplat_hip_code_balance_workspace_bytes": (_sz, [_PB]),
+    "gsplat_hip_code_balance_forward": (ctypes.c_int, [_PB] + [_vp] * 8 + [_sz, _vp]),
+    "gsplat_hip_code_balance_backward": (ctypes.c_int, [_PB] + [_vp] * 8),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -644,6 +644,119 @@ int gsplat_hip_tile_render(const gsplat_raster_meta* meta,
                            void* render_workspace,
                            size_t render_workspace_bytes, void* stream);
 
+/* ---- Scenes in codes: splats that name rows of a learned codebook instead
+ * of owning their attributes.  No counterpart in the reference.
+ *
+ * Element types of codebooks and logits (and of their gradients).  Sums,
+ * softmax statistics, scales and losses are float; values are rounded to the
+ * element type once, when they are stored. */
+#define GSPLAT_F32 0
+#define GSPLAT_BF16 1
+#define GSPLAT_F16 2
+
+/* Codes are int32 or int64 (code_bytes 4 or 8).  -1: the splat has no code.
+ * Any other value outside [0, num_codes) is a mistake: nothing is read or
+ * counted for it, and the outputs that depend on it are NaN. */
+
+/* out[n] = factor * scales[n] * codebook[codes[n]], zeros without a code. */
+typedef struct gsplat_lookup_meta {
+  int64_t rows;      /* splats, 0 <= rows <= 2^29 */
+  int32_t num_codes; /* codebook rows, 1 .. 2^28 */
+  int32_t width;     /* values per row, 1 .. 2^20 */
+  int64_t stride;    /* elements between codebook rows, >= width */
+  int32_t dtype;     /* GSPLAT_F32 / _BF16 / _F16 */
+  int32_t code_bytes;
+  float factor;
+} gsplat_lookup_meta;
+
+/* scales: rows floats, or NULL for ones.  out: rows x width, contiguous. */
+int gsplat_hip_lookup_forward(const gsplat_lookup_meta* meta, const void* codes,
+                              const void* codebook, const float* scales,
+                              void* out, void* stream);
+/* g_codebook (num_codes x width, contiguous; may be NULL): sums by code in
+ * ascending splat order, the same bits on every call; every row is written.
+ * g_scales (rows floats; may be NULL).  grad_out: rows x width, contiguous.
+ * codebook is read only for g_scales.  The workspace is needed only for
+ * g_codebook.  If the sort's look-back gives up (see
+ * GSPLAT_STATUS_LOOKBACK_TIMEOUT), g_codebook is NaN. */
+size_t gsplat_hip_lookup_backward_workspace_bytes(const gsplat_lookup_meta* meta);
+int gsplat_hip_lookup_backward(const gsplat_lookup_meta* meta,
+                               const void* grad_out, const void* codes,
+                               const void* codebook, const float* scales,
+                               void* g_codebook, float* g_scales,
+                               void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Log probabilities under softmax(logits / T) over the codes.
+ *   log_probs[n]      of codes[n] (0 without a code); NULL if codes is NULL
+ *   entropy[n]        of the row's distribution
+ *   top_log_probs, top_codes [rows][top]: the likeliest codes, best first, of
+ *                     equal logits the lower code first, NaN above all; NULL
+ *                     if top = 0
+ *   row_stats[n]      two floats for the backward (may be NULL)
+ * A row whose logits are all -inf has log probabilities of -inf, entropy 0
+ * and no gradient.  A NaN or +inf makes its row NaN. */
+typedef struct gsplat_probs_meta {
+  int64_t rows;      /* 0 <= rows < 2^31 */
+  int32_t num_codes; /* 1 .. 2^28 */
+  int32_t top;       /* 0 .. min(num_codes, GSPLAT_MAX_TOP) */
+  int64_t stride;    /* elements between rows of logits, >= num_codes */
+  int32_t dtype;
+  int32_t code_bytes;
+  float temperature; /* T > 0 */
+} gsplat_probs_meta;
+#define GSPLAT_MAX_TOP 64
+
+size_t gsplat_hip_code_probs_workspace_bytes(const gsplat_probs_meta* meta);
+int gsplat_hip_code_probs_forward(const gsplat_probs_meta* meta,
+                                  const void* logits, const void* codes,
+                                  float* log_probs, float* entropy,
+                                  float* top_log_probs, int32_t* top_codes,
+                                  float* row_stats, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+/* g_log_probs, g_entropy, g_top_log_probs: each may be NULL (zero).  g_logits:
+ * rows x num_codes, contiguous. */
+int gsplat_hip_code_probs_backward(const gsplat_probs_meta* meta,
+                                   const void* logits, const void* codes,
+                                   const int32_t* top_codes,
+                                   const float* row_stats, const float* entropy,
+                                   const float* g_log_probs,
+                                   const float* g_entropy,
+                                   const float* g_top_log_probs,
+                                   void* g_logits, void* stream);
+
+/* How evenly the splats of each image use the codes:
+ *   counts[b][k]      choices of code k
+ *   mean_probs[b][k]  mean of softmax(logits) over the rows with a code
+ *   loss[b]           num_codes * sum_k counts_k / (all choices) * mean_probs_k
+ * row_stats (2 floats a row) and totals (4 ints an image: rows with a code,
+ * choices, codes out of range, 0) are kept for the backward.  No gradient
+ * passes through the counts.  An image without any code has loss 0. */
+typedef struct gsplat_balance_meta {
+  int64_t rows;      /* per image; batch * rows * choices < 2^31 */
+  int32_t batch;     /* 1 .. 65535 */
+  int32_t num_codes; /* 1 .. 2^24 */
+  int32_t choices;   /* codes per row, >= 1 */
+  int32_t dtype;
+  int64_t stride;
+  int32_t code_bytes;
+} gsplat_balance_meta;
+
+size_t gsplat_hip_code_balance_workspace_bytes(const gsplat_balance_meta* meta);
+int gsplat_hip_code_balance_forward(const gsplat_balance_meta* meta,
+                                    const void* logits, const void* codes,
+                                    float* loss, int32_t* counts,
+                                    float* mean_probs, float* row_stats,
+                                    int32_t* totals, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+/* g_loss [batch], g_mean_probs [batch][num_codes]: each may be NULL (zero). */
+int gsplat_hip_code_balance_backward(const gsplat_balance_meta* meta,
+                                     const void* logits, const int32_t* counts,
+                                     const float* row_stats,
+                                     const int32_t* totals, const float* g_loss,
+                                     const float* g_mean_probs, void* g_logits,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif
