@@ -14,54 +14,20 @@
 // images above the two-launch depth order, dense scenes to be sliced, staged
 // timing.
 #include <ATen/SavedTensorHooks.h>
-#include <ATen/core/grad_mode.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/PythonDispatcherTLS.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
-#include <hip/hip_runtime_api.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/extension.h>
 
 #include <algorithm>
 #include <array>
-#include <atomic>
 #include <chrono>
 #include <memory>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
 
-#include "../../include/gsplat_hip.h"
+#include "host_common.h"
 
+namespace gs_host {
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// The C ABI, from the library that the Python layer has loaded.
-#define GS_API(F)                       \
-  F(last_error)                         \
-  F(bin_workspace_bytes)                \
-  F(render_workspace_bytes)             \
-  F(bin_render_forward)                 \
-  F(render_forward_long)                \
-  F(render_backward)                    \
-  F(direct_workspace_bytes)             \
-  F(direct_pairs)                       \
-  F(direct_render)                      \
-  F(tile_workspace_bytes)               \
-  F(tile_render)                        \
-  F(project_forward)                    \
-  F(project_backward)                   \
-  F(project_backward_workspace_bytes)
-struct Api {
-#define GS_POINTER(name) decltype(&gsplat_hip_##name) name = nullptr;
-  GS_API(GS_POINTER)
-#undef GS_POINTER
-} api;
 
 void bind(const std::string& path) {
   void* h = dlopen(path.c_str(), RTLD_NOW | RTLD_NOLOAD);
@@ -73,72 +39,6 @@ void bind(const std::string& path) {
   GS_API(GS_RESOLVE)
 #undef GS_RESOLVE
 }
-
-void check(int rc, const char* what) {
-  if (rc == 0) return;
-  const char* msg = api.last_error();
-  TORCH_CHECK(false, what, " failed (status ", rc, "): ", msg ? msg : "");
-}
-
-hipStream_t stream_of(const Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-constexpr int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-
-const float* f32(const Tensor& t) { return t.data_ptr<float>(); }
-
-// A tensor the C++ path takes: an ordinary strided float32 tensor in device
-// memory, of a type whose operations nothing intercepts.
-bool plain(PyObject* o) {
-  if (!THPVariable_CheckExact(o)) return false;
-  const Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || !t.is_cuda() || t.scalar_type() != at::kFloat ||
-      t.layout() != at::kStrided || !t.has_storage())
-    return false;
-  const auto ks = t.key_set();
-  if (ks.has_any(c10::DispatchKeySet(
-          {c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
-           c10::DispatchKey::FuncTorchGradWrapper,
-           c10::DispatchKey::Functionalize})) ||
-      t.is_conj() || t.is_neg())
-    return false;
-  return !t._fw_grad(0).defined();
-}
-
-// Nothing that intercepts operations is active (modes, functorch, tracing).
-bool plain_context() {
-  return !c10::impl::dispatch_mode_enabled() &&
-         c10::impl::PythonDispatcherTLS::get_state() == nullptr &&
-         !c10::impl::tls_is_dispatch_key_included(
-             c10::DispatchKey::FuncTorchDynamicLayerFrontMode) &&
-         !torch::jit::tracer::isTracing();
-}
-
-// Timing of a backward call by the Python layer (_ops.set_timing): the
-// context manager _ops._timed, entered around the C-ABI call.
-std::atomic<bool> g_timed{false};
-struct Timed {
-  PyObject* cm = nullptr;
-  explicit Timed(const char* name) {
-    if (!g_timed.load(std::memory_order_relaxed)) return;
-    py::gil_scoped_acquire gil;
-    py::object ops = py::module_::import("torch_gsplat_bridge_fast._ops");
-    py::object c = ops.attr("_timed")(name);
-    c.attr("__enter__")();
-    cm = c.release().ptr();
-  }
-  ~Timed() {
-    if (cm == nullptr) return;
-    py::gil_scoped_acquire gil;
-    try {
-      py::object c = py::reinterpret_steal<py::object>(cm);
-      c.attr("__exit__")(py::none(), py::none(), py::none());
-    } catch (py::error_already_set& e) {
-      e.discard_as_unraisable("gsplat timing");
-    }
-  }
-};
 
 // Pinned words for the binnings' reports: 1024 rows of {N, status, long-range
 // flag, ready} per device, one per call.
@@ -216,10 +116,6 @@ struct Result {
   int32_t n = 0;  // N of a binned call
   bool skewed = false;  // a tiled call that is to be done by kBinned
 };
-
-Tensor bytes(int64_t n, const Tensor& like) {
-  return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false));
-}
 
 std::vector<int64_t> image_shape(const Call& c, bool rgb) {
   std::vector<int64_t> s;
@@ -727,8 +623,11 @@ py::object project(py::handle means3d, py::handle scales, py::handle quats,
 }
 
 }  // namespace
+}  // namespace gs_host
 
 PYBIND11_MODULE(_host, m) {
+  using namespace gs_host;
+  def_codes(m);
   m.def("bind", &bind);
   m.def("set_timed", [](bool on) { g_timed.store(on); });
   // Whether saved tensors go through hooks of the caller's (checkpointing,

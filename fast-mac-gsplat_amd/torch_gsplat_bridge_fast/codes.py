@@ -365,6 +365,9 @@ def lookup_codes(codes: Tensor, codebook: Tensor, scales: Optional[Tensor] = Non
     codes [...] (-1: zeros), codebook [K,D], scales float32 of the codes' shape or None.  The result has
     the codebook's type.  Gradients flow to codebook and scales; a row of the codebook's gradient is the
     sum over the splats that name it, in their order."""
+    out = _lib.host().lookup_codes(codes, codebook, scales, factor)
+    if out is not None:
+        return out
     _check_lookup(codes, codebook, scales)
     return _lookup(codes, codebook, scales, float(factor))
 
@@ -377,6 +380,9 @@ def code_log_probs(logits: Tensor, codes: Optional[Tensor] = None, top: int = 0,
     first, and their log probabilities; among equal logits the lower code comes first, NaN ranks above
     everything.  A splat whose logits are all -inf has log probabilities of -inf, entropy 0 and no
     gradient.  Gradients flow from log_probs, entropy and top_log_probs to logits."""
+    out = _lib.host().code_log_probs(logits, codes, top, temperature)
+    if out is not None:
+        return CodeLogProbs(*out)
     _check_probs(logits, codes, top, temperature)
     log_probs, entropy, top_log_probs, top_codes, _ = _probs(logits, codes, int(top), float(temperature))
     return CodeLogProbs(None if codes is None else log_probs, entropy, top_log_probs if top else None,
@@ -391,6 +397,9 @@ def code_balance(logits: Tensor, codes: Tensor) -> CodeBalance:
     code.  loss = K * sum_k counts_k / (all choices) * mean_probs_k: 1 when both are even, larger the more
     they agree on a few codes; 0 for an image without any code.  Gradients flow from loss and mean_probs to
     logits (the counts are constants)."""
+    out = _lib.host().code_balance(logits, codes)
+    if out is not None:
+        return CodeBalance(*out)
     _check_balance(logits, codes)
     loss, counts, mean_probs, _, _ = _balance(logits, codes)
     return CodeBalance(loss, counts, mean_probs)

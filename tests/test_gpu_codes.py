@@ -534,3 +534,30 @@ def test_operators(gpu):
     both(lambda b, s: [gs.lookup_codes(codes, b, s, 2.0)], lambda b, s: [ops.lookup_codes(codes, b, s, 2.0)], book, s)
     both(lambda x: list(gs.code_log_probs(x, codes, top=2)), lambda x: list(ops.code_log_probs(x, codes, 2, 1.0)[:4]), x)
     both(lambda x: list(gs.code_balance(x, codes)), lambda x: list(ops.code_balance(x, codes)[:3]), x)
+
+
+def test_differentiated_once(gpu):
+    """A gradient taken under create_graph says so when it is to be differentiated again."""
+    x = torch.randn(20, 30, device=gpu, requires_grad=True)
+    codes = torch.randint(0, 30, (20,), device=gpu)
+    book = torch.randn(30, 4, device=gpu, requires_grad=True)
+    for y, leaf in ((gs.lookup_codes(codes, book).square().sum(), book),
+                    (gs.code_log_probs(x, codes, top=1).log_probs.square().sum(), x),
+                    (gs.code_balance(x, codes).loss, x)):
+        g, = torch.autograd.grad(y, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            torch.autograd.grad(g.sum(), leaf)
+
+
+def test_inputs_that_are_not_plain(gpu):
+    """Tensor subclasses take the operators and get the same values."""
+    class Sub(torch.Tensor):
+        pass
+
+    x, codes = torch.randn(20, 30, device=gpu), torch.randint(0, 30, (20,), device=gpu)
+    book = torch.randn(30, 4, device=gpu)
+    assert torch.equal(gs.lookup_codes(codes, book.as_subclass(Sub)).as_subclass(torch.Tensor), gs.lookup_codes(codes, book))
+    a, b = gs.code_log_probs(x.as_subclass(Sub), codes, top=2), gs.code_log_probs(x, codes, top=2)
+    assert all(torch.equal(torch.Tensor(u) if u.is_floating_point() else u, v) for u, v in zip(a, b))
+    a, b = gs.code_balance(x.as_subclass(Sub), codes), gs.code_balance(x, codes)
+    assert torch.equal(a.counts, b.counts) and torch.equal(torch.Tensor(a.mean_probs), b.mean_probs)
