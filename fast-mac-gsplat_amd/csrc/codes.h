@@ -28,23 +28,102 @@ struct Codes {
   }
 };
 
-// e^z with denormal results kept (the hardware's base-2 exponential flushes
-// them): probabilities of gradients go down to the type's smallest values.
-__device__ __forceinline__ float exp_full(float z) {
-  return exp2f(z * 1.44269504088896340736f);
-}
+// 2^t with denormal results kept (the hardware's base-2 exponential flushes
+// them): gradients go down to the type's smallest values.
+__device__ __forceinline__ float exp2_full(float t) { return exp2f(t); }
+// The hardware's exponential and logarithm: results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float t) { return __builtin_amdgcn_exp2f(t); }
+__device__ __forceinline__ float log2_fast(float t) { return __builtin_amdgcn_logf(t); }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// 16 bytes of elements, loaded and stored at any multiple of the element size
+// (rows of logits start anywhere; the memory pipeline takes dwordx4 accesses
+// at any address).
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T>
+using vec_t = T __attribute__((ext_vector_type(16 / sizeof(T))));
+
+template <typename T>
+__device__ __forceinline__ vec_t<T> load_vec(const T* p) {
+  vec_t<T> v;
+  __builtin_memcpy(&v, p, 16);
   return v;
 }
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, vec_t<T> v) {
+  __builtin_memcpy(p, &v, 16);
+}
 
-__device__ __forceinline__ float wave_max(float v) {
+// Elements i .. i + kVec - 1 of a row of n, `fill` past its end.
+template <typename T>
+__device__ __forceinline__ vec_t<T> load_part(const T* row, int i, int n, T fill) {
+  if (i + kVec<T> <= n) return load_vec(row + i);
+  vec_t<T> v;
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  for (int j = 0; j < kVec<T>; ++j) v[j] = i + j < n ? row[i + j] : fill;
   return v;
 }
+template <typename T>
+__device__ __forceinline__ void store_part(T* row, int i, int n, vec_t<T> v) {
+  if (i + kVec<T> <= n) {
+    store_vec(row + i, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j)
+    if (i + j < n) row[i + j] = v[j];
+}
+
+// Reductions over teams of L consecutive lanes (a power of two up to the
+// wavefront); every lane gets the result, the same bits in each.  Partners: in
+// the quad by quad_perm, in eight and sixteen lanes by the mirrors (the lanes
+// of a quad are equal by then), across 16 and 32 lanes by the row swaps.
+template <int Ctrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, Ctrl, 0xf, 0xf, false);
+}
+template <int L, typename Op>
+__device__ __forceinline__ uint32_t team_reduce(uint32_t v, Op op) {
+  if constexpr (L >= 2) v = op(v, dpp<0xB1>(v));   // quad_perm 1,0,3,2
+  if constexpr (L >= 4) v = op(v, dpp<0x4E>(v));   // quad_perm 2,3,0,1
+  if constexpr (L >= 8) v = op(v, dpp<0x141>(v));  // row_half_mirror
+  if constexpr (L >= 16) v = op(v, dpp<0x140>(v)); // row_mirror
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float team_max(float v) {
+  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+template <int L>
+__device__ __forceinline__ float team_sum(float v) {
+  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+template <int L>
+__device__ __forceinline__ uint32_t team_min(uint32_t v) {
+  return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+template <int L>
+__device__ __forceinline__ uint32_t team_umax(uint32_t v) {
+  return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
+__device__ __forceinline__ float wave_sum(float v) { return team_sum<64>(v); }
+__device__ __forceinline__ float wave_max(float v) { return team_max<64>(v); }
 
 // The same over a workgroup of W wavefronts (red: W floats of LDS; every
 // thread gets the result).
@@ -57,18 +136,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   float r = red[0];
 #pragma unroll
   for (int w = 1; w < W; ++w) r += red[w];
-  return r;
-}
-
-template <int W>
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = red[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) r = fmaxf(r, red[w]);
   return r;
 }
 
