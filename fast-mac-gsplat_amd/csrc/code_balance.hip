@@ -9,8 +9,9 @@
 // p = 0.  No gradient passes through the counts.  A code outside [-1, K) is
 // not counted and makes its image's loss NaN.
 //
-// Sums over rows are taken in a fixed order (chunks of rows, then the chunks),
-// counts are integers: the same inputs give the same bits.
+// Sums over rows are taken in a fixed order (rows of a team, teams of a
+// workgroup, workgroups), counts are integers: the same inputs give the same
+// bits.
 #include <algorithm>
 
 #include "codes.h"
@@ -18,178 +19,617 @@
 namespace gs {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kChunk = 256;  // rows whose probabilities one workgroup adds up
+// A team reads a row once and holds it in registers: TL lanes of one wavefront
+// (W = 1), or W wavefronts.  A thread holds R vectors, at most 16 elements, of
+// the row at hand, its probabilities and (forward) its columns' sums or
+// (backward) its columns' a; the next row is loaded while this one is worked
+// on.
+template <typename T, int TL, int W, int R>
+struct Team {
+  static constexpr int V = kVec<T>;
+  static constexpr int kThreads = W > 1 ? 64 * W : 256;
+  static constexpr int kTeams = kThreads / (TL * W);  // per workgroup
+  static constexpr int kColumns = TL * W * V * R;
+  static __device__ __forceinline__ int team() { return threadIdx.x / (TL * W); }
+  static __device__ __forceinline__ int member() { return threadIdx.x & (TL * W - 1); }
+  static __device__ __forceinline__ int column(int r) { return (r * TL * W + member()) * V; }
+  static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int K) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      x[r] = load_part<T>(row, column(r), K, static_cast<T>(-INFINITY));
+  }
+};
 
-// One wavefront per row: stats = {max, 1 / sum}, {., 0} for a row that takes
-// no part; the row's choices are counted (counts and totals zero on entry).
-// totals[b] = {rows that take part, choices, bad codes, 0}
-template <typename T>
-__global__ __launch_bounds__(kThreads) void balance_rows_kernel(
-    BalanceParams P, const T* __restrict__ logits, int32_t* __restrict__ counts,
-    float2* __restrict__ stats, int32_t* __restrict__ totals) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (r >= P.rows * P.batch) return;
-  const int b = (int)(r / P.rows);
-  const T* row = logits + r * P.stride;
-  float m = -INFINITY;
-  for (int i = lane; i < P.K; i += 64) m = fmaxf(m, to_float(row[i]));
-  m = wave_max(m);
-  if (m == -INFINITY) m = 0.0f;
+// What the workgroups of the row pass leave: for image b and workgroup i
+// (blocks of them per image) sums[(b * blocks + i) * K + k], and counts and
+// totals likewise for i < count_blocks.
+struct Partials {
+  int blocks, count_blocks;
+  float* sums;
+  int32_t* counts;
+  int4* totals;  // rows that take part, choices, bad codes
+  float* loss;   // [batch][column groups]
+  uint32_t* tickets;  // [batch], zeroed by the row pass
+};
+
+// The choices of a row (kept by the lanes of a wavefront): counts them.
+struct Choices {
+  int given = 0, bad = 0;
+  __device__ __forceinline__ void count(int c, int32_t* hist) {
+    if (c >= 0) {
+      ++given;
+      if (hist) atomicAdd(&hist[c], 1);
+    } else if (c == kBadCode) {
+      ++bad;
+    }
+  }
+};
+
+template <typename T, int TL, int W, int R>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
+    BalanceParams P, const T* __restrict__ logits, float2* __restrict__ stats,
+    Partials out) {
+  using G = Team<T, TL, W, R>;
+  constexpr int V = G::V;
+  extern __shared__ int32_t lds[];  // K counts, then (teams > 1) K sums
+  __shared__ float2 slots[2][W];
+  __shared__ int sum4[3];
+  int32_t* hist = lds;
+  float* sums = reinterpret_cast<float*>(lds + P.K);
+  const int b = blockIdx.y;
+  const int64_t per = (P.rows + out.blocks - 1) / out.blocks;
+  const int64_t first = blockIdx.x * per;
+  const int64_t count = max((int64_t)0, min(per, P.rows - first));
+  for (int k = threadIdx.x; k < P.K; k += G::kThreads) hist[k] = 0;
+  if (threadIdx.x < 3) sum4[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) out.tickets[b] = 0;
+  __syncthreads();
+
+  const float c = kLog2e;
+  const int lane = threadIdx.x & (TL - 1), w = W > 1 ? threadIdx.x >> 6 : 0;
+  const int S = P.choices;
+  float acc[R * V];
+#pragma unroll
+  for (int j = 0; j < R * V; ++j) acc[j] = 0.0f;
+  int took = 0, given = 0, bad = 0;
+  vec_t<T> x[R], next[R];
+  const int64_t base_row = b * P.rows + first;
+  auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
+  int64_t i = G::team();
+  int code = kNoCode, code_next = kNoCode;
+  if (count > 0) {
+    G::load(x, logits + row_of(i) * P.stride, P.K);
+    if (lane < S) code = P.codes.at(row_of(i) * S + lane, P.K);
+  }
+  // (every team makes the same number of turns; those past the rows count nothing)
+  for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
+    const int64_t r0 = row_of(i);
+    const bool here = i < count;
+    if ((turn + 1) * G::kTeams < count) {
+      const int64_t rn = row_of(i + G::kTeams);
+      G::load(next, logits + rn * P.stride, P.K);
+      code_next = lane < S ? P.codes.at(rn * S + lane, P.K) : kNoCode;
+    }
+    Choices mine;
+    if (here) {
+      int32_t* h = w == 0 ? hist : nullptr;
+      if (lane < S) mine.count(code, h);
+      for (int j = lane + TL; j < S; j += TL) mine.count(P.codes.at(r0 * S + j, P.K), h);
+    }
+    const bool part = team_umax<TL>(mine.given) != 0;
+    given += mine.given;
+    bad += mine.bad;
+    took += part && lane == 0;
+
+    float m = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) m = fmaxf(m, to_float(x[r][v]));
+    m = team_max<TL>(m);
+    float base = m == -INFINITY ? 0.0f : m;
+    float e[R * V], s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        e[r * V + v] = exp2_fast((to_float(x[r][v]) - base) * c);
+        s += e[r * V + v];
+      }
+    s = team_sum<TL>(s);
+    float scale = 1.0f;
+    if constexpr (W > 1) {  // (two sets of slots: one barrier a row)
+      float2* slot = slots[turn & 1];
+      if (lane == 0) slot[w] = make_float2(m, s);
+      __syncthreads();
+      float all = slot[0].x;
+#pragma unroll
+      for (int j = 1; j < W; ++j) all = fmaxf(all, slot[j].x);
+      const float b_all = all == -INFINITY ? 0.0f : all;
+      s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        s += slot[j].y * exp2_fast(fmaxf((slot[j].x - b_all) * c, -1000.0f));
+      scale = exp2_fast(fmaxf((m - b_all) * c, -1000.0f));
+      base = b_all;
+    }
+    const float inv = part && s != 0.0f ? 1.0f / s : 0.0f;
+    if (here && G::member() == 0) stats[r0] = make_float2(base, inv);
+    if (here && inv != 0.0f) {
+      const float f = scale * inv;
+#pragma unroll
+      for (int j = 0; j < R * V; ++j) acc[j] = __builtin_fmaf(e[j], f, acc[j]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = next[r];
+    code = code_next;
+  }
+
+  // rows, choices and bad codes of the workgroup (wavefront 0 of a wide team)
+  if (W == 1 || w == 0) {
+    given = wave_isum(given);
+    bad = wave_isum(bad);
+    took = wave_isum(took);
+    if ((threadIdx.x & 63) == 0) {
+      atomicAdd(&sum4[0], took);
+      atomicAdd(&sum4[1], given);
+      atomicAdd(&sum4[2], bad);
+    }
+  }
+  const int64_t at = (int64_t)b * out.blocks + blockIdx.x;
+  if constexpr (G::kTeams > 1) {
+    // teams of a wavefront, then the wavefronts one after another
+    if constexpr (TL < 64)
+#pragma unroll
+      for (int j = 0; j < R * V; ++j)
+#pragma unroll
+        for (int d = TL; d < 64; d <<= 1) acc[j] += __shfl_xor(acc[j], d, 64);
+    const int wave = threadIdx.x >> 6;
+    for (int q = 0; q < G::kThreads / 64; ++q) {
+      if (wave == q && (threadIdx.x & 63) < TL)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const int k = G::column(r) + v;
+            if (k < P.K) sums[k] = q == 0 ? acc[r * V + v] : sums[k] + acc[r * V + v];
+          }
+      __syncthreads();
+    }
+    for (int k = threadIdx.x; k < P.K; k += G::kThreads) out.sums[at * P.K + k] = sums[k];
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int k = G::column(r) + v;
+        if (k < P.K) out.sums[at * P.K + k] = acc[r * V + v];
+      }
+  }
+  for (int k = threadIdx.x; k < P.K; k += G::kThreads) out.counts[at * P.K + k] = hist[k];
+  if (threadIdx.x == 0) out.totals[at] = make_int4(sum4[0], sum4[1], sum4[2], 0);
+}
+
+// ---- the workgroups' sums joined: 64 columns of an image per workgroup, 16
+// wavefronts that each take every 16th of them.  The image's last workgroup
+// adds up the loss.
+
+constexpr int kJoinWaves = 16;
+
+__global__ __launch_bounds__(64 * kJoinWaves) void balance_join_kernel(
+    BalanceParams P, Partials in, float* __restrict__ loss,
+    int32_t* __restrict__ counts, float* __restrict__ mean,
+    int4* __restrict__ totals) {
+  __shared__ float sums[kJoinWaves][64];
+  __shared__ int nums[kJoinWaves][64];
+  __shared__ int all[3];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = blockIdx.y;
+  const int k = blockIdx.x * 64 + lane;
+  if (threadIdx.x < 3) all[threadIdx.x] = 0;
+  __syncthreads();
+  int4 t = make_int4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < in.count_blocks; i += 64 * kJoinWaves) {
+    const int4 q = in.totals[(int64_t)b * in.count_blocks + i];
+    t.x += q.x;
+    t.y += q.y;
+    t.z += q.z;
+  }
+  if (t.x) atomicAdd(&all[0], t.x);
+  if (t.y) atomicAdd(&all[1], t.y);
+  if (t.z) atomicAdd(&all[2], t.z);
   float s = 0.0f;
-  for (int i = lane; i < P.K; i += 64) s += __expf(to_float(row[i]) - m);
-  s = wave_sum(s);
-  if (lane == 0) {
-    int given = 0, bad = 0;
-    for (int j = 0; j < P.choices; ++j) {
-      const int c = P.codes.at(r * P.choices + j, P.K);
-      if (c >= 0) {
-        ++given;
-        atomicAdd(&counts[(int64_t)b * P.K + c], 1);
-      } else if (c == kBadCode) {
-        ++bad;
+  int n = 0;
+  if (k < P.K) {
+    const float* ps = in.sums + (int64_t)b * in.blocks * P.K + k;
+#pragma unroll 4
+    for (int i = w; i < in.blocks; i += kJoinWaves) s += ps[(int64_t)i * P.K];
+    const int32_t* pn = in.counts + (int64_t)b * in.count_blocks * P.K + k;
+#pragma unroll 4
+    for (int i = w; i < in.count_blocks; i += kJoinWaves) n += pn[(int64_t)i * P.K];
+  }
+  sums[w][lane] = s;
+  nums[w][lane] = n;
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int j = 1; j < kJoinWaves; ++j) {
+    s += sums[j][lane];
+    n += nums[j][lane];
+  }
+  const float mu = s / (float)max(all[0], 1);
+  if (k < P.K) {
+    counts[(int64_t)b * P.K + k] = n;
+    mean[(int64_t)b * P.K + k] = mu;
+  }
+  if (blockIdx.x == 0 && lane == 0) totals[b] = make_int4(all[0], all[1], all[2], 0);
+  // (an image with nothing counted: 0, whatever the means are)
+  float l = wave_sum(n ? (float)n * mu : 0.0f);
+  const float factor = (float)P.K / (float)max(all[1], 1);
+  if (gridDim.x > 1) {
+    float* mine = in.loss + (int64_t)b * gridDim.x;
+    uint32_t ticket = 0;
+    if (lane == 0) {
+      __hip_atomic_store(&mine[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      ticket = __hip_atomic_fetch_add(&in.tickets[b], 1u, __ATOMIC_ACQ_REL,
+                                      __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if ((uint32_t)__builtin_amdgcn_readfirstlane((int)ticket) != gridDim.x - 1) return;
+    l = 0.0f;
+    for (unsigned i = lane; i < gridDim.x; i += 64)
+      l += __hip_atomic_load(&mine[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    l = wave_sum(l);
+  }
+  if (lane == 0) loss[b] = all[2] ? __builtin_nanf("") : l * factor;
+}
+
+// ---- backward
+
+template <typename T, int TL, int W, int R>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
+    BalanceParams P, const T* __restrict__ logits,
+    const int32_t* __restrict__ counts, const float2* __restrict__ stats,
+    const int4* __restrict__ totals, const float* __restrict__ g_loss,
+    const float* __restrict__ g_mean, T* __restrict__ g_logits) {
+  using G = Team<T, TL, W, R>;
+  constexpr int V = G::V;
+  __shared__ float slots[2][W];
+  const int b = blockIdx.y;
+  const int64_t per = (P.rows + gridDim.x - 1) / gridDim.x;
+  const int64_t first = blockIdx.x * per;
+  const int64_t count = min(per, P.rows - first);
+  if (count <= 0) return;
+  const int lane = threadIdx.x & (TL - 1), w = W > 1 ? threadIdx.x >> 6 : 0;
+  const int4 tot = totals[b];
+  const float per_row = 1.0f / (float)max(tot.x, 1);
+  const float per_count = g_loss ? g_loss[b] * ((float)P.K / (float)max(tot.y, 1)) : 0.0f;
+  float a[R * V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int k = G::column(r) + v;
+      float f = 0.0f;
+      if (k < P.K) {
+        f = per_count * (float)counts[(int64_t)b * P.K + k];
+        if (g_mean) f += g_mean[(int64_t)b * P.K + k];
+      }
+      a[r * V + v] = f;
+    }
+  const int64_t base_row = b * P.rows + first;
+  auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
+  int64_t i = G::team();
+  vec_t<T> x[R], next[R];
+  G::load(x, logits + row_of(i) * P.stride, P.K);
+  float2 st = stats[row_of(i)], st_next = st;
+  for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
+    const int64_t r0 = row_of(i);
+    if ((turn + 1) * G::kTeams < count) {
+      const int64_t rn = row_of(i + G::kTeams);
+      G::load(next, logits + rn * P.stride, P.K);
+      st_next = stats[rn];
+    }
+    float p[R * V], dot = 0.0f;
+    const bool some = st.y != 0.0f;  // (else the row has no probabilities)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int j = r * V + v;
+        p[j] = some ? exp2_full((to_float(x[r][v]) - st.x) * kLog2e) * st.y : 0.0f;
+        dot = __builtin_fmaf(p[j], a[j], dot);
+      }
+    dot = team_sum<TL>(dot);
+    if constexpr (W > 1) {
+      float* slot = slots[turn & 1];
+      if (lane == 0) slot[w] = dot;
+      __syncthreads();
+      dot = slot[0];
+#pragma unroll
+      for (int j = 1; j < W; ++j) dot += slot[j];
+    }
+    if (i < count) {
+      T* out = g_logits + r0 * P.K;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        vec_t<T> o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int j = r * V + v;
+          o[v] = static_cast<T>(p[j] * (a[j] - dot) * per_row);
+        }
+        store_part<T>(out, G::column(r), P.K, o);
       }
     }
-    if (given) {
-      atomicAdd(&totals[4 * b], 1);
-      atomicAdd(&totals[4 * b + 1], given);
-    }
-    if (bad) atomicAdd(&totals[4 * b + 2], bad);
-    stats[r] = make_float2(m, given && s != 0.0f ? 1.0f / s : 0.0f);
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = next[r];
+    st = st_next;
   }
 }
 
+// ---- codebooks above 16384: a row does not fit a workgroup's registers, and
+// is read twice in each direction
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+
 __device__ __forceinline__ float prob(float x, float2 st) {
-  return st.y == 0.0f ? 0.0f : __expf(x - st.x) * st.y;
+  return st.y == 0.0f ? 0.0f : exp2_full((x - st.x) * kLog2e) * st.y;
 }
 
+// A workgroup per row.  The only counts and totals of an image: zero on entry.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void balance_long_rows_kernel(
+    BalanceParams P, const T* __restrict__ logits, float2* __restrict__ stats,
+    Partials out) {
+  __shared__ float2 slots[kWaves];
+  const int64_t r = blockIdx.x;
+  const int b = (int)(r / P.rows);
+  const T* row = logits + r * P.stride;
+  // online: (m, s) of this thread's elements
+  float m = -INFINITY, s = 0.0f;
+  for (int i = threadIdx.x * kVec<T>; i < P.K; i += kThreads * kVec<T>) {
+    const vec_t<T> x = load_part<T>(row, i, P.K, static_cast<T>(-INFINITY));
+    float top = m;
+#pragma unroll
+    for (int v = 0; v < kVec<T>; ++v) top = fmaxf(top, to_float(x[v]));
+    const float base = top == -INFINITY ? 0.0f : top;
+    s *= exp2_fast(fmaxf((m - base) * kLog2e, -1000.0f));
+#pragma unroll
+    for (int v = 0; v < kVec<T>; ++v) s += exp2_fast((to_float(x[v]) - base) * kLog2e);
+    m = top;
+  }
+  const float wm = wave_max(m), wb = wm == -INFINITY ? 0.0f : wm;
+  s = wave_sum(s * exp2_fast(fmaxf((m - wb) * kLog2e, -1000.0f)));
+  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = make_float2(wm, s);
+  Choices mine;
+  for (int j = threadIdx.x; j < P.choices; j += kThreads)
+    mine.count(P.codes.at(r * P.choices + j, P.K), out.counts + (int64_t)b * P.K);
+  if (mine.given) atomicAdd(&out.totals[b].y, mine.given);
+  if (mine.bad) atomicAdd(&out.totals[b].z, mine.bad);
+  const bool part = __syncthreads_or(mine.given);
+  if (threadIdx.x != 0) return;
+  m = slots[0].x;
+  for (int j = 1; j < kWaves; ++j) m = fmaxf(m, slots[j].x);
+  const float base = m == -INFINITY ? 0.0f : m;
+  s = 0.0f;
+  for (int j = 0; j < kWaves; ++j)
+    s += slots[j].y * exp2_fast(fmaxf((slots[j].x - base) * kLog2e, -1000.0f));
+  stats[r] = make_float2(base, part && s != 0.0f ? 1.0f / s : 0.0f);
+  if (part) atomicAdd(&out.totals[b].x, 1);
+}
+
+// Sums of columns over a chunk of an image's rows.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void balance_columns_kernel(
     BalanceParams P, const T* __restrict__ logits,
-    const float2* __restrict__ stats, int chunks, float* __restrict__ partials) {
-  const int k = blockIdx.x * kThreads + threadIdx.x;
-  const int chunk = blockIdx.y, b = blockIdx.z;
+    const float2* __restrict__ stats, Partials out) {
+  const int k = (blockIdx.x * kThreads + threadIdx.x) * kVec<T>;
+  const int b = blockIdx.z;
   if (k >= P.K) return;
-  const int64_t end = min((int64_t)(chunk + 1) * kChunk, P.rows);
-  float acc = 0.0f;
-  for (int64_t n = (int64_t)chunk * kChunk; n < end; ++n) {
+  const int64_t per = (P.rows + out.blocks - 1) / out.blocks;
+  const int64_t first = blockIdx.y * per, end = min(first + per, P.rows);
+  float acc[kVec<T>];
+#pragma unroll
+  for (int v = 0; v < kVec<T>; ++v) acc[v] = 0.0f;
+  for (int64_t n = first; n < end; ++n) {
     const int64_t r = b * P.rows + n;
-    acc += prob(to_float(logits[r * P.stride + k]), stats[r]);
+    const float2 st = stats[r];
+    const vec_t<T> x = load_part<T>(logits + r * P.stride, k, P.K, static_cast<T>(-INFINITY));
+#pragma unroll
+    for (int v = 0; v < kVec<T>; ++v) acc[v] += prob(to_float(x[v]), st);
   }
-  partials[((int64_t)b * chunks + chunk) * P.K + k] = acc;
-}
-
-__global__ __launch_bounds__(kThreads) void balance_mean_kernel(
-    BalanceParams P, const float* __restrict__ partials, int chunks,
-    const int32_t* __restrict__ totals, float* __restrict__ mean) {
-  const int k = blockIdx.x * kThreads + threadIdx.x, b = blockIdx.y;
-  if (k >= P.K) return;
-  float acc = 0.0f;
-  for (int c = 0; c < chunks; ++c)
-    acc += partials[((int64_t)b * chunks + c) * P.K + k];
-  mean[(int64_t)b * P.K + k] = acc / (float)max(totals[4 * b], 1);
-}
-
-__global__ __launch_bounds__(kThreads) void balance_loss_kernel(
-    BalanceParams P, const float* __restrict__ mean,
-    const int32_t* __restrict__ counts, const int32_t* __restrict__ totals,
-    float* __restrict__ loss) {
-  __shared__ float red[kWaves];
-  const int b = blockIdx.x;
-  float acc = 0.0f;
-  for (int k = threadIdx.x; k < P.K; k += kThreads)
-    acc += (float)counts[(int64_t)b * P.K + k] * mean[(int64_t)b * P.K + k];
-  acc = block_sum<kWaves>(acc, red);
-  if (threadIdx.x == 0) {
-    acc *= (float)P.K / (float)max(totals[4 * b + 1], 1);
-    loss[b] = totals[4 * b + 2] ? __builtin_nanf("") : acc;
-  }
+  float* to = out.sums + ((int64_t)b * out.blocks + blockIdx.y) * P.K;
+#pragma unroll
+  for (int v = 0; v < kVec<T>; ++v)
+    if (k + v < P.K) to[k + v] = acc[v];
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void balance_bwd_kernel(
+__global__ __launch_bounds__(kThreads) void balance_long_bwd_kernel(
     BalanceParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ counts, const float2* __restrict__ stats,
-    const int32_t* __restrict__ totals, const float* __restrict__ g_loss,
+    const int4* __restrict__ totals, const float* __restrict__ g_loss,
     const float* __restrict__ g_mean, T* __restrict__ g_logits) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (r >= P.rows * P.batch) return;
+  __shared__ float red[kWaves];
+  const int64_t r = blockIdx.x;
   const int b = (int)(r / P.rows);
   const T* row = logits + r * P.stride;
   T* out = g_logits + r * P.K;
   const float2 st = stats[r];
-  const float per_row = 1.0f / (float)max(totals[4 * b], 1);
-  const float per_count =
-      g_loss ? g_loss[b] * ((float)P.K / (float)max(totals[4 * b + 1], 1)) : 0.0f;
+  const int4 tot = totals[b];
+  const float per_row = 1.0f / (float)max(tot.x, 1);
+  const float per_count = g_loss ? g_loss[b] * ((float)P.K / (float)max(tot.y, 1)) : 0.0f;
   auto a_of = [&](int k) {
+    if (k >= P.K) return 0.0f;
     const float f = per_count * (float)counts[(int64_t)b * P.K + k];
     return g_mean ? f + g_mean[(int64_t)b * P.K + k] : f;
   };
   float dot = 0.0f;
-  for (int k = lane; k < P.K; k += 64) dot += prob(to_float(row[k]), st) * a_of(k);
-  dot = wave_sum(dot);
-  for (int k = lane; k < P.K; k += 64) {
-    const float p = prob(to_float(row[k]), st);
-    out[k] = static_cast<T>(p * (a_of(k) - dot) * per_row);
+  for (int k = threadIdx.x * kVec<T>; k < P.K; k += kThreads * kVec<T>) {
+    const vec_t<T> x = load_part<T>(row, k, P.K, static_cast<T>(-INFINITY));
+#pragma unroll
+    for (int v = 0; v < kVec<T>; ++v)
+      dot = __builtin_fmaf(prob(to_float(x[v]), st), a_of(k + v), dot);
+  }
+  dot = block_sum<kWaves>(dot, red);
+  for (int k = threadIdx.x * kVec<T>; k < P.K; k += kThreads * kVec<T>) {
+    const vec_t<T> x = load_part<T>(row, k, P.K, static_cast<T>(-INFINITY));
+    vec_t<T> o;
+#pragma unroll
+    for (int v = 0; v < kVec<T>; ++v)
+      o[v] = static_cast<T>(prob(to_float(x[v]), st) * (a_of(k + v) - dot) * per_row);
+    store_part<T>(out, k, P.K, o);
   }
 }
 
-int chunks_of(const BalanceParams& P) { return (int)((P.rows + kChunk - 1) / kChunk); }
+// ---- host
+
+constexpr int kLongest = 16384;  // codes of a row that a workgroup holds
+
+// Workgroups per image of the row pass.  A workgroup leaves 8 bytes per code,
+// so it takes at least 32 bytes of every column (a quarter of that again); 1024
+// workgroups in all keep the GPU busy.
+int blocks_of(const BalanceParams& P) {
+  if (P.rows == 0) return 1;
+  if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
+  const int64_t least = P.dtype == GSPLAT_F32 ? 8 : 16;
+  const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 256 : P.K > 4096 ? 512 : 1024) / P.batch);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, P.rows / least));
+}
+
+int column_groups(const BalanceParams& P) { return (P.K + 63) / 64; }
+
+struct Layout {
+  size_t sums, counts, totals, loss, tickets, total;
+};
+Layout layout(const BalanceParams& P) {
+  const size_t blocks = (size_t)blocks_of(P) * P.batch;
+  const size_t count_blocks = P.K > kLongest ? (size_t)P.batch : blocks;
+  Layout L{};
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += align_up(bytes, 256);
+    return at;
+  };
+  L.sums = take(blocks * P.K * 4);
+  L.counts = take(count_blocks * P.K * 4);
+  L.totals = take(count_blocks * sizeof(int4));
+  L.loss = take((size_t)P.batch * column_groups(P) * 4);
+  L.tickets = take((size_t)P.batch * 4);
+  L.total = off;
+  return L;
+}
+
+// The kernel for rows of K codes: CALL(TL, W, R).
+#define GS_TEAMS(CALL)                                              \
+  if (vecs <= 2) CALL(2, 1, 1);                                     \
+  if (vecs <= 4) CALL(4, 1, 1);                                     \
+  if (vecs <= 8) CALL(8, 1, 1);                                     \
+  if (vecs <= 16) CALL(16, 1, 1);                                   \
+  if (vecs <= 32) CALL(32, 1, 1);                                   \
+  if (vecs <= 64) CALL(64, 1, 1);                                   \
+  if (vecs <= 128) CALL(64, 1, 2);                                  \
+  constexpr int kR = 16 / kVec<T>;                                  \
+  if (vecs <= 64 * kR) CALL(64, 1, kR);                             \
+  if (vecs <= 128 * kR) CALL(64, 2, kR);                            \
+  if (vecs <= 256 * kR) CALL(64, 4, kR);                            \
+  if (vecs <= 512 * kR) CALL(64, 8, kR);                            \
+  CALL(64, 16, kR);
+
+template <typename T>
+int rows_of(const BalanceParams& P, const T* x, float2* stats, const Partials& w,
+            hipStream_t stream) {
+  const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
+#define GS_ROWS(TL, W, R)                                                     \
+  {                                                                           \
+    using G = Team<T, TL, W, R>;                                              \
+    launch_traced("balance_rows_kernel", (balance_rows_kernel<T, TL, W, R>),  \
+                  dim3((unsigned)w.blocks, (unsigned)P.batch), dim3(G::kThreads), \
+                  (size_t)P.K * (G::kTeams > 1 ? 8 : 4), stream, P, x, stats, w); \
+    return check_launch("balance_rows_kernel");                               \
+  }
+  GS_TEAMS(GS_ROWS)
+#undef GS_ROWS
+}
 
 template <typename T>
 int forward_of(const BalanceParams& P, const void* logits, float* loss,
                int32_t* counts, float* mean, float2* stats, int32_t* totals,
-               float* partials, hipStream_t stream) {
-  const int64_t rows = P.rows * P.batch;
-  const int chunks = chunks_of(P);
+               char* ws, hipStream_t stream) {
   const T* x = static_cast<const T*>(logits);
-  int rc = launch_zero2(reinterpret_cast<uint32_t*>(counts), (int64_t)P.batch * P.K,
-                        reinterpret_cast<uint32_t*>(totals), 4 * (int64_t)P.batch,
-                        stream);
-  if (rc) return rc;
-  const unsigned cols = (unsigned)((P.K + kThreads - 1) / kThreads);
-  if (rows > 0) {
-    launch_traced("balance_rows_kernel", (balance_rows_kernel<T>),
-                  dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0,
-                  stream, P, x, counts, stats, totals);
-    rc = check_launch("balance_rows_kernel");
+  const Layout L = layout(P);
+  const bool is_long = P.K > kLongest;
+  Partials w{blocks_of(P), is_long ? 1 : blocks_of(P),
+             reinterpret_cast<float*>(ws + L.sums),
+             reinterpret_cast<int32_t*>(ws + L.counts),
+             reinterpret_cast<int4*>(ws + L.totals),
+             reinterpret_cast<float*>(ws + L.loss),
+             reinterpret_cast<uint32_t*>(ws + L.tickets)};
+  int rc;
+  if (!is_long) {
+    rc = rows_of<T>(P, x, stats, w, stream);
+  } else {
+    // (one launch zeroes counts, totals, the loss' parts and the tickets; the
+    // sums of no rows are zeroed too)
+    rc = launch_zero_u32(reinterpret_cast<uint32_t*>(ws + (P.rows ? L.counts : L.sums)),
+                         (int64_t)(L.total - (P.rows ? L.counts : L.sums)) / 4, stream);
     if (rc) return rc;
-    launch_traced("balance_columns_kernel", (balance_columns_kernel<T>),
-                  dim3(cols, (unsigned)chunks, (unsigned)P.batch), dim3(kThreads), 0,
-                  stream, P, x, stats, chunks, partials);
-    rc = check_launch("balance_columns_kernel");
-    if (rc) return rc;
+    if (P.rows > 0) {
+      launch_traced("balance_long_rows_kernel", (balance_long_rows_kernel<T>),
+                    dim3((unsigned)(P.rows * P.batch)), dim3(kThreads), 0, stream, P, x,
+                    stats, w);
+      rc = check_launch("balance_long_rows_kernel");
+      if (rc) return rc;
+      const int per = kThreads * kVec<T>;
+      launch_traced("balance_columns_kernel", (balance_columns_kernel<T>),
+                    dim3((unsigned)((P.K + per - 1) / per), (unsigned)w.blocks,
+                         (unsigned)P.batch),
+                    dim3(kThreads), 0, stream, P, x, stats, w);
+      rc = check_launch("balance_columns_kernel");
+    }
   }
-  launch_traced("balance_mean_kernel", balance_mean_kernel,
-                dim3(cols, (unsigned)P.batch), dim3(kThreads), 0, stream, P,
-                partials, chunks, totals, mean);
-  rc = check_launch("balance_mean_kernel");
   if (rc) return rc;
-  launch_traced("balance_loss_kernel", balance_loss_kernel, dim3((unsigned)P.batch),
-                dim3(kThreads), 0, stream, P, mean, counts, totals, loss);
-  return check_launch("balance_loss_kernel");
+  launch_traced("balance_join_kernel", balance_join_kernel,
+                dim3((unsigned)column_groups(P), (unsigned)P.batch),
+                dim3(64 * kJoinWaves), 0, stream, P, w, loss, counts, mean,
+                reinterpret_cast<int4*>(totals));
+  return check_launch("balance_join_kernel");
 }
 
 template <typename T>
 int backward_of(const BalanceParams& P, const void* logits, const int32_t* counts,
-                const float2* stats, const int32_t* totals, const float* g_loss,
+                const float2* stats, const int4* totals, const float* g_loss,
                 const float* g_mean, void* g_logits, hipStream_t stream) {
-  const int64_t rows = P.rows * P.batch;
-  launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T>),
-                dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0,
-                stream, P, static_cast<const T*>(logits), counts, stats, totals,
-                g_loss, g_mean, static_cast<T*>(g_logits));
-  return check_launch("balance_bwd_kernel");
+  const T* x = static_cast<const T*>(logits);
+  T* g = static_cast<T*>(g_logits);
+  if (P.K > kLongest) {
+    launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T>),
+                  dim3((unsigned)(P.rows * P.batch)), dim3(kThreads), 0, stream, P, x,
+                  counts, stats, totals, g_loss, g_mean, g);
+    return check_launch("balance_long_bwd_kernel");
+  }
+  const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
+#define GS_BWD(TL, W, R)                                                      \
+  {                                                                           \
+    using G = Team<T, TL, W, R>;                                              \
+    const int64_t most = std::max(1, (W > 4 ? 4096 / W : 1024) / P.batch);         \
+    const int64_t turns = (P.rows + G::kTeams - 1) / G::kTeams;               \
+    launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T, TL, W, R>),    \
+                  dim3((unsigned)std::min(most, turns), (unsigned)P.batch),   \
+                  dim3(G::kThreads), 0, stream, P, x, counts, stats, totals,  \
+                  g_loss, g_mean, g);                                         \
+    return check_launch("balance_bwd_kernel");                                \
+  }
+  GS_TEAMS(GS_BWD)
+#undef GS_BWD
 }
+#undef GS_TEAMS
 
 }  // namespace
 
-size_t balance_workspace_bytes(const BalanceParams& P) {
-  return align_up((size_t)P.batch * chunks_of(P) * P.K * 4, 256);
-}
+size_t balance_workspace_bytes(const BalanceParams& P) { return layout(P).total; }
 
 int launch_balance_forward(const BalanceParams& P, const void* logits,
                            float* loss, int32_t* counts, float* mean_probs,
@@ -199,7 +639,7 @@ int launch_balance_forward(const BalanceParams& P, const void* logits,
            : P.dtype == GSPLAT_BF16 ? forward_of<__bf16>
                                     : forward_of<_Float16>;
   return f(P, logits, loss, counts, mean_probs, stats, totals,
-           static_cast<float*>(workspace), stream);
+           static_cast<char*>(workspace), stream);
 }
 
 int launch_balance_backward(const BalanceParams& P, const void* logits,
@@ -211,7 +651,8 @@ int launch_balance_backward(const BalanceParams& P, const void* logits,
   auto f = P.dtype == GSPLAT_F32    ? backward_of<float>
            : P.dtype == GSPLAT_BF16 ? backward_of<__bf16>
                                     : backward_of<_Float16>;
-  return f(P, logits, counts, stats, totals, g_loss, g_mean, g_logits, stream);
+  return f(P, logits, counts, stats, reinterpret_cast<const int4*>(totals), g_loss,
+           g_mean, g_logits, stream);
 }
 
 }  // namespace gs

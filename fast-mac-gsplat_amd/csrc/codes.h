@@ -122,6 +122,9 @@ __device__ __forceinline__ uint32_t team_umax(uint32_t v) {
   return team_reduce<L>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
+__device__ __forceinline__ int wave_isum(int v) {
+  return (int)team_reduce<64>((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; });
+}
 __device__ __forceinline__ float wave_sum(float v) { return team_sum<64>(v); }
 __device__ __forceinline__ float wave_max(float v) { return team_max<64>(v); }
 
