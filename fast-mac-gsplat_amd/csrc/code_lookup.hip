@@ -1,17 +1,22 @@
 // code_lookup.hip -- attributes of splats from a codebook, and the gradient.
 //
 //   out[n] = f s_n C[c_n]                     (c_n = -1: zeros)
-//   gC[k]  = f * sum over n with c_n = k, in ascending n, of s_n g[n]
+//   gC[k]  = f * sum over n with c_n = k of s_n g[n]
 //   gs[n]  = f <g[n], C[c_n]>
 //
-// The gradient of the codebook is a sum by code.  The splats are sorted by
-// code (stable), so a code's splats are one run of the sorted positions, and
-// runs are cut at every kPiece-th position: a piece (a run's part between two
-// cuts) is one wavefront's work however the splats are spread over the codes.
-// Runs inside one cut are written at once; the others' pieces go to two
-// partial rows per cut (one for the run that comes in from the left, one for
-// the run that goes on to the right) and are added up by a second launch in
-// the order of the positions.  No atomics: the same inputs give the same bits.
+// The gradient of the codebook is a sum by code, in an order that does not
+// depend on the run (no atomics: the same inputs give the same bits).
+//
+// Few splats: a wavefront takes four codes, reads every splat's code, lists
+// those that name one of the four and adds up their rows (one launch).
+//
+// More splats: they are sorted by code (stable), so that a code's splats are
+// one run of the sorted positions.  A team of lanes adds up `piece` positions,
+// whatever runs they belong to: runs that begin and end there are written at
+// once, the others meet in a segmented scan over the workgroup's teams, and
+// what runs over the workgroup's ends goes to two partial rows, which a second
+// launch adds up.  Every workgroup has the same work however the splats are
+// spread over the codes.  The splats' rows are read once, for both gradients.
 #include <algorithm>
 
 #include "codes.h"
@@ -20,130 +25,549 @@ namespace gs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPiece = 128;  // sorted positions between two cuts
 
-template <typename T>
+__device__ __forceinline__ float nan_for(int c) {
+  return c == kBadCode ? __builtin_nanf("") : 0.0f;
+}
+
+// ---- forward
+
+// Each thread writes kUnroll vectors of 16 bytes of the output, taken as one
+// array; block b starts at element b * kThreads * V * kUnroll.  div: the
+// quotient of a 32-bit offset by D (below).
+constexpr int kUnroll = 4;
+
+// n / d for n < 2^31 by one 32 x 32 multiplication: floor(n m / 2^(32 + s))
+// with m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1 (exact for n < 2^31: the
+// error n (m d - 2^(32 + s)) / (d 2^(32 + s)) is below 1 / d).
+struct Divide {
+  uint32_t d, m, s;
+  explicit Divide(uint32_t d_) : d(d_), m(0), s(0) {
+    if (d == 1) return;
+    while ((uint64_t(1) << (s + 1)) < d) ++s;
+    m = (uint32_t)(((uint64_t(1) << (32 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    return d == 1 ? n : __umulhi(n, m) >> s;
+  }
+};
+
+template <typename T, bool Rows>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
-    LookupParams P, const T* __restrict__ codebook,
+    LookupParams P, Divide div, const T* __restrict__ codebook,
     const float* __restrict__ scales, T* __restrict__ out) {
+  constexpr int V = kVec<T>;
   const int64_t total = P.rows * P.D;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * kThreads) {
-    const int64_t n = i / P.D;
-    const int d = (int)(i - n * P.D);
-    const int c = P.codes.at(n, P.K);
-    float v = c == kBadCode ? __builtin_nanf("") : 0.0f;
-    if (c >= 0) {
-      v = to_float(codebook[c * P.stride + d]) * (scales ? P.factor * scales[n] : P.factor);
+  const int64_t start = (int64_t)blockIdx.x * (kThreads * V * kUnroll);
+  const int64_t row0 = start / P.D;
+  const uint32_t skip = (uint32_t)(start - row0 * P.D);
+  int64_t at[kUnroll];
+  uint32_t d[kUnroll];
+  int64_t n[kUnroll];
+  int c[kUnroll];
+  float s[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t i = (u * kThreads + threadIdx.x) * V;
+    at[u] = start + i;
+    const uint32_t q = div(skip + i);
+    d[u] = skip + i - q * P.D;
+    n[u] = row0 + q;
+    const bool in = at[u] < total;
+    c[u] = in ? P.codes.at(n[u], P.K) : kNoCode;
+    s[u] = P.factor;
+    if (scales && in) s[u] *= scales[n[u]];
+  }
+  vec_t<T> x[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const T* row = codebook + (int64_t)max(c[u], 0) * P.stride;
+    if (Rows || d[u] + V <= (uint32_t)P.D) {
+      x[u] = load_vec(row + d[u]);
+    } else {
+      // the vector goes on in the next rows
+      uint32_t e = d[u];
+      int64_t r = n[u];
+      int k = c[u];
+      float f = s[u];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float y = nan_for(k);
+        if (k >= 0) y = to_float(codebook[(int64_t)k * P.stride + e]) * f;
+        x[u][v] = static_cast<T>(y);
+        if (++e == (uint32_t)P.D) {
+          e = 0;
+          ++r;
+          if (v + 1 < V && r < P.rows) {
+            k = P.codes.at(r, P.K);
+            f = scales ? P.factor * scales[r] : P.factor;
+          }
+        }
+      }
     }
-    out[i] = static_cast<T>(v);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (at[u] >= total) continue;
+    vec_t<T> y = x[u];
+    if (Rows || d[u] + V <= (uint32_t)P.D) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        y[v] = static_cast<T>(c[u] >= 0 ? to_float(x[u][v]) * s[u] : nan_for(c[u]));
+    }
+    if (at[u] + V <= total) {
+      store_vec(out + at[u], y);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (at[u] + v < total) out[at[u] + v] = y[v];
+    }
   }
 }
 
+// ---- backward
+
+// A team of TL lanes holds R vectors per lane of a row's columns from c0 on.
+template <typename T, int TL, int R>
+struct Columns {
+  static constexpr int V = kVec<T>;
+  static constexpr int kWidth = TL * V * R;
+  static constexpr int kTeams = kThreads / TL;
+  static __device__ __forceinline__ int lane() { return threadIdx.x & (TL - 1); }
+  static __device__ __forceinline__ int column(int c0, int r) { return c0 + (r * TL + lane()) * V; }
+  static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int c0, int D) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      x[r] = load_part<T>(row, column(c0, r), D, static_cast<T>(0.0f));
+  }
+  static __device__ __forceinline__ void store(T* row, int c0, int D, const float (&a)[R * V],
+                                               float f) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      vec_t<T> o;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = static_cast<T>(a[r * V + v] * f);
+      if (column(c0, r) < D) store_part<T>(row, column(c0, r), D, o);
+    }
+  }
+  static __device__ __forceinline__ void load_sums(float (&a)[R * V], const float* row, int c0,
+                                                   int D) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int k = column(c0, r) + v;
+        a[r * V + v] = k < D ? row[k] : 0.0f;
+      }
+  }
+  static __device__ __forceinline__ void store_sums(float* row, int c0, int D,
+                                                    const float (&a)[R * V]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int k = column(c0, r) + v;
+        if (k < D) row[k] = a[r * V + v];
+      }
+  }
+};
+
+// Few splats.  Wavefront w takes codes 4w .. 4w + 3.  The splats are read
+// kList at a time; per code the rows found are shared out over the wavefront's
+// teams, whose sums are added in the order of the teams.
+constexpr int kList = 256;
+constexpr int kCodes = 4;  // per wavefront
+
+template <typename T, int TL, int R>
+__global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
+    LookupParams P, const T* __restrict__ grad, const T* __restrict__ codebook,
+    const float* __restrict__ scales, T* __restrict__ g_codebook,
+    float* __restrict__ g_scales) {
+  using C = Columns<T, TL, R>;
+  constexpr int V = C::V, kT = 64 / TL;
+  __shared__ uint16_t lists[kThreads / 64][kCodes][kList];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int team = lane / TL;
+  const int first = ((int)blockIdx.x * (kThreads / 64) + w) * kCodes;
+  if (first >= P.K) return;
+  const int c0 = blockIdx.y * C::kWidth;
+  const bool dots = g_scales != nullptr;
+  float acc[kCodes][R * V];
+#pragma unroll
+  for (int q = 0; q < kCodes; ++q)
+#pragma unroll
+    for (int j = 0; j < R * V; ++j) acc[q][j] = 0.0f;
+  for (int64_t base = 0; base < P.rows; base += kList) {
+    int found[kCodes] = {0, 0, 0, 0};
+    int mine[kList / 64];
+#pragma unroll
+    for (int u = 0; u < kList / 64; ++u) {
+      const int64_t n = base + u * 64 + lane;
+      mine[u] = n < P.rows ? P.codes.at(n, P.K) : kNoCode;
+      if (dots && first == 0 && n < P.rows && mine[u] < 0) g_scales[n] = nan_for(mine[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kList / 64; ++u) {
+      const unsigned rel = (unsigned)(mine[u] - first);
+      if (__ballot(rel < (unsigned)kCodes) == 0) continue;
+#pragma unroll
+      for (int q = 0; q < kCodes; ++q) {
+        const uint64_t hit = __ballot(rel == (unsigned)q);
+        if (rel == (unsigned)q)
+          lists[w][q][found[q] + __builtin_amdgcn_mbcnt_hi(
+                                     (uint32_t)(hit >> 32),
+                                     __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0))] =
+              (uint16_t)(u * 64 + lane);
+        found[q] += __popcll(hit);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < kCodes; ++q) {
+      if (found[q] == 0) continue;
+      vec_t<T> row[R];
+      if (dots) C::load(row, codebook + (int64_t)(first + q) * P.stride, c0, P.D);
+      // (every team makes the same number of turns: the sums of a row's
+      // products run over whole teams)
+      for (int i0 = 0; i0 < found[q]; i0 += kT) {
+        const int i = i0 + team;
+        const bool here = i < found[q];
+        const int64_t n = base + lists[w][q][here ? i : 0];
+        vec_t<T> g[R];
+        C::load(g, grad + n * P.D, c0, P.D);
+        const float s = !here ? 0.0f : scales ? scales[n] : 1.0f;
+        float dot = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float x = to_float(g[r][v]);
+            if (here) acc[q][r * V + v] = __builtin_fmaf(x, s, acc[q][r * V + v]);
+            if (dots) dot = __builtin_fmaf(x, to_float(row[r][v]), dot);
+          }
+        if (dots) {
+          dot = team_sum<TL>(dot);
+          if (here && C::lane() == 0) g_scales[n] = dot * P.factor;
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (g_codebook == nullptr) return;
+#pragma unroll
+  for (int q = 0; q < kCodes; ++q) {
+    if (first + q >= P.K) return;
+#pragma unroll
+    for (int j = 0; j < R * V; ++j)
+#pragma unroll
+      for (int d = TL; d < 64; d <<= 1) acc[q][j] += __shfl_xor(acc[q][j], d, 64);
+    if (team == 0) C::store(g_codebook + (int64_t)(first + q) * P.D, c0, P.D, acc[q], P.factor);
+  }
+}
+
+// Keys of the sort (K for splats without a code: after all others), and zeros
+// for the sort's control words and the codebook's gradient (zero_bytes of it,
+// 16 at a time and the rest by bytes).
 __global__ __launch_bounds__(kThreads) void lookup_keys_kernel(
-    LookupParams P, uint32_t* __restrict__ keys) {
-  const int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (n >= P.rows) return;
-  const int c = P.codes.at(n, P.K);
-  keys[n] = c >= 0 ? (uint32_t)c : (uint32_t)P.K;  // (no code: after all codes)
-}
-
-// edges[k] = the first sorted position whose key is at least k, k = 0..K.
-__global__ __launch_bounds__(kThreads) void lookup_edges_kernel(
-    const uint32_t* __restrict__ keys, int64_t n, int K,
-    int32_t* __restrict__ edges) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i > n) return;
-  const int64_t before = i == 0 ? -1 : (int64_t)min(keys[i - 1], (uint32_t)K);
-  const int64_t here = i == n ? (int64_t)K : (int64_t)min(keys[i], (uint32_t)K);
-  for (int64_t k = before + 1; k <= here; ++k) edges[k] = (int32_t)i;
-}
-
-// The code whose pieces hold piece i: code k's pieces are numbered from
-// k + edges[k] / kPiece (a number that grows with k by the cuts passed and one).
-__device__ __forceinline__ int code_of_piece(const int32_t* edges, int K,
-                                             int64_t i) {
-  int lo = 0, hi = K - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (mid + edges[mid] / kPiece <= i) lo = mid; else hi = mid - 1;
+    LookupParams P, uint32_t* __restrict__ keys, uint32_t* __restrict__ ctl,
+    int64_t ctl_words, char* __restrict__ g_codebook, int64_t zero_bytes) {
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  for (int64_t n = t; n < P.rows; n += step) {
+    const int c = P.codes.at(n, P.K);
+    keys[n] = c >= 0 ? (uint32_t)c : (uint32_t)P.K;
   }
-  return lo;
+  for (int64_t i = t; i < ctl_words; i += step) ctl[i] = 0;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int64_t i = t; i < zero_bytes / 16; i += step)
+    __builtin_memcpy(g_codebook + 16 * i, &zero, 16);
+  for (int64_t i = zero_bytes / 16 * 16 + t; i < zero_bytes; i += step) g_codebook[i] = 0;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void lookup_pieces_kernel(
-    LookupParams P, const int32_t* __restrict__ edges,
-    const uint32_t* __restrict__ order, const T* __restrict__ grad,
-    const float* __restrict__ scales, const uint32_t* __restrict__ err,
-    float* __restrict__ partials, T* __restrict__ g_codebook) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  const int k = code_of_piece(edges, P.K, i);
-  const int first = edges[k], end = edges[k + 1];
-  const int64_t block = i - k;  // (of the sorted positions, kPiece each)
-  const int64_t a = max((int64_t)first, block * kPiece);
-  const int64_t b = min((int64_t)end, (block + 1) * kPiece);
-  if (i >= P.K + (int64_t)edges[P.K] / kPiece) return;  // past the last piece
-  const bool whole = end == first || first / kPiece == (end - 1) / kPiece;
-  if (whole ? block != first / kPiece : a >= b) return;  // an empty last piece
-  const bool bad = *err != 0;
-  for (int d = lane; d < P.D; d += 64) {
-    float acc = 0.0f;
-    for (int64_t j = a; j < b; ++j) {
-      const int64_t n = order[j];
-      const float g = to_float(grad[n * P.D + d]);
-      acc += scales ? g * scales[n] : g;
+// The sorted splats and the two partial rows of each workgroup's positions
+// [b * span, (b + 1) * span): in[b] the end of a run that began before them, out[b]
+// the part of a run that goes on after them.
+constexpr uint32_t kNone = ~0u;
+struct Sorted {
+  const uint32_t* keys;
+  const uint32_t* order;
+  const uint32_t* err;  // the sort gave up: neither holds anything
+  int piece, span, blocks;
+  uint32_t* out_key;  // [blocks] the run that goes on after them, or kNone
+  float* in;          // [blocks][D]
+  float* out;
+};
+
+template <typename T, int TL, int R>
+__global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
+    LookupParams P, Sorted S, const T* __restrict__ grad,
+    const T* __restrict__ codebook, const float* __restrict__ scales,
+    T* __restrict__ g_codebook, float* __restrict__ g_scales) {
+  using C = Columns<T, TL, R>;
+  constexpr int V = C::V, kTeams = C::kTeams, kRows = R > 1 ? 2 : 4;
+  __shared__ float open[kTeams][C::kWidth + 1];  // (+ 1: teams of one lane)
+  __shared__ uint8_t ended[kTeams];
+  const int team = threadIdx.x / TL, c0 = blockIdx.y * C::kWidth;
+  const int64_t first = (int64_t)blockIdx.x * S.span;
+  const int64_t last = min(first + S.span, P.rows);
+  if (*S.err != 0) {
+    if (g_scales)
+      for (int64_t n = first + threadIdx.x; n < last; n += kThreads)
+        g_scales[n] = __builtin_nanf("");
+    return;
+  }
+  const int64_t a = min(first + (int64_t)team * S.piece, last);
+  const int64_t b = min(a + S.piece, last);
+  const bool dots = g_scales != nullptr;
+  auto write = [&](uint32_t k, const float (&x)[R * V]) {
+    if (k < (uint32_t)P.K) C::store(g_codebook + (int64_t)k * P.D, c0, P.D, x, P.factor);
+  };
+  float acc[R * V], head[R * V];
+#pragma unroll
+  for (int j = 0; j < R * V; ++j) acc[j] = head[j] = 0.0f;
+  // The run that came in from the left, until it ends.
+  const uint32_t before = a > 0 && a < b ? S.keys[a - 1] : kNone;
+  bool coming = a < b && before == S.keys[a];
+  const uint32_t head_key = before;
+  bool head_ended = false, any_end = false;
+  for (int64_t j0 = a; j0 < b; j0 += kRows) {
+    uint32_t key[kRows + 1];
+    int64_t n[kRows];
+    float s[kRows];
+    vec_t<T> g[kRows][R], row[kRows][R];
+#pragma unroll
+    for (int u = 0; u <= kRows; ++u)
+      key[u] = j0 + u < P.rows ? S.keys[j0 + u] : kNone;
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) n[u] = S.order[min(j0 + u, b - 1)];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      s[u] = scales ? scales[n[u]] : 1.0f;
+      C::load(g[u], grad + n[u] * P.D, c0, P.D);
     }
-    if (bad) acc = __builtin_nanf("");
-    if (whole)
-      g_codebook[(int64_t)k * P.D + d] = static_cast<T>(acc * P.factor);
-    else
-      partials[(2 * block + (a == first ? 1 : 0)) * P.D + d] = acc;
+    if (dots)
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+        C::load(row[u], codebook + (int64_t)min(key[u], (uint32_t)P.K - 1) * P.stride, c0, P.D);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if (j0 + u >= b) break;
+      float dot = 0.0f;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float x = to_float(g[u][r][v]);
+          acc[r * V + v] = __builtin_fmaf(x, s[u], acc[r * V + v]);
+          if (dots) dot = __builtin_fmaf(x, to_float(row[u][r][v]), dot);
+        }
+      if (dots) {
+        dot = team_sum<TL>(dot) * P.factor;
+        if (C::lane() == 0)
+          g_scales[n[u]] = key[u] < (uint32_t)P.K ? dot : nan_for(P.codes.at(n[u], P.K));
+      }
+      if (key[u] != key[u + 1]) {  // the run ends
+        any_end = true;
+        if (coming) {
+          coming = false;
+          head_ended = true;
+#pragma unroll
+          for (int q = 0; q < R * V; ++q) head[q] = acc[q];
+        } else {
+          write(key[u], acc);
+        }
+#pragma unroll
+        for (int q = 0; q < R * V; ++q) acc[q] = 0.0f;
+      }
+    }
   }
+  if (g_codebook == nullptr) return;
+  // Inclusive segmented scan of the teams' open sums: open[t] becomes the sum of
+  // the run that goes on after team t, from the workgroup's first position on.
+  auto column_of = [&](int r, int v) { return (r * TL + C::lane()) * V + v; };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) open[team][column_of(r, v)] = acc[r * V + v];
+  if (C::lane() == 0) ended[team] = any_end;
+  __syncthreads();
+  bool seen = any_end;
+  for (int d = 1; d < kTeams; d <<= 1) {
+    const bool take = team >= d && !seen;
+    const bool more = team >= d && ended[team - d];
+    if (take)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          acc[r * V + v] += open[team - d][column_of(r, v)];
+    __syncthreads();
+    if (take) {
+      seen = more;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v) open[team][column_of(r, v)] = acc[r * V + v];
+      if (C::lane() == 0) ended[team] = seen;
+    }
+    __syncthreads();
+  }
+  const uint32_t left = first > 0 ? S.keys[first - 1] : kNone;
+  if (head_ended) {
+    if (team > 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          head[r * V + v] += open[team - 1][column_of(r, v)];
+    if (left == head_key) {
+      C::store_sums(S.in + (int64_t)blockIdx.x * P.D, c0, P.D, head);
+    } else {
+      write(head_key, head);
+    }
+  }
+  const uint32_t right = last < P.rows ? S.keys[last] : kNone;
+  const uint32_t last_key = S.keys[last - 1];
+  if (threadIdx.x == 0 && blockIdx.y == 0)
+    S.out_key[blockIdx.x] = last_key == right ? last_key : kNone;
+  if (team == kTeams - 1 && last_key == right)
+    C::store_sums(S.out + (int64_t)blockIdx.x * P.D, c0, P.D, acc);
 }
 
-template <typename T>
+// One workgroup per workgroup of the launch above: where a run begins that goes
+// on after its positions, that run's partial rows are added up (teams take
+// every kTeams-th row, then the teams in order).  A sort that gave up makes
+// the gradient NaN.
+template <typename T, int TL, int R>
 __global__ __launch_bounds__(kThreads) void lookup_join_kernel(
-    LookupParams P, const int32_t* __restrict__ edges,
-    const float* __restrict__ partials, T* __restrict__ g_codebook) {
-  const int k = (int)blockIdx.x;
-  const int first = edges[k], end = edges[k + 1];
-  if (end == first || first / kPiece == (end - 1) / kPiece) return;
-  for (int d = threadIdx.x; d < P.D; d += kThreads) {
-    float acc = partials[(2 * (int64_t)(first / kPiece) + 1) * P.D + d];
-    for (int64_t b = first / kPiece + 1; b <= (end - 1) / kPiece; ++b)
-      acc += partials[2 * b * P.D + d];
-    g_codebook[(int64_t)k * P.D + d] = static_cast<T>(acc * P.factor);
+    LookupParams P, Sorted S, T* __restrict__ g_codebook) {
+  using C = Columns<T, TL, R>;
+  constexpr int V = C::V, kTeams = C::kTeams;
+  __shared__ float sums[kTeams][C::kWidth + 1];
+  __shared__ int ends[kThreads / 64];
+  if (*S.err != 0) {
+    const int64_t total = (int64_t)P.K * P.D;
+    if (blockIdx.y == 0)
+      for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total;
+           i += (int64_t)gridDim.x * kThreads)
+        g_codebook[i] = static_cast<T>(__builtin_nanf(""));
+    return;
   }
+  const int b = blockIdx.x, c0 = blockIdx.y * C::kWidth;
+  const uint32_t k = S.out_key[b];
+  if (k >= (uint32_t)P.K) return;  // (kNone, or the splats without a code)
+  const int64_t first = (int64_t)b * S.span;
+  if (first > 0 && S.keys[first] == k && S.keys[first - 1] == k) return;  // began before
+  // the workgroup where the run ends: the first after b whose out_key is not k
+  int end = b + 1;
+  for (;; end += kThreads) {
+    const int i = end + threadIdx.x;
+    const uint64_t other = __ballot(i >= S.blocks || S.out_key[i] != k);
+    if ((threadIdx.x & 63) == 0)
+      ends[threadIdx.x >> 6] = other ? __builtin_ctzll(other) + (int)(threadIdx.x & ~63) : kThreads;
+    __syncthreads();
+    int e = kThreads;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) e = min(e, ends[w]);
+    __syncthreads();
+    if (e < kThreads) {
+      end += e;
+      break;
+    }
+  }
+  const int team = threadIdx.x / TL;
+  float acc[R * V], x[R * V];
+#pragma unroll
+  for (int j = 0; j < R * V; ++j) acc[j] = 0.0f;
+  for (int i = b + team; i <= end; i += kTeams) {
+    C::load_sums(x, (i < end ? S.out : S.in) + (int64_t)i * P.D, c0, P.D);
+#pragma unroll
+    for (int j = 0; j < R * V; ++j) acc[j] += x[j];
+  }
+  auto column_of = [&](int r, int v) { return (r * TL + C::lane()) * V + v; };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) sums[team][column_of(r, v)] = acc[r * V + v];
+  __syncthreads();
+  if (team != 0) return;
+  for (int t = 1; t < kTeams; ++t)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[r * V + v] += sums[t][column_of(r, v)];
+  C::store(g_codebook + (int64_t)k * P.D, c0, P.D, acc, P.factor);
 }
 
+// A wavefront per splat: the gradient of the scales where a row takes several
+// workgroups, or where it is the only gradient.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void lookup_scales_kernel(
     LookupParams P, const T* __restrict__ grad, const T* __restrict__ codebook,
     float* __restrict__ g_scales) {
+  constexpr int V = kVec<T>;
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (n >= P.rows) return;
   const int c = P.codes.at(n, P.K);
   float acc = 0.0f;
   if (c >= 0)
-    for (int d = lane; d < P.D; d += 64)
-      acc += to_float(grad[n * P.D + d]) * to_float(codebook[c * P.stride + d]);
+    for (int d = lane * V; d < P.D; d += 64 * V) {
+      const vec_t<T> g = load_part<T>(grad + n * P.D, d, P.D, static_cast<T>(0.0f));
+      const vec_t<T> x =
+          load_part<T>(codebook + (int64_t)c * P.stride, d, P.D, static_cast<T>(0.0f));
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc = __builtin_fmaf(to_float(g[v]), to_float(x[v]), acc);
+    }
   acc = wave_sum(acc);
-  if (lane == 0) g_scales[n] = c == kBadCode ? __builtin_nanf("") : acc * P.factor;
+  if (lane == 0) g_scales[n] = c < 0 ? nan_for(c) : acc * P.factor;
+}
+
+// ---- host
+
+// Lanes of a team and vectors of a lane for rows of D values: CALL(TL, R).
+#define GS_WIDTHS(CALL)          \
+  if (vecs <= 1) CALL(1, 1)      \
+  if (vecs <= 2) CALL(2, 1)      \
+  if (vecs <= 4) CALL(4, 1)      \
+  if (vecs <= 8) CALL(8, 1)      \
+  if (vecs <= 16) CALL(16, 1)    \
+  if (vecs <= 32) CALL(32, 1)    \
+  if (vecs <= 64) CALL(64, 1)    \
+  CALL(64, 2)
+
+int vec_of(const LookupParams& P) { return P.dtype == GSPLAT_F32 ? 4 : 8; }
+int vecs_of(const LookupParams& P) { return (P.D + vec_of(P) - 1) / vec_of(P); }
+int lanes_of(const LookupParams& P) {
+  int tl = 1;
+  while (tl < 64 && tl < vecs_of(P)) tl *= 2;
+  return tl;
+}
+
+// The one-launch way reads all codes once for each four of the codebook.
+bool few(const LookupParams& P) {
+  return P.rows <= 8192 && P.rows * P.K <= (int64_t(1) << 26);
 }
 
 struct Layout {
   RadixPlan sort;
-  size_t ctl, buffers, keys, sorted, order, edges, partials, total;
+  int piece, span, blocks;
+  size_t ctl, buffers, keys, sorted, order, out_key, in, out, total;
 };
 
 Layout layout(const LookupParams& P) {
   Layout L{};
+  if (few(P)) return L;
   int bits = 1;
   while (bits < 32 && (int64_t(1) << bits) <= P.K) ++bits;
   L.sort = radix_plan(P.rows, 1, 0, bits);
+  // Positions per team: 4 to 64, about 2048 workgroups.
+  const int tl = lanes_of(P);
+  L.piece = 4;
+  while (L.piece < 64 && P.rows * tl > (int64_t)L.piece * kThreads * 2048) L.piece *= 2;
+  L.span = L.piece * (kThreads / tl);
+  L.blocks = (int)((P.rows + L.span - 1) / L.span);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -155,8 +579,9 @@ Layout layout(const LookupParams& P) {
   L.keys = take((size_t)P.rows * 4);
   L.sorted = take((size_t)P.rows * 4);
   L.order = take((size_t)P.rows * 4);
-  L.edges = take((size_t)(P.K + 1) * 4);
-  L.partials = take((size_t)(P.rows / kPiece + 1) * 2 * P.D * 4);
+  L.out_key = take((size_t)L.blocks * 4);
+  L.in = take((size_t)L.blocks * P.D * 4);
+  L.out = take((size_t)L.blocks * P.D * 4);
   L.total = off;
   return L;
 }
@@ -165,10 +590,17 @@ template <typename T>
 int forward_of(const LookupParams& P, const void* codebook, const float* scales,
                void* out, hipStream_t stream) {
   const int64_t total = P.rows * P.D;
-  const int64_t grid = std::min<int64_t>((total + kThreads - 1) / kThreads, 1 << 20);
-  launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T>), dim3((unsigned)grid),
-                dim3(kThreads), 0, stream, P, static_cast<const T*>(codebook),
-                scales, static_cast<T*>(out));
+  const int64_t per = kThreads * kVec<T> * kUnroll;
+  const dim3 grid((unsigned)((total + per - 1) / per));
+  const T* book = static_cast<const T*>(codebook);
+  T* o = static_cast<T*>(out);
+  const Divide div((uint32_t)P.D);
+  if (P.D % kVec<T> == 0)
+    launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, true>), grid,
+                  dim3(kThreads), 0, stream, P, div, book, scales, o);
+  else
+    launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, false>), grid,
+                  dim3(kThreads), 0, stream, P, div, book, scales, o);
   return check_launch("lookup_fwd_kernel");
 }
 
@@ -177,52 +609,70 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
                 const float* scales, void* g_codebook, float* g_scales,
                 void* workspace, hipStream_t stream) {
   const T* grad = static_cast<const T*>(grad_out);
-  if (g_scales && P.rows > 0) {
+  const T* book = static_cast<const T*>(codebook);
+  T* g_book = static_cast<T*>(g_codebook);
+  const int vecs = vecs_of(P);
+  // (a row of up to 128 vectors is one team's)
+  const unsigned tiles = (unsigned)((vecs + 127) / 128);
+  if (g_scales && P.rows > 0 && (tiles > 1 || !g_book)) {
     launch_traced("lookup_scales_kernel", (lookup_scales_kernel<T>),
                   dim3((unsigned)((P.rows + 3) / 4)), dim3(kThreads), 0, stream, P,
-                  grad, static_cast<const T*>(codebook), g_scales);
+                  grad, book, g_scales);
     const int rc = check_launch("lookup_scales_kernel");
     if (rc) return rc;
+    g_scales = nullptr;
   }
-  if (!g_codebook) return GSPLAT_OK;
+  if (!g_book) return GSPLAT_OK;
+  if (few(P)) {
+    const int per = kThreads / 64 * kCodes;
+    const dim3 grid((unsigned)((P.K + per - 1) / per), tiles);
+#define GS_SCAN(TL, R)                                                          \
+  {                                                                             \
+    launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R>), grid,   \
+                  dim3(kThreads), 0, stream, P, grad, book, scales, g_book,     \
+                  g_scales);                                                    \
+    return check_launch("lookup_scan_kernel");                                  \
+  }
+    GS_WIDTHS(GS_SCAN)
+#undef GS_SCAN
+  }
   const Layout L = layout(P);
   char* w = static_cast<char*>(workspace);
   auto* keys = reinterpret_cast<uint32_t*>(w + L.keys);
   auto* sorted = reinterpret_cast<uint32_t*>(w + L.sorted);
   auto* order = reinterpret_cast<uint32_t*>(w + L.order);
-  auto* edges = reinterpret_cast<int32_t*>(w + L.edges);
-  auto* partials = reinterpret_cast<float*>(w + L.partials);
   const RadixCtl C = radix_ctl_at(L.sort, w + L.ctl);
-  int rc = GSPLAT_OK;
-  if (P.rows > 0) {
-    launch_traced("lookup_keys_kernel", lookup_keys_kernel,
-                  dim3((unsigned)((P.rows + kThreads - 1) / kThreads)),
-                  dim3(kThreads), 0, stream, P, keys);
-    rc = check_launch("lookup_keys_kernel");
-  }
-  if (!rc) rc = launch_zero_u32(C.ghist, (int64_t)radix_ctl_bytes(L.sort) / 4, stream);
+  const int64_t zero_bytes = (int64_t)P.K * P.D * sizeof(T);
+  const int64_t most = std::max(P.rows, zero_bytes / 16) / kThreads + 1;
+  launch_traced("lookup_keys_kernel", lookup_keys_kernel,
+                dim3((unsigned)std::min<int64_t>(most, 2048)), dim3(kThreads), 0,
+                stream, P, keys, C.ghist, (int64_t)radix_ctl_bytes(L.sort) / 4,
+                reinterpret_cast<char*>(g_book), zero_bytes);
+  int rc = check_launch("lookup_keys_kernel");
   if (!rc) rc = radix_global_hist(L.sort, C, keys, nullptr, stream);
   if (!rc)
     rc = radix_passes(L.sort, C, w + L.buffers, keys, nullptr, nullptr, sorted,
                       order, stream);
   if (rc) return rc;
-  launch_traced("lookup_edges_kernel", lookup_edges_kernel,
-                dim3((unsigned)((P.rows + kThreads) / kThreads)), dim3(kThreads), 0,
-                stream, sorted, P.rows, P.K, edges);
-  rc = check_launch("lookup_edges_kernel");
-  if (rc) return rc;
-  const int64_t pieces = P.K + P.rows / kPiece + 1;
-  launch_traced("lookup_pieces_kernel", (lookup_pieces_kernel<T>),
-                dim3((unsigned)((pieces + 3) / 4)), dim3(kThreads), 0, stream, P,
-                edges, order, grad, scales, C.err, partials,
-                static_cast<T*>(g_codebook));
-  rc = check_launch("lookup_pieces_kernel");
-  if (rc) return rc;
-  launch_traced("lookup_join_kernel", (lookup_join_kernel<T>), dim3((unsigned)P.K),
-                dim3(kThreads), 0, stream, P, edges, partials,
-                static_cast<T*>(g_codebook));
-  return check_launch("lookup_join_kernel");
+  const Sorted S{sorted, order, C.err, L.piece, L.span, L.blocks,
+                 reinterpret_cast<uint32_t*>(w + L.out_key),
+                 reinterpret_cast<float*>(w + L.in), reinterpret_cast<float*>(w + L.out)};
+  const dim3 grid((unsigned)L.blocks, tiles);
+#define GS_RUNS(TL, R)                                                          \
+  {                                                                             \
+    launch_traced("lookup_runs_kernel", (lookup_runs_kernel<T, TL, R>), grid,   \
+                  dim3(kThreads), 0, stream, P, S, grad, book, scales, g_book,  \
+                  g_scales);                                                    \
+    rc = check_launch("lookup_runs_kernel");                                    \
+    if (rc) return rc;                                                          \
+    launch_traced("lookup_join_kernel", (lookup_join_kernel<T, TL, R>), grid,   \
+                  dim3(kThreads), 0, stream, P, S, g_book);                     \
+    return check_launch("lookup_join_kernel");                                  \
+  }
+  GS_WIDTHS(GS_RUNS)
+#undef GS_RUNS
 }
+#undef GS_WIDTHS
 
 }  // namespace
 

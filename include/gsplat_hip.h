@@ -676,9 +676,9 @@ int gsplat_hip_lookup_forward(const gsplat_lookup_meta* meta, const void* codes,
 /* g_codebook (num_codes x width, contiguous; may be NULL): sums by code in
  * ascending splat order, the same bits on every call; every row is written.
  * g_scales (rows floats; may be NULL).  grad_out: rows x width, contiguous.
- * codebook is read only for g_scales.  The workspace is needed only for
- * g_codebook.  If the sort's look-back gives up (see
- * GSPLAT_STATUS_LOOKBACK_TIMEOUT), g_codebook is NaN. */
+ * codebook is read only for g_scales.  The workspace (0 bytes for few splats)
+ * is needed only for g_codebook.  If the sort's look-back gives up (see
+ * GSPLAT_STATUS_LOOKBACK_TIMEOUT), the gradients are NaN. */
 size_t gsplat_hip_lookup_backward_workspace_bytes(const gsplat_lookup_meta* meta);
 int gsplat_hip_lookup_backward(const gsplat_lookup_meta* meta,
                                const void* grad_out, const void* codes,

@@ -51,11 +51,9 @@ def lookup(codes, codebook, scales=None, factor=1.0, grad=None):
         terms = g * (s * factor)[:, None]
         total, size = torch.zeros(K, D, dtype=torch.float64), torch.zeros(K, D, dtype=torch.float64)
         count = torch.zeros(K, dtype=torch.float64)
-        for n in range(N):
-            if good[n]:
-                total[c[n]] += terms[n]
-                size[c[n]] += terms[n].abs()
-                count[c[n]] += 1
+        total.index_add_(0, c[good], terms[good])
+        size.index_add_(0, c[good], terms[good].abs())
+        count.index_add_(0, c[good], torch.ones(int(good.sum()), dtype=torch.float64))
         r["g_codebook"] = (total, _rounded((count[:, None] + 4) * E * size, total, dtype))
         gs = factor * (g * rows).sum(-1)
         gs[(c < -1) | (c >= K)] = math.nan

@@ -93,9 +93,10 @@ def test_c_abi_checks():
         _refused(L.gsplat_hip_lookup_backward(lookup(**kw), d, d, d, None, d, None, d, 1 << 30, None), text)
         assert L.gsplat_hip_lookup_backward_workspace_bytes(lookup(**kw)) == 0
     _refused(L.gsplat_hip_lookup_forward(lookup(), None, d, None, d, None), "NULL pointer")
-    need = L.gsplat_hip_lookup_backward_workspace_bytes(lookup())
+    many = lookup(rows=100_000)  # (few splats need no workspace)
+    need = L.gsplat_hip_lookup_backward_workspace_bytes(many)
     assert need > 0
-    assert L.gsplat_hip_lookup_backward(lookup(), d, d, d, None, d, None, d, need - 1, None) == 3
+    assert L.gsplat_hip_lookup_backward(many, d, d, d, None, d, None, d, need - 1, None) == 3
 
     def probs(**kw):
         m = _lib.ProbsMeta(10, 5, 2, 5, 0, 4, 1.0)

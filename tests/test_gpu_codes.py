@@ -66,6 +66,27 @@ def test_lookup_runs_over_many_pieces(gpu, D, dtype):
     _check_lookup(gpu, *_lookup_inputs((20011,), 300, D, dtype, skew=True, seed=D), what=f"D={D}")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 5, 8, 9, 16, 17, 31, 33, 64, 65, 100, 130, 256, 257, 512, 520, 1037])
+def test_lookup_widths_of_many_splats(gpu, dtype, D):
+    """Above the splats that one launch takes: runs of one to hundreds of splats, rows of every team's width."""
+    _check_lookup(gpu, *_lookup_inputs((8200 + D,), 2000, D, dtype, skew=D % 2 == 0, seed=D), what=f"D={D} {dtype}")
+
+
+@pytest.mark.parametrize("N", [8193, 8200, 16384, 65536, 70001, 262145])
+def test_lookup_run_ends(gpu, N):
+    """Runs that end at, before and after the cuts of the sorted positions; one run of all; one run each."""
+    g = _gen(N)
+    K = 40000
+    for codes in (torch.arange(N) // 64 % K, torch.arange(N) // 63 % K, torch.zeros(N, dtype=torch.long) + 7,
+                  torch.arange(N) // 1024, torch.full((N,), -1), torch.arange(N) % K,
+                  torch.cat([torch.full((N // 2,), -1), torch.full((N - N // 2,), K - 1)])):
+        codes = codes[torch.randperm(N, generator=g)].to(torch.int32)
+        for D, scales in ((3, True), (24, False)):
+            _check_lookup(gpu, codes, torch.randn(K, D, generator=g), torch.rand(N, generator=g) if scales else None,
+                          torch.randn(N, D, generator=g), what=f"N={N} D={D}")
+
+
 @pytest.mark.parametrize("K", [70001, 1 << 18])
 def test_lookup_large_codebook(gpu, K):
     codes, book, s, grad = _lookup_inputs((6007,), K, 4, F32, seed=3)
