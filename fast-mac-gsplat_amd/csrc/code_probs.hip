@@ -34,6 +34,12 @@ __device__ __forceinline__ float bounded(float t) { return fmaxf(t, -1000.0f); }
 
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// A part whose exponents lacked a shift, as small as a rounding's error.
+__device__ __forceinline__ Part shifted(Part p, float shift) {
+  const float f = exp2_fast(shift);
+  return Part{p.m, p.s * f, (p.st + shift * p.s) * f};
+}
+
 // The statistics of a's and b's parts as one (a NaN in either s stays).
 __device__ __forceinline__ Part joined(Part a, Part b, float c) {
   Part r;
@@ -59,6 +65,20 @@ __device__ __forceinline__ uint64_t team_best(uint64_t k) {
   const uint32_t hi = team_umax<L>((uint32_t)(k >> 32));
   const uint32_t lo = team_umax<L>((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
   return ((uint64_t)hi << 32) | lo;
+}
+
+// A lower bound of the top-th largest of 64 lanes' values, of its 16 leading bits:
+// found bit by bit with a count of the lanes that reach it.
+__device__ __forceinline__ float top_bound(float v, int top) {
+  const uint32_t key = depth_key(v) >> 16;
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t q = t | (1u << bit);
+    if (__popcll(__ballot(key >= q)) >= top) t = q;
+  }
+  const uint32_t u = t << 16;
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
 struct ProbsOut {
@@ -105,27 +125,31 @@ struct Held {
       x[r] = load_part<T>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
   }
   __device__ __forceinline__ int column(int r, int v) const { return (r * TL + lane) * V + v; }
-  __device__ __forceinline__ float max() const {
-    float m = -INFINITY;
+  // The largest element of vector r (of the thread: the largest of them).
+  __device__ __forceinline__ float max_of(int r) const {
+    float m = max3(to_float(x[r][0]), to_float(x[r][1]), to_float(x[r][2]));
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int v = 0; v < V; ++v) m = fmaxf(m, to_float(x[r][v]));
-    return m;
+    for (int v = 3; v + 1 < V; v += 2) m = max3(m, to_float(x[r][v]), to_float(x[r][v + 1]));
+    return max3(m, m, to_float(x[r][V - 1]));
   }
-  // s and st of this thread's elements for the maximum m.
-  __device__ __forceinline__ Part part(float m, float c) const {
-    Part p{m, 0.0f, 0.0f};
-    const float base = base_of(m);
+  // s and st of this thread's elements, exponents from e (without its shift).
+  __device__ __forceinline__ Part part(const Exponent& e) const {
+    Part p{e.m, 0.0f, 0.0f};
+    auto sum = [&](auto exponent) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float t = (to_float(x[r][v]) - base) * c;
-        const float e = exp2_fast(t);
-        p.s += e;
-        p.st = __builtin_fmaf(e, bounded(t), p.st);
-      }
+        for (int v = 0; v < V; ++v) {
+          const float t = exponent(to_float(x[r][v]));
+          const float y = exp2_fast(t);
+          p.s += y;
+          p.st = __builtin_fmaf(y, bounded(t), p.st);
+        }
+    };
+    if (e.plain)
+      sum([&](float x) { return e.fast(x); });
+    else
+      sum([&](float x) { return e.slow(x); });
     return p;
   }
   // The largest key below `last` among this thread's elements.
@@ -160,7 +184,8 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
   constexpr int kTeams = kThreads / TL;
   __shared__ uint64_t found[TL == 64 ? kWaves * 64 : 1];
   const int lane = threadIdx.x & (TL - 1);
-  int64_t n = (int64_t)blockIdx.x * kTeams + threadIdx.x / TL;
+  const int team = TL == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TL) : threadIdx.x / TL;
+  int64_t n = (int64_t)blockIdx.x * kTeams + team;
   const bool active = n < P.rows;
   if (!active) n = P.rows - 1;  // (its lanes go along)
   const T* row = logits + n * P.stride;
@@ -172,11 +197,19 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
   }
   Held<T, TL, R> x;
   x.load(row, lane, P.K);
-  const float mine = x.max();
-  const float c = P.inv_t * kLog2e;
-  Part p = x.part(team_max<TL>(mine), c);
+  float most[R];  // of each vector
+#pragma unroll
+  for (int r = 0; r < R; ++r) most[r] = x.max_of(r);
+  float mine = most[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) mine = fmaxf(mine, most[r]);
+  const float m = team_max<TL>(mine);
+  const Exponent ex(base_of(m), 0.0f, P.inv_t * kLog2e);
+  Part p = x.part(ex);
+  p.m = m;
   p.s = team_sum<TL>(p.s);
   p.st = team_sum<TL>(p.st);
+  p = shifted(p, ex.shift);
   const RowEnd e(p, P.inv_t);
   if (lane == 0 && active) write_row(out, n, p, e, code, code_logit);
   const int top = P.top;
@@ -201,17 +234,13 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
     // largest logit: the logits from there up are few (ties aside), are
     // collected, and find their places by counting.
     if (plain && top > 1) {
-      float rest = mine, bound = p.m;
-      for (int j = 0; j < top; ++j) {
-        bound = team_max<64>(rest);
-        const uint64_t at = __ballot(rest == bound);
-        if (lane == __builtin_ctzll(at)) rest = -INFINITY;
-      }
+      const float bound = top_bound(mine, top);
       if (bound > -INFINITY) {
         uint64_t* list = found + (threadIdx.x & ~63);
         int total = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+          if (__ballot(most[r] >= bound) == 0) continue;
 #pragma unroll
           for (int v = 0; v < kVec<T>; ++v) {
             const float f = to_float(x.x[r][v]);
@@ -223,6 +252,7 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
             if (f >= bound && at < 64) list[at] = rank_key(f, x.column(r, v));
             total += __popcll(hit);
           }
+        }
         if (total <= 64) {
           __builtin_amdgcn_wave_barrier();
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -260,13 +290,14 @@ struct Split {
 
 constexpr int kFound = 256;  // logits collected for the best ones
 
-template <typename T, int R>
-__global__ __launch_bounds__(kThreads) void probs_parts_kernel(
+template <typename T, int W, int R>
+__global__ __launch_bounds__(64 * W) void probs_parts_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out, Split split) {
-  __shared__ Part parts[kWaves];
-  __shared__ float bounds[kWaves];
+  constexpr int kThreads = 64 * W;
+  __shared__ Part parts[W];
+  __shared__ float bounds[W];
   __shared__ uint64_t found[kFound];
-  __shared__ uint64_t best[kWaves];
+  __shared__ uint64_t best[W];
   __shared__ int total;
   const int64_t n = blockIdx.x / (unsigned)split.parts;
   const int part = (int)(blockIdx.x - (uint32_t)n * (unsigned)split.parts);
@@ -282,21 +313,23 @@ __global__ __launch_bounds__(kThreads) void probs_parts_kernel(
   }
   Held<T, kThreads, R> x;
   x.load(row + first, threadIdx.x, len);
-  const float mine = x.max();
+  float most[R];  // of each vector
+#pragma unroll
+  for (int r = 0; r < R; ++r) most[r] = x.max_of(r);
+  float mine = most[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) mine = fmaxf(mine, most[r]);
   const float c = P.inv_t * kLog2e;
-  Part p = x.part(wave_max(mine), c);
+  const float m = wave_max(mine);
+  const Exponent ex(base_of(m), 0.0f, c);
+  Part p = x.part(ex);
+  p.m = m;
   p.s = wave_sum(p.s);
   p.st = wave_sum(p.st);
+  p = shifted(p, ex.shift);
   const int top = min(P.top, len);
-  float bound = p.m;
-  if (top > 1) {
-    float rest = mine;
-    for (int j = 0; j < top; ++j) {
-      bound = wave_max(rest);
-      const uint64_t at = __ballot(rest == bound);
-      if (lane == __builtin_ctzll(at)) rest = -INFINITY;
-    }
-  }
+  float bound = m;
+  if (top > 1) bound = top_bound(mine, top);
   if (lane == 0) {
     parts[w] = p;
     bounds[w] = bound;
@@ -306,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void probs_parts_kernel(
   p = parts[0];
   bound = bounds[0];
 #pragma unroll
-  for (int j = 1; j < kWaves; ++j) {
+  for (int j = 1; j < W; ++j) {
     p = joined(p, parts[j], c);
     bound = fmaxf(bound, bounds[j]);
   }
@@ -331,7 +364,8 @@ __global__ __launch_bounds__(kThreads) void probs_parts_kernel(
   for (int j = top + threadIdx.x; j < P.top; j += kThreads) put(j, 0);
   if (p.s == p.s && bound > -INFINITY) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      if (most[r] < bound) continue;
 #pragma unroll
       for (int v = 0; v < kVec<T>; ++v) {
         const float f = to_float(x.x[r][v]);
@@ -340,14 +374,15 @@ __global__ __launch_bounds__(kThreads) void probs_parts_kernel(
           if (at < kFound) found[at] = rank_key(f, x.column(r, v));
         }
       }
+    }
     __syncthreads();
-    const int m = total;
-    if (m <= kFound) {
+    const int count = total;
+    if (count <= kFound) {
       // (the list's order depends on the run, the places do not)
-      if ((int)threadIdx.x < m) {
+      if ((int)threadIdx.x < count) {
         const uint64_t k = found[threadIdx.x];
         int place = 0;
-        for (int j = 0; j < m; ++j) place += found[j] > k;
+        for (int j = 0; j < count; ++j) place += found[j] > k;
         if (place < top) put(place, k);
       }
       return;
@@ -361,7 +396,7 @@ __global__ __launch_bounds__(kThreads) void probs_parts_kernel(
     __syncthreads();
     k = best[0];
 #pragma unroll
-    for (int q = 1; q < kWaves; ++q) k = max64(k, best[q]);
+    for (int q = 1; q < W; ++q) k = max64(k, best[q]);
     last = k;
     if (threadIdx.x == 0) put(j, k);
   }
@@ -410,9 +445,11 @@ __global__ __launch_bounds__(64) void probs_join_kernel(
 // ---- backward
 
 // dL/dx = -p (total + gH (log p + H)) + gl at the code + gt at the
-// alternatives, over T: per element a fused multiply-add, a base-2 exponential
-// and two products.  A team of TL lanes per part of a row of TL * kVec * R
-// columns (`parts` of them per row).
+// alternatives, over T.  Per element two fused multiply-adds, a base-2
+// exponential and a product: p = 2^(t + down), log p = (t + down) ln 2 with t from
+// Exponent, and everything that is the same for the row is in two constants.
+// A team of TL lanes per part of a row of TL * kVec * R columns (`parts` of
+// them per row).
 template <typename T, int TL, int R>
 __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     ProbsParams P, const T* __restrict__ logits,
@@ -420,12 +457,13 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     const float* __restrict__ entropy, const float* __restrict__ g_log_probs,
     const float* __restrict__ g_entropy, const float* __restrict__ g_top,
     T* __restrict__ g_logits, int parts) {
-  constexpr int kTeams = kThreads / TL, V = kVec<T>;
+  constexpr int kTeams = kThreads / TL, V = kVec<T>, kSpan = TL * V * R;
   const int lane = threadIdx.x & (TL - 1);
-  const int64_t i = (int64_t)blockIdx.x * kTeams + threadIdx.x / TL;
+  const int team = TL == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TL) : threadIdx.x / TL;
+  const int64_t i = (int64_t)blockIdx.x * kTeams + team;
   if (i >= P.rows * parts) return;
-  const int64_t n = i / parts;
-  const int first = (int)(i - n * parts) * (TL * V * R);
+  const int64_t n = parts == 1 ? i : i / parts;
+  const int first = (int)(i - n * parts) * kSpan;
   const T* row = logits + n * P.stride;
   T* out = g_logits + n * P.K;
   vec_t<T> x[R];
@@ -446,50 +484,63 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   const float* gt = g_top + n * P.top;
   const int32_t* tc = top_codes + n * P.top;
   for (int j = 0; j < top; ++j) total += gt[j];
-  const float c = P.inv_t * kLog2e;
-  const float per_t = ge * kLn2, fixed = total + ge * entropy[n];
+  // 16 bits of a result: exponents 32 up, so that probabilities that the
+  // hardware's exponential flushes are far below the type's smallest step (the
+  // exponents' own steps, 4e-6 there, are lost in 16 bits).  32 bits: exp2_full.
+  constexpr float kUp = sizeof(T) == 2 ? 32.0f : 0.0f;
+  const Exponent e(st.x, st.y - kUp, P.inv_t * kLog2e);
+  const float down = e.shift - kUp;
+  const float f = -P.inv_t * exp2_fast(down);
+  const float fixed = f * (total + ge * (entropy[n] + down * kLn2));
+  const float per_t = f * ge * kLn2;
+  gl *= P.inv_t;
+  float g[R * V];
+  auto products = [&](auto exponent) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        // (a masked logit: 0.  A row with a NaN has NaN constants.)
+        const float t = bounded(exponent(to_float(x[r][v])));
+        const float y = sizeof(T) == 2 ? exp2_fast(t) : exp2_full(t);
+        g[r * V + v] = y * __builtin_fmaf(per_t, t, fixed);
+      }
+  };
+  if (e.plain)
+    products([&](float x) { return e.fast(x); });
+  else
+    products([&](float x) { return e.slow(x); });
+  auto add = [&](int col, float w) {
+    if ((unsigned)(col - first) >= (unsigned)kSpan) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        g[r * V + v] += col - first == (r * TL + lane) * V + v ? w : 0.0f;
+  };
+  if (code >= 0) add(code, gl);
+  for (int j = 0; j < top; ++j) add(tc[j], gt[j] * P.inv_t);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int at = first + (r * TL + lane) * V;
-    float g[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float t = (to_float(x[r][v]) - st.x) * c - st.y;
-      g[v] = -exp2_full(t) * __builtin_fmaf(per_t, bounded(t), fixed);
-    }
-    auto add = [&](int col, float w) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) g[v] += col == at + v ? w : 0.0f;
-    };
-    if ((unsigned)(code - at) < (unsigned)V) add(code, gl);
-    for (int j = 0; j < top; ++j) {
-      const int col = tc[j];
-      if ((unsigned)(col - at) < (unsigned)V) add(col, gt[j]);
-    }
     vec_t<T> o;
 #pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = static_cast<T>(g[v] * P.inv_t);
-    store_part<T>(out, at, P.K, o);
+    for (int v = 0; v < V; ++v) o[v] = static_cast<T>(g[r * V + v]);
+    store_part<T>(out, first + (r * TL + lane) * V, P.K, o);
   }
 }
 
-// Rows of at most this many codes are one team's; longer ones are cut.
-template <typename T>
-constexpr int kPartLong = kThreads * kVec<T> * (sizeof(T) == 4 ? 16 : 8);
+// Rows of at most this many codes are one workgroup's; longer ones are cut.
+constexpr int kPartLong = 16384;
 
-Split split_of(const ProbsParams& P, int longest) {
+Split split_of(const ProbsParams& P) {
   Split s{1, P.K, nullptr, nullptr};
-  if (P.K <= longest) return s;
+  if (P.K <= kPartLong) return s;
   // Few rows: shorter parts, until there is one for each of 512 workgroups.
-  int64_t length = longest;
+  int64_t length = kPartLong;
   while (length > 2048 && P.rows * ((P.K + length - 1) / length) < 512) length /= 2;
   s.length = (int)length;
   s.parts = (int)((P.K + length - 1) / length);
   return s;
-}
-
-int longest_of(const ProbsParams& P) {
-  return P.dtype == GSPLAT_F32 ? kPartLong<float> : kPartLong<__bf16>;
 }
 
 template <typename T>
@@ -508,7 +559,7 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   GS_ROWS(2, 1) GS_ROWS(4, 1) GS_ROWS(8, 1) GS_ROWS(16, 1) GS_ROWS(32, 1)
   GS_ROWS(64, 1) GS_ROWS(64, 2) GS_ROWS(64, 4)
 #undef GS_ROWS
-  Split s = split_of(P, kPartLong<T>);
+  Split s = split_of(P);
   if (s.parts > 1) {
     s.stats = static_cast<Part*>(workspace);
     s.best = reinterpret_cast<uint64_t*>(
@@ -517,13 +568,13 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   }
   const dim3 grid((unsigned)(P.rows * s.parts));
   const int len = (s.length + V - 1) / V;
-#define GS_PARTS(R)                                                            \
-  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, R>), grid,        \
-                dim3(kThreads), 0, stream, P, x, out, s)
-  if (len <= 2 * kThreads) GS_PARTS(2);
-  else if (len <= 4 * kThreads) GS_PARTS(4);
-  else if (len <= 8 * kThreads) GS_PARTS(8);
-  else if constexpr (sizeof(T) == 4) GS_PARTS(16);
+#define GS_PARTS(W, R)                                                         \
+  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, W, R>), grid,     \
+                dim3(64 * W), 0, stream, P, x, out, s)
+  constexpr int kR = 16 / V;  // vectors of 16 elements
+  if (len <= 256 * kR) GS_PARTS(4, kR);
+  else if (len <= 512 * kR) GS_PARTS(4, 2 * kR);
+  else GS_PARTS(8, 2 * kR);
 #undef GS_PARTS
   const int rc = check_launch("probs_parts_kernel");
   if (rc || s.parts == 1) return rc;
@@ -564,7 +615,7 @@ int backward_of(const ProbsParams& P, const void* logits, const int32_t* top_cod
 }  // namespace
 
 size_t probs_workspace_bytes(const ProbsParams& P) {
-  const Split s = split_of(P, longest_of(P));
+  const Split s = split_of(P);
   if (s.parts == 1) return 0;
   return align_up((size_t)P.rows * s.parts * sizeof(Part), 256) +
          (size_t)P.rows * s.parts * P.top * sizeof(uint64_t);

@@ -38,6 +38,36 @@ __device__ __forceinline__ float log2_fast(float t) { return __builtin_amdgcn_lo
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+// The largest of three in one instruction (fmaxf first quiets each operand that
+// might be a signalling NaN, an instruction apiece).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Exponents (x - m) c - l of a row's elements in one fused multiply-add: t(x) =
+// x c - k with k = m c + l rounded, and what the rounding of k took, the same
+// for all the row's elements: the exponent is t + shift.  Rows whose k is past
+// 1e30 (a largest logit near the type's limits, no probabilities at all) are
+// not `plain` and take slow(x), whose shift is 0.
+struct Exponent {
+  float m, l, c, k, shift;
+  bool plain;
+  __device__ __forceinline__ Exponent(float m_, float l_, float c_) : m(m_), l(l_), c(c_) {
+#pragma clang fp contract(off)
+    const float hi = m * c;
+    const float lo = __builtin_fmaf(m, c, -hi);
+    k = hi + l;
+    const float back = k - hi;
+    const float rest = (hi - (k - back)) + (l - back);
+    plain = __builtin_fabsf(k) < 1e30f;
+    shift = plain ? -(lo + rest) : 0.0f;
+  }
+  __device__ __forceinline__ float fast(float x) const { return __builtin_fmaf(x, c, -k); }
+  __device__ __forceinline__ float slow(float x) const { return (x - m) * c - l; }
+};
+
 // 16 bytes of elements, loaded and stored at any multiple of the element size
 // (rows of logits start anywhere; the memory pipeline takes dwordx4 accesses
 // at any address).
@@ -83,7 +113,7 @@ __device__ __forceinline__ void store_part(T* row, int i, int n, vec_t<T> v) {
 // of a quad are equal by then), across 16 and 32 lanes by the row swaps.
 template <int Ctrl>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, Ctrl, 0xf, 0xf, false);
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, Ctrl, 0xf, 0xf, true);
 }
 template <int L, typename Op>
 __device__ __forceinline__ uint32_t team_reduce(uint32_t v, Op op) {
