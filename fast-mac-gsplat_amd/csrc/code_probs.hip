@@ -81,6 +81,24 @@ __device__ __forceinline__ float top_bound(float v, int top) {
   return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
+// A logit that may be among the best, and its column.
+struct Found {
+  float x;
+  uint32_t i;
+};
+
+// How many of the first n lanes' keys are above this lane's.
+__device__ __forceinline__ int place_among(uint64_t k, int n) {
+  int place = 0;
+  for (int j = 0; j < n; ++j) {
+    const uint64_t q =
+        ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), j) << 32) |
+        (uint32_t)__builtin_amdgcn_readlane((int)k, j);
+    place += q > k;
+  }
+  return place;
+}
+
 struct ProbsOut {
   float* log_probs;
   float* entropy;
@@ -125,17 +143,22 @@ struct Held {
       x[r] = load_part<T>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
   }
   __device__ __forceinline__ int column(int r, int v) const { return (r * TL + lane) * V + v; }
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int r = 0; r < R; ++r) gs::forget<T>(x[r]);
+  }
   // The largest element of vector r (of the thread: the largest of them).
   __device__ __forceinline__ float max_of(int r) const {
     float m = max3(to_float(x[r][0]), to_float(x[r][1]), to_float(x[r][2]));
 #pragma unroll
     for (int v = 3; v + 1 < V; v += 2) m = max3(m, to_float(x[r][v]), to_float(x[r][v + 1]));
-    return max3(m, m, to_float(x[r][V - 1]));
+    return fmaxf(m, to_float(x[r][V - 1]));
   }
   // s and st of this thread's elements, exponents from e (without its shift).
-  __device__ __forceinline__ Part part(const Exponent& e) const {
+  __device__ __forceinline__ Part part(const Exponent& e) {
     Part p{e.m, 0.0f, 0.0f};
     auto sum = [&](auto exponent) {
+      forget();
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -182,21 +205,16 @@ template <typename T, int TL, int R>
 __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out) {
   constexpr int kTeams = kThreads / TL;
-  __shared__ uint64_t found[TL == 64 ? kWaves * 64 : 1];
+  __shared__ Found found[TL == 64 ? kWaves * 64 : 1];
   const int lane = threadIdx.x & (TL - 1);
   const int team = TL == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TL) : threadIdx.x / TL;
   int64_t n = (int64_t)blockIdx.x * kTeams + team;
   const bool active = n < P.rows;
   if (!active) n = P.rows - 1;  // (its lanes go along)
   const T* row = logits + n * P.stride;
-  int code = kNoCode;
-  float code_logit = 0.0f;
-  if (P.codes.p) {
-    code = P.codes.at(n, P.K);
-    if (code >= 0) code_logit = to_float(row[code]);
-  }
   Held<T, TL, R> x;
   x.load(row, lane, P.K);
+  const int code = P.codes.p ? P.codes.at(n, P.K) : kNoCode;
   float most[R];  // of each vector
 #pragma unroll
   for (int r = 0; r < R; ++r) most[r] = x.max_of(r);
@@ -204,6 +222,8 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
 #pragma unroll
   for (int r = 1; r < R; ++r) mine = fmaxf(mine, most[r]);
   const float m = team_max<TL>(mine);
+  T code_logit = static_cast<T>(0.0f);
+  if (code >= 0) code_logit = row[code];
   const Exponent ex(base_of(m), 0.0f, P.inv_t * kLog2e);
   Part p = x.part(ex);
   p.m = m;
@@ -211,7 +231,8 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
   p.st = team_sum<TL>(p.st);
   p = shifted(p, ex.shift);
   const RowEnd e(p, P.inv_t);
-  if (lane == 0 && active) write_row(out, n, p, e, code, code_logit);
+  if (lane == 0 && active) write_row(out, n, p, e, code, to_float(code_logit));
+  x.forget();
   const int top = P.top;
   if (top == 0) return;
   auto put = [&](int j, uint32_t i, float v) {
@@ -236,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
     if (plain && top > 1) {
       const float bound = top_bound(mine, top);
       if (bound > -INFINITY) {
-        uint64_t* list = found + (threadIdx.x & ~63);
+        Found* list = found + (threadIdx.x & ~63);
         int total = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -249,20 +270,16 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
             const int at = total + __builtin_amdgcn_mbcnt_hi(
                                        (uint32_t)(hit >> 32),
                                        __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
-            if (f >= bound && at < 64) list[at] = rank_key(f, x.column(r, v));
+            if (f >= bound && at < 64) list[at] = Found{f, (uint32_t)x.column(r, v)};
             total += __popcll(hit);
           }
         }
         if (total <= 64) {
           __builtin_amdgcn_wave_barrier();
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          const uint64_t k = lane < total ? list[lane] : 0;
-          int place = 0;
-          for (int j = 0; j < total; ++j) place += list[j] > k;
-          if (lane < total && place < top) {
-            const uint32_t i = ~(uint32_t)k;
-            put(place, i, to_float(row[i]));
-          }
+          const Found mine = lane < total ? list[lane] : Found{-INFINITY, ~0u};
+          const int place = place_among(rank_key(mine.x, mine.i), total);
+          if (lane < total && place < top) put(place, mine.i, mine.x);
           return;
         }
       }
@@ -295,8 +312,8 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out, Split split) {
   constexpr int kThreads = 64 * W;
   __shared__ Part parts[W];
-  __shared__ float bounds[W];
-  __shared__ uint64_t found[kFound];
+  __shared__ float groups[64];  // largest logits of groups of W lanes
+  __shared__ Found found[kFound];
   __shared__ uint64_t best[W];
   __shared__ int total;
   const int64_t n = blockIdx.x / (unsigned)split.parts;
@@ -305,14 +322,9 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
   const int len = min(split.length, P.K - first);
   const T* row = logits + n * P.stride;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int code = kNoCode;
-  float code_logit = 0.0f;
-  if (P.codes.p && split.parts == 1) {
-    code = P.codes.at(n, P.K);
-    if (code >= 0) code_logit = to_float(row[code]);
-  }
   Held<T, kThreads, R> x;
   x.load(row + first, threadIdx.x, len);
+  const int code = P.codes.p && split.parts == 1 ? P.codes.at(n, P.K) : kNoCode;
   float most[R];  // of each vector
 #pragma unroll
   for (int r = 0; r < R; ++r) most[r] = x.max_of(r);
@@ -321,6 +333,8 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
   for (int r = 1; r < R; ++r) mine = fmaxf(mine, most[r]);
   const float c = P.inv_t * kLog2e;
   const float m = wave_max(mine);
+  T code_logit = static_cast<T>(0.0f);
+  if (code >= 0) code_logit = row[code];
   const Exponent ex(base_of(m), 0.0f, c);
   Part p = x.part(ex);
   p.m = m;
@@ -328,40 +342,39 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
   p.st = wave_sum(p.st);
   p = shifted(p, ex.shift);
   const int top = min(P.top, len);
-  float bound = m;
-  if (top > 1) bound = top_bound(mine, top);
-  if (lane == 0) {
-    parts[w] = p;
-    bounds[w] = bound;
-  }
+  const float group = team_max<W>(mine);
+  if ((lane & (W - 1)) == 0) groups[threadIdx.x / W] = group;
+  if (lane == 0) parts[w] = p;
   if (threadIdx.x == 0) total = 0;
+  x.forget();
   __syncthreads();
-  p = parts[0];
-  bound = bounds[0];
-#pragma unroll
-  for (int j = 1; j < W; ++j) {
-    p = joined(p, parts[j], c);
-    bound = fmaxf(bound, bounds[j]);
-  }
+  // (joined by teams of W lanes, each lane a wavefront's part)
+  p = parts[lane & (W - 1)];
+  const float all = team_max<W>(p.m);
+  const float d = bounded((p.m - base_of(all)) * c), f = exp2_fast(d);
+  p.st = team_sum<W>(f * (p.st + d * p.s));
+  p.s = team_sum<W>(f * p.s);
+  p.m = all;
   const RowEnd e(p, P.inv_t);
   if (threadIdx.x == 0) {
     if (split.parts == 1)
-      write_row(out, n, p, e, code, code_logit);
+      write_row(out, n, p, e, code, to_float(code_logit));
     else
       split.stats[(int64_t)blockIdx.x] = p;
   }
   if (P.top == 0) return;
-  auto put = [&](int j, uint64_t key) {
+  auto put = [&](int j, uint64_t key, float x) {
     if (split.parts == 1) {
-      const uint32_t i = ~(uint32_t)key;
-      out.top_codes[n * P.top + j] = (int)i;
-      out.top_log_probs[n * P.top + j] = e.log_prob(to_float(row[i]));
+      out.top_codes[n * P.top + j] = (int)~(uint32_t)key;
+      out.top_log_probs[n * P.top + j] = e.log_prob(x);
     } else {
       // (columns of the whole row; 0 where the part has fewer than top)
       split.best[(int64_t)blockIdx.x * P.top + j] = key == 0 ? 0 : key - (uint32_t)first;
     }
   };
-  for (int j = top + threadIdx.x; j < P.top; j += kThreads) put(j, 0);
+  for (int j = top + threadIdx.x; j < P.top; j += kThreads) put(j, 0, 0.0f);
+  // (64 groups: the top-th largest of their largest logits is a lower bound)
+  const float bound = top == 1 ? all : top_bound(groups[lane], top);
   if (p.s == p.s && bound > -INFINITY) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -371,19 +384,28 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
         const float f = to_float(x.x[r][v]);
         if (f >= bound) {
           const int at = atomicAdd(&total, 1);
-          if (at < kFound) found[at] = rank_key(f, x.column(r, v));
+          if (at < kFound) found[at] = Found{f, (uint32_t)x.column(r, v)};
         }
       }
     }
     __syncthreads();
     const int count = total;
+    // (the list's order depends on the run, the places do not)
+    if (count <= 64) {
+      if (w != 0) return;
+      const Found mine = lane < count ? found[lane] : Found{-INFINITY, ~0u};
+      const uint64_t k = rank_key(mine.x, mine.i);
+      const int place = place_among(k, count);
+      if (lane < count && place < top) put(place, k, mine.x);
+      return;
+    }
     if (count <= kFound) {
-      // (the list's order depends on the run, the places do not)
       if ((int)threadIdx.x < count) {
-        const uint64_t k = found[threadIdx.x];
+        const Found mine = found[threadIdx.x];
+        const uint64_t k = rank_key(mine.x, mine.i);
         int place = 0;
-        for (int j = 0; j < count; ++j) place += found[j] > k;
-        if (place < top) put(place, k);
+        for (int j = 0; j < count; ++j) place += rank_key(found[j].x, found[j].i) > k;
+        if (place < top) put(place, k, mine.x);
       }
       return;
     }
@@ -398,7 +420,7 @@ __global__ __launch_bounds__(64 * W) void probs_parts_kernel(
 #pragma unroll
     for (int q = 1; q < W; ++q) k = max64(k, best[q]);
     last = k;
-    if (threadIdx.x == 0) put(j, k);
+    if (threadIdx.x == 0) put(j, k, to_float(row[~(uint32_t)k]));
   }
 }
 
@@ -574,7 +596,7 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   constexpr int kR = 16 / V;  // vectors of 16 elements
   if (len <= 256 * kR) GS_PARTS(4, kR);
   else if (len <= 512 * kR) GS_PARTS(4, 2 * kR);
-  else GS_PARTS(8, 2 * kR);
+  else GS_PARTS(4, 4 * kR);
 #undef GS_PARTS
   const int rc = check_launch("probs_parts_kernel");
   if (rc || s.parts == 1) return rc;

@@ -39,7 +39,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 // The largest of three in one instruction (fmaxf first quiets each operand that
-// might be a signalling NaN, an instruction apiece).
+// might be a signalling NaN, an instruction apiece).  Not for an operand of a
+// cross-lane move: the compiler does not see that an instruction wrote it.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -87,6 +88,19 @@ __device__ __forceinline__ void store_vec(T* p, vec_t<T> v) {
   __builtin_memcpy(p, &v, 16);
 }
 
+// The same 16 bytes, of which the compiler no longer knows that it has them as
+// floats already: two passes over a row in registers convert its elements twice
+// rather than keep twice the registers.
+template <typename T>
+__device__ __forceinline__ void forget(vec_t<T>& v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    words w = __builtin_bit_cast(words, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(vec_t<T>, w);
+  }
+}
+
 // Elements i .. i + kVec - 1 of a row of n, `fill` past its end.
 template <typename T>
 __device__ __forceinline__ vec_t<T> load_part(const T* row, int i, int n, T fill) {
@@ -131,11 +145,14 @@ __device__ __forceinline__ uint32_t team_reduce(uint32_t v, Op op) {
   }
   return v;
 }
+// (As integers that keep the floats' order: one instruction a step.  A NaN is
+// above everything or, negative, below.)
 template <int L>
 __device__ __forceinline__ float team_max(float v) {
-  return __uint_as_float(team_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-  }));
+  const uint32_t u = __float_as_uint(v);
+  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  const uint32_t r = team_reduce<L>(k, [](uint32_t a, uint32_t b) { return max(a, b); });
+  return __uint_as_float(r ^ (~(uint32_t)((int32_t)r >> 31) | 0x80000000u));
 }
 template <int L>
 __device__ __forceinline__ float team_sum(float v) {
