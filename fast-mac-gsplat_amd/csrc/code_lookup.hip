@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
         y[v] = static_cast<T>(c[u] >= 0 ? to_float(x[u][v]) * s[u] : nan_for(c[u]));
     }
     if (at[u] + V <= total) {
-      store_vec(out + at[u], y);
+      store_vec_stream(out + at[u], y);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v)
@@ -331,6 +331,8 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
   bool coming = a < b && before == S.keys[a];
   const uint32_t head_key = before;
   bool head_ended = false, any_end = false;
+  vec_t<T> now[R];
+  uint32_t held = kNone;
   for (int64_t j0 = a; j0 < b; j0 += kRows) {
     uint32_t key[kRows + 1];
     int64_t n[kRows];
@@ -346,10 +348,18 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
       s[u] = scales ? scales[n[u]] : 1.0f;
       C::load(g[u], grad + n[u] * P.D, c0, P.D);
     }
-    if (dots)
+    if (dots) {
+      // (the codebook's row of each new run)
 #pragma unroll
-      for (int u = 0; u < kRows; ++u)
-        C::load(row[u], codebook + (int64_t)min(key[u], (uint32_t)P.K - 1) * P.stride, c0, P.D);
+      for (int u = 0; u < kRows; ++u) {
+        if (key[u] != held) {
+          C::load(now, codebook + (int64_t)min(key[u], (uint32_t)P.K - 1) * P.stride, c0, P.D);
+          held = key[u];
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) row[u][r] = now[r];
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       if (j0 + u >= b) break;

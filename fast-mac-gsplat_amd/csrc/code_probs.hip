@@ -308,7 +308,7 @@ struct Split {
 constexpr int kFound = 256;  // logits collected for the best ones
 
 template <typename T, int W, int R>
-__global__ __launch_bounds__(64 * W) void probs_parts_kernel(
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) void probs_parts_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out, Split split) {
   constexpr int kThreads = 64 * W;
   __shared__ Part parts[W];

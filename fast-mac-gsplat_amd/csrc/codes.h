@@ -88,6 +88,13 @@ __device__ __forceinline__ void store_vec(T* p, vec_t<T> v) {
   __builtin_memcpy(p, &v, 16);
 }
 
+// For what nothing reads soon: it leaves the caches to what is read again.
+template <typename T>
+__device__ __forceinline__ void store_vec_stream(T* p, vec_t<T> v) {
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(words, v), reinterpret_cast<words*>(p));
+}
+
 // The same 16 bytes, of which the compiler no longer knows that it has them as
 // floats already: two passes over a row in registers convert its elements twice
 // rather than keep twice the registers.
