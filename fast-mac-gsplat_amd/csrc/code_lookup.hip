@@ -333,21 +333,32 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
   bool head_ended = false, any_end = false;
   vec_t<T> now[R];
   uint32_t held = kNone;
+  // (the next rows' codes and places are loaded while these rows are on their way)
+  uint32_t key[kRows + 1], key_next[kRows];
+  int n[kRows], n_next[kRows];
+  auto look = [&](int64_t j0) {
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      key_next[u] = S.keys[min(j0 + u, P.rows - 1)];
+      n_next[u] = (int)S.order[min(j0 + u, P.rows - 1)];
+    }
+  };
+  if (a < b) look(a);
   for (int64_t j0 = a; j0 < b; j0 += kRows) {
-    uint32_t key[kRows + 1];
-    int64_t n[kRows];
     float s[kRows];
     vec_t<T> g[kRows][R], row[kRows][R];
 #pragma unroll
-    for (int u = 0; u <= kRows; ++u)
-      key[u] = j0 + u < P.rows ? S.keys[j0 + u] : kNone;
-#pragma unroll
-    for (int u = 0; u < kRows; ++u) n[u] = S.order[min(j0 + u, b - 1)];
+    for (int u = 0; u < kRows; ++u) {
+      key[u] = key_next[u];
+      n[u] = n_next[u];
+    }
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       s[u] = scales ? scales[n[u]] : 1.0f;
-      C::load(g[u], grad + n[u] * P.D, c0, P.D);
+      C::load(g[u], grad + (int64_t)n[u] * P.D, c0, P.D);
     }
+    look(j0 + kRows);
+    key[kRows] = key_next[0];
     if (dots) {
       // (the codebook's row of each new run)
 #pragma unroll
@@ -377,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
         if (C::lane() == 0)
           g_scales[n[u]] = key[u] < (uint32_t)P.K ? dot : nan_for(P.codes.at(n[u], P.K));
       }
-      if (key[u] != key[u + 1]) {  // the run ends
+      if (key[u] != key[u + 1] || j0 + u + 1 == P.rows) {  // the run ends
         any_end = true;
         if (coming) {
           coming = false;
@@ -547,6 +558,8 @@ __global__ __launch_bounds__(kThreads) void lookup_scales_kernel(
   if (vecs <= 64) CALL(64, 1)    \
   CALL(64, 2)
 
+constexpr int64_t kBlocksWanted = 8192;
+
 int vec_of(const LookupParams& P) { return P.dtype == GSPLAT_F32 ? 4 : 8; }
 int vecs_of(const LookupParams& P) { return (P.D + vec_of(P) - 1) / vec_of(P); }
 int lanes_of(const LookupParams& P) {
@@ -575,7 +588,7 @@ Layout layout(const LookupParams& P) {
   // Positions per team: 4 to 64, about 2048 workgroups.
   const int tl = lanes_of(P);
   L.piece = 4;
-  while (L.piece < 64 && P.rows * tl > (int64_t)L.piece * kThreads * 2048) L.piece *= 2;
+  while (L.piece < 64 && P.rows * tl > (int64_t)L.piece * kThreads * kBlocksWanted) L.piece *= 2;
   L.span = L.piece * (kThreads / tl);
   L.blocks = (int)((P.rows + L.span - 1) / L.span);
   size_t off = 0;
