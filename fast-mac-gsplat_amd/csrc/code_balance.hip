@@ -20,10 +20,12 @@ namespace gs {
 namespace {
 
 // A team reads a row once and holds it in registers: TL lanes of one wavefront
-// (W = 1), or W wavefronts.  A thread holds R vectors, at most 16 elements, of
-// the row at hand, its probabilities and (forward) its columns' sums or
-// (backward) its columns' a; the next row is loaded while this one is worked
-// on.
+// (W = 1), or W wavefronts.  A thread holds R vectors, 16 elements of most rows
+// and 32 of those above 1024 codes, of the row at hand, its probabilities and
+// (forward) its columns' sums or (backward) its columns' a; the next row is
+// loaded while this one is worked on.  What a row costs besides its elements
+// (reductions, its choices) is the same for a lane with 4 elements and one
+// with 32, so teams are as narrow as that allows.
 template <typename T, int TL, int W, int R>
 struct Team {
   static constexpr int V = kVec<T>;
@@ -123,40 +125,48 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
 
     float m = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      float most = to_float(x[r][0]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) m = fmaxf(m, to_float(x[r][v]));
+      for (int v = 1; v + 1 < V; v += 2) most = max3(most, to_float(x[r][v]), to_float(x[r][v + 1]));
+      m = max3(m, most, to_float(x[r][V - 1]));
+      forget<T>(x[r]);
+    }
     m = team_max<TL>(m);
-    float base = m == -INFINITY ? 0.0f : m;
+    const Exponent ex(m == -INFINITY ? 0.0f : m, 0.0f, c);
     float e[R * V], s = 0.0f;
+    auto powers = [&](auto exponent) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        e[r * V + v] = exp2_fast((to_float(x[r][v]) - base) * c);
-        s += e[r * V + v];
-      }
+        for (int v = 0; v < V; ++v) {
+          e[r * V + v] = exp2_fast(exponent(to_float(x[r][v])));
+          s += e[r * V + v];
+        }
+    };
+    if (ex.plain)
+      powers([&](float y) { return ex.fast(y); });
+    else
+      powers([&](float y) { return ex.slow(y); });
     s = team_sum<TL>(s);
-    float scale = 1.0f;
+    // (the powers lack ex.shift: it cancels from e / s, not from log2 s)
+    float base = ex.m, shift = ex.shift, f = 1.0f;
     if constexpr (W > 1) {  // (two sets of slots: one barrier a row)
       float2* slot = slots[turn & 1];
-      if (lane == 0) slot[w] = make_float2(m, s);
+      if (lane == 0) slot[w] = make_float2(m, s * exp2_fast(shift));
       __syncthreads();
-      float all = slot[0].x;
-#pragma unroll
-      for (int j = 1; j < W; ++j) all = fmaxf(all, slot[j].x);
-      const float b_all = all == -INFINITY ? 0.0f : all;
-      s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        s += slot[j].y * exp2_fast(fmaxf((slot[j].x - b_all) * c, -1000.0f));
-      scale = exp2_fast(fmaxf((m - b_all) * c, -1000.0f));
-      base = b_all;
+      const float2 q = slot[lane & (W - 1)];
+      const float all = team_max<W>(q.x);
+      base = all == -INFINITY ? 0.0f : all;
+      s = team_sum<W>(q.y * exp2_fast(fmaxf((q.x - base) * c, -1000.0f)));
+      f = exp2_fast(fmaxf((m - base) * c, -1000.0f) + shift);
+      shift = 0.0f;
     }
-    const float inv = part && s != 0.0f ? 1.0f / s : 0.0f;
-    if (here && G::member() == 0) stats[r0] = make_float2(base, inv);
-    if (here && inv != 0.0f) {
-      const float f = scale * inv;
+    const bool counts_in = here && part && s != 0.0f;
+    if (here && G::member() == 0)
+      stats[r0] = make_float2(base, counts_in ? log2_fast(s) + shift : INFINITY);
+    if (counts_in) {
+      f *= __builtin_amdgcn_rcpf(s);
 #pragma unroll
       for (int j = 0; j < R * V; ++j) acc[j] = __builtin_fmaf(e[j], f, acc[j]);
     }
@@ -293,6 +303,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
     const float* __restrict__ g_mean, T* __restrict__ g_logits) {
   using G = Team<T, TL, W, R>;
   constexpr int V = G::V;
+  constexpr float kUp = sizeof(T) == 2 ? 32.0f : 0.0f;
   __shared__ float slots[2][W];
   const int b = blockIdx.y;
   const int64_t per = (P.rows + gridDim.x - 1) / gridDim.x;
@@ -329,34 +340,43 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
       G::load(next, logits + rn * P.stride, P.K);
       st_next = stats[rn];
     }
+    // p = 2^(t + down) with t from Exponent (16 bits: exponents 32 up, as in
+    // code_probs.hip); a row that takes no part has log2 s = inf and p = 0.
+    const Exponent ex(st.x, st.y - kUp, kLog2e);
+    const float down = exp2_fast(ex.shift - kUp);
     float p[R * V], dot = 0.0f;
-    const bool some = st.y != 0.0f;  // (else the row has no probabilities)
+    auto products = [&](auto exponent) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int j = r * V + v;
-        p[j] = some ? exp2_full((to_float(x[r][v]) - st.x) * kLog2e) * st.y : 0.0f;
-        dot = __builtin_fmaf(p[j], a[j], dot);
-      }
-    dot = team_sum<TL>(dot);
+        for (int v = 0; v < V; ++v) {
+          const int j = r * V + v;
+          const float t = exponent(to_float(x[r][v]));
+          p[j] = sizeof(T) == 2 ? exp2_fast(t) : exp2_full(t);
+          dot = __builtin_fmaf(p[j], a[j], dot);
+        }
+    };
+    if (ex.plain)
+      products([&](float y) { return ex.fast(y); });
+    else
+      products([&](float y) { return ex.slow(y); });
+    dot = team_sum<TL>(dot) * down;
     if constexpr (W > 1) {
       float* slot = slots[turn & 1];
       if (lane == 0) slot[w] = dot;
       __syncthreads();
-      dot = slot[0];
-#pragma unroll
-      for (int j = 1; j < W; ++j) dot += slot[j];
+      dot = team_sum<W>(slot[lane & (W - 1)]);
     }
     if (i < count) {
       T* out = g_logits + r0 * P.K;
+      const float f = down * per_row, less = -dot * f;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         vec_t<T> o;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int j = r * V + v;
-          o[v] = static_cast<T>(p[j] * (a[j] - dot) * per_row);
+          o[v] = static_cast<T>(p[j] * __builtin_fmaf(a[j], f, less));
         }
         store_part<T>(out, G::column(r), P.K, o);
       }
@@ -374,7 +394,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 
 __device__ __forceinline__ float prob(float x, float2 st) {
-  return st.y == 0.0f ? 0.0f : exp2_full((x - st.x) * kLog2e) * st.y;
+  return exp2_full((x - st.x) * kLog2e - st.y);
 }
 
 // A workgroup per row.  The only counts and totals of an image: zero on entry.
@@ -415,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void balance_long_rows_kernel(
   s = 0.0f;
   for (int j = 0; j < kWaves; ++j)
     s += slots[j].y * exp2_fast(fmaxf((slots[j].x - base) * kLog2e, -1000.0f));
-  stats[r] = make_float2(base, part && s != 0.0f ? 1.0f / s : 0.0f);
+  stats[r] = make_float2(base, part && s != 0.0f ? log2_fast(s) : INFINITY);
   if (part) atomicAdd(&out.totals[b].x, 1);
 }
 
@@ -494,7 +514,7 @@ int blocks_of(const BalanceParams& P) {
   if (P.rows == 0) return 1;
   if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
   const int64_t least = P.dtype == GSPLAT_F32 ? 8 : 16;
-  const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 256 : P.K > 4096 ? 512 : 1024) / P.batch);
+  const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 512 : 1024) / P.batch);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, P.rows / least));
 }
 
@@ -524,19 +544,18 @@ Layout layout(const BalanceParams& P) {
 
 // The kernel for rows of K codes: CALL(TL, W, R).
 #define GS_TEAMS(CALL)                                              \
-  if (vecs <= 2) CALL(2, 1, 1);                                     \
-  if (vecs <= 4) CALL(4, 1, 1);                                     \
-  if (vecs <= 8) CALL(8, 1, 1);                                     \
-  if (vecs <= 16) CALL(16, 1, 1);                                   \
-  if (vecs <= 32) CALL(32, 1, 1);                                   \
-  if (vecs <= 64) CALL(64, 1, 1);                                   \
-  if (vecs <= 128) CALL(64, 1, 2);                                  \
   constexpr int kR = 16 / kVec<T>;                                  \
+  if (vecs <= 2) CALL(2, 1, 1);                                     \
+  if (vecs <= 2 * kR) CALL(2, 1, kR);                               \
+  if (vecs <= 4 * kR) CALL(4, 1, kR);                               \
+  if (vecs <= 8 * kR) CALL(8, 1, kR);                               \
+  if (vecs <= 16 * kR) CALL(16, 1, kR);                             \
+  if (vecs <= 32 * kR) CALL(32, 1, kR);                             \
   if (vecs <= 64 * kR) CALL(64, 1, kR);                             \
-  if (vecs <= 128 * kR) CALL(64, 2, kR);                            \
-  if (vecs <= 256 * kR) CALL(64, 4, kR);                            \
-  if (vecs <= 512 * kR) CALL(64, 8, kR);                            \
-  CALL(64, 16, kR);
+  if (vecs <= 128 * kR) CALL(64, 1, 2 * kR);                        \
+  if (vecs <= 256 * kR) CALL(64, 2, 2 * kR);                        \
+  if (vecs <= 512 * kR) CALL(64, 4, 2 * kR);                        \
+  CALL(64, 8, 2 * kR);
 
 template <typename T>
 int rows_of(const BalanceParams& P, const T* x, float2* stats, const Partials& w,
@@ -614,7 +633,7 @@ int backward_of(const BalanceParams& P, const void* logits, const int32_t* count
 #define GS_BWD(TL, W, R)                                                      \
   {                                                                           \
     using G = Team<T, TL, W, R>;                                              \
-    const int64_t most = std::max(1, (W > 4 ? 4096 / W : 1024) / P.batch);         \
+    const int64_t most = std::max(1, (W > 4 ? 512 : 1024) / P.batch);         \
     const int64_t turns = (P.rows + G::kTeams - 1) / G::kTeams;               \
     launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T, TL, W, R>),    \
                   dim3((unsigned)std::min(most, turns), (unsigned)P.batch),   \
