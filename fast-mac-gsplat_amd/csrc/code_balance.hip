@@ -21,24 +21,29 @@ namespace {
 
 // A team reads a row once and holds it in registers: TL lanes of one wavefront
 // (W = 1), or W wavefronts.  A thread holds R vectors, 16 elements of most rows
-// and 32 of those above 1024 codes, of the row at hand, its probabilities and
+// and 32 of those above 1024 codes in 16 bits, of the row at hand, its probabilities and
 // (forward) its columns' sums or (backward) its columns' a; the next row is
-// loaded while this one is worked on.  What a row costs besides its elements
+// loaded once its probabilities are there.  What a row costs besides its elements
 // (reductions, its choices) is the same for a lane with 4 elements and one
 // with 32, so teams are as narrow as that allows.
-template <typename T, int TL, int W, int R>
+//
+// (Four wavefronts per SIMD: the compiler would otherwise take more registers
+// than it needs with 32 elements a lane.)
+#define GS_WAVES __attribute__((amdgpu_waves_per_eu(4)))
+template <typename T, int TL, int W, int R, bool Even>
 struct Team {
   static constexpr int V = kVec<T>;
-  static constexpr int kThreads = W > 1 ? 64 * W : 256;
+  static constexpr int kThreads = W > 4 ? 64 * W : 256;
   static constexpr int kTeams = kThreads / (TL * W);  // per workgroup
   static constexpr int kColumns = TL * W * V * R;
   static __device__ __forceinline__ int team() { return threadIdx.x / (TL * W); }
   static __device__ __forceinline__ int member() { return threadIdx.x & (TL * W - 1); }
+  static __device__ __forceinline__ int wave() { return W > 1 ? (threadIdx.x >> 6) & (W - 1) : 0; }
   static __device__ __forceinline__ int column(int r) { return (r * TL * W + member()) * V; }
   static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int K) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T>(row, column(r), K, static_cast<T>(-INFINITY));
+      x[r] = load_part<T, Even>(row, column(r), K, static_cast<T>(-INFINITY));
   }
 };
 
@@ -67,14 +72,14 @@ struct Choices {
   }
 };
 
-template <typename T, int TL, int W, int R>
-__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
+template <typename T, int TL, int W, int R, bool Even>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_kernel(
     BalanceParams P, const T* __restrict__ logits, float2* __restrict__ stats,
     Partials out) {
-  using G = Team<T, TL, W, R>;
+  using G = Team<T, TL, W, R, Even>;
   constexpr int V = G::V;
   extern __shared__ int32_t lds[];  // K counts, then (teams > 1) K sums
-  __shared__ float2 slots[2][W];
+  __shared__ float2 slots[2][G::kTeams][W];
   __shared__ int sum4[3];
   int32_t* hist = lds;
   float* sums = reinterpret_cast<float*>(lds + P.K);
@@ -88,17 +93,17 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
   __syncthreads();
 
   const float c = kLog2e;
-  const int lane = threadIdx.x & (TL - 1), w = W > 1 ? threadIdx.x >> 6 : 0;
+  const int lane = threadIdx.x & (TL - 1), w = G::wave();
   const int S = P.choices;
   float acc[R * V];
 #pragma unroll
   for (int j = 0; j < R * V; ++j) acc[j] = 0.0f;
   int took = 0, given = 0, bad = 0;
-  vec_t<T> x[R], next[R];
+  vec_t<T> x[R];
   const int64_t base_row = b * P.rows + first;
   auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
   int64_t i = G::team();
-  int code = kNoCode, code_next = kNoCode;
+  int code = kNoCode;
   if (count > 0) {
     G::load(x, logits + row_of(i) * P.stride, P.K);
     if (lane < S) code = P.codes.at(row_of(i) * S + lane, P.K);
@@ -107,11 +112,6 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
   for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
     const int64_t r0 = row_of(i);
     const bool here = i < count;
-    if ((turn + 1) * G::kTeams < count) {
-      const int64_t rn = row_of(i + G::kTeams);
-      G::load(next, logits + rn * P.stride, P.K);
-      code_next = lane < S ? P.codes.at(rn * S + lane, P.K) : kNoCode;
-    }
     Choices mine;
     if (here) {
       int32_t* h = w == 0 ? hist : nullptr;
@@ -130,29 +130,35 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
 #pragma unroll
       for (int v = 1; v + 1 < V; v += 2) most = max3(most, to_float(x[r][v]), to_float(x[r][v + 1]));
       m = max3(m, most, to_float(x[r][V - 1]));
-      forget<T>(x[r]);
     }
     m = team_max<TL>(m);
     const Exponent ex(m == -INFINITY ? 0.0f : m, 0.0f, c);
     float e[R * V], s = 0.0f;
     auto powers = [&](auto exponent) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        forget<T>(x[r]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           e[r * V + v] = exp2_fast(exponent(to_float(x[r][v])));
           s += e[r * V + v];
         }
+      }
     };
     if (ex.plain)
       powers([&](float y) { return ex.fast(y); });
     else
       powers([&](float y) { return ex.slow(y); });
+    if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
+      const int64_t rn = row_of(i + G::kTeams);
+      G::load(x, logits + rn * P.stride, P.K);
+      code = lane < S ? P.codes.at(rn * S + lane, P.K) : kNoCode;
+    }
     s = team_sum<TL>(s);
     // (the powers lack ex.shift: it cancels from e / s, not from log2 s)
     float base = ex.m, shift = ex.shift, f = 1.0f;
     if constexpr (W > 1) {  // (two sets of slots: one barrier a row)
-      float2* slot = slots[turn & 1];
+      float2* slot = slots[turn & 1][W > 1 ? G::team() : 0];
       if (lane == 0) slot[w] = make_float2(m, s * exp2_fast(shift));
       __syncthreads();
       const float2 q = slot[lane & (W - 1)];
@@ -170,9 +176,6 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
 #pragma unroll
       for (int j = 0; j < R * V; ++j) acc[j] = __builtin_fmaf(e[j], f, acc[j]);
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = next[r];
-    code = code_next;
   }
 
   // rows, choices and bad codes of the workgroup (wavefront 0 of a wide team)
@@ -188,15 +191,15 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_rows_kernel(
   }
   const int64_t at = (int64_t)b * out.blocks + blockIdx.x;
   if constexpr (G::kTeams > 1) {
-    // teams of a wavefront, then the wavefronts one after another
+    // teams of a wavefront, then wavefronts or wider teams one after another
     if constexpr (TL < 64)
 #pragma unroll
       for (int j = 0; j < R * V; ++j)
 #pragma unroll
         for (int d = TL; d < 64; d <<= 1) acc[j] += __shfl_xor(acc[j], d, 64);
-    const int wave = threadIdx.x >> 6;
-    for (int q = 0; q < G::kThreads / 64; ++q) {
-      if (wave == q && (threadIdx.x & 63) < TL)
+    const int group = threadIdx.x / (64 * W);
+    for (int q = 0; q < G::kThreads / (64 * W); ++q) {
+      if (group == q && (threadIdx.x & 63) < TL)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -295,22 +298,22 @@ __global__ __launch_bounds__(64 * kJoinWaves) void balance_join_kernel(
 
 // ---- backward
 
-template <typename T, int TL, int W, int R>
-__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
+template <typename T, int TL, int W, int R, bool Even>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_kernel(
     BalanceParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ counts, const float2* __restrict__ stats,
     const int4* __restrict__ totals, const float* __restrict__ g_loss,
     const float* __restrict__ g_mean, T* __restrict__ g_logits) {
-  using G = Team<T, TL, W, R>;
+  using G = Team<T, TL, W, R, Even>;
   constexpr int V = G::V;
   constexpr float kUp = sizeof(T) == 2 ? 32.0f : 0.0f;
-  __shared__ float slots[2][W];
+  __shared__ float slots[2][G::kTeams][W];
   const int b = blockIdx.y;
   const int64_t per = (P.rows + gridDim.x - 1) / gridDim.x;
   const int64_t first = blockIdx.x * per;
   const int64_t count = min(per, P.rows - first);
   if (count <= 0) return;
-  const int lane = threadIdx.x & (TL - 1), w = W > 1 ? threadIdx.x >> 6 : 0;
+  const int lane = threadIdx.x & (TL - 1), w = G::wave();
   const int4 tot = totals[b];
   const float per_row = 1.0f / (float)max(tot.x, 1);
   const float per_count = g_loss ? g_loss[b] * ((float)P.K / (float)max(tot.y, 1)) : 0.0f;
@@ -330,16 +333,11 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
   const int64_t base_row = b * P.rows + first;
   auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
   int64_t i = G::team();
-  vec_t<T> x[R], next[R];
+  vec_t<T> x[R];
   G::load(x, logits + row_of(i) * P.stride, P.K);
-  float2 st = stats[row_of(i)], st_next = st;
+  float2 st = stats[row_of(i)];
   for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
     const int64_t r0 = row_of(i);
-    if ((turn + 1) * G::kTeams < count) {
-      const int64_t rn = row_of(i + G::kTeams);
-      G::load(next, logits + rn * P.stride, P.K);
-      st_next = stats[rn];
-    }
     // p = 2^(t + down) with t from Exponent (16 bits: exponents 32 up, as in
     // code_probs.hip); a row that takes no part has log2 s = inf and p = 0.
     const Exponent ex(st.x, st.y - kUp, kLog2e);
@@ -347,7 +345,8 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
     float p[R * V], dot = 0.0f;
     auto products = [&](auto exponent) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        forget<T>(x[r]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int j = r * V + v;
@@ -355,14 +354,20 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
           p[j] = sizeof(T) == 2 ? exp2_fast(t) : exp2_full(t);
           dot = __builtin_fmaf(p[j], a[j], dot);
         }
+      }
     };
     if (ex.plain)
       products([&](float y) { return ex.fast(y); });
     else
       products([&](float y) { return ex.slow(y); });
+    if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
+      const int64_t rn = row_of(i + G::kTeams);
+      G::load(x, logits + rn * P.stride, P.K);
+      st = stats[rn];
+    }
     dot = team_sum<TL>(dot) * down;
     if constexpr (W > 1) {
-      float* slot = slots[turn & 1];
+      float* slot = slots[turn & 1][W > 1 ? G::team() : 0];
       if (lane == 0) slot[w] = dot;
       __syncthreads();
       dot = team_sum<W>(slot[lane & (W - 1)]);
@@ -378,12 +383,9 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_bwd_kernel(
           const int j = r * V + v;
           o[v] = static_cast<T>(p[j] * __builtin_fmaf(a[j], f, less));
         }
-        store_part<T>(out, G::column(r), P.K, o);
+        store_part<T, Even>(out, G::column(r), P.K, o);
       }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = next[r];
-    st = st_next;
   }
 }
 
@@ -514,7 +516,7 @@ int blocks_of(const BalanceParams& P) {
   if (P.rows == 0) return 1;
   if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
   const int64_t least = P.dtype == GSPLAT_F32 ? 8 : 16;
-  const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 512 : 1024) / P.batch);
+  const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 256 : P.K > 4096 ? 512 : 1024) / P.batch);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, P.rows / least));
 }
 
@@ -552,19 +554,26 @@ Layout layout(const BalanceParams& P) {
   if (vecs <= 16 * kR) CALL(16, 1, kR);                             \
   if (vecs <= 32 * kR) CALL(32, 1, kR);                             \
   if (vecs <= 64 * kR) CALL(64, 1, kR);                             \
-  if (vecs <= 128 * kR) CALL(64, 1, 2 * kR);                        \
-  if (vecs <= 256 * kR) CALL(64, 2, 2 * kR);                        \
-  if (vecs <= 512 * kR) CALL(64, 4, 2 * kR);                        \
-  CALL(64, 8, 2 * kR);
+  if constexpr (sizeof(T) == 2 && Even) {                           \
+    if (vecs <= 128 * kR) CALL(64, 1, 2 * kR);                      \
+    if (vecs <= 256 * kR) CALL(64, 2, 2 * kR);                      \
+    if (vecs <= 512 * kR) CALL(64, 4, 2 * kR);                      \
+    CALL(64, 8, 2 * kR);                                            \
+  } else {                                                          \
+    if (vecs <= 128 * kR) CALL(64, 2, kR);                          \
+    if (vecs <= 256 * kR) CALL(64, 4, kR);                          \
+    if (vecs <= 512 * kR) CALL(64, 8, kR);                          \
+    CALL(64, 16, kR);                                               \
+  }
 
-template <typename T>
+template <typename T, bool Even>
 int rows_of(const BalanceParams& P, const T* x, float2* stats, const Partials& w,
             hipStream_t stream) {
   const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
 #define GS_ROWS(TL, W, R)                                                     \
   {                                                                           \
-    using G = Team<T, TL, W, R>;                                              \
-    launch_traced("balance_rows_kernel", (balance_rows_kernel<T, TL, W, R>),  \
+    using G = Team<T, TL, W, R, Even>;                                              \
+    launch_traced("balance_rows_kernel", (balance_rows_kernel<T, TL, W, R, Even>),  \
                   dim3((unsigned)w.blocks, (unsigned)P.batch), dim3(G::kThreads), \
                   (size_t)P.K * (G::kTeams > 1 ? 8 : 4), stream, P, x, stats, w); \
     return check_launch("balance_rows_kernel");                               \
@@ -588,7 +597,8 @@ int forward_of(const BalanceParams& P, const void* logits, float* loss,
              reinterpret_cast<uint32_t*>(ws + L.tickets)};
   int rc;
   if (!is_long) {
-    rc = rows_of<T>(P, x, stats, w, stream);
+    rc = P.K % kVec<T> == 0 ? rows_of<T, true>(P, x, stats, w, stream)
+                            : rows_of<T, false>(P, x, stats, w, stream);
   } else {
     // (one launch zeroes counts, totals, the loss' parts and the tickets; the
     // sums of no rows are zeroed too)
@@ -617,25 +627,17 @@ int forward_of(const BalanceParams& P, const void* logits, float* loss,
   return check_launch("balance_join_kernel");
 }
 
-template <typename T>
-int backward_of(const BalanceParams& P, const void* logits, const int32_t* counts,
-                const float2* stats, const int4* totals, const float* g_loss,
-                const float* g_mean, void* g_logits, hipStream_t stream) {
-  const T* x = static_cast<const T*>(logits);
-  T* g = static_cast<T*>(g_logits);
-  if (P.K > kLongest) {
-    launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T>),
-                  dim3((unsigned)(P.rows * P.batch)), dim3(kThreads), 0, stream, P, x,
-                  counts, stats, totals, g_loss, g_mean, g);
-    return check_launch("balance_long_bwd_kernel");
-  }
+template <typename T, bool Even>
+int gradients_of(const BalanceParams& P, const T* x, const int32_t* counts,
+                 const float2* stats, const int4* totals, const float* g_loss,
+                 const float* g_mean, T* g, hipStream_t stream) {
   const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
 #define GS_BWD(TL, W, R)                                                      \
   {                                                                           \
-    using G = Team<T, TL, W, R>;                                              \
-    const int64_t most = std::max(1, (W > 4 ? 512 : 1024) / P.batch);         \
+    using G = Team<T, TL, W, R, Even>;                                              \
+    const int64_t most = std::max(1, (W > 4 ? 4096 / W : 1024) / P.batch);         \
     const int64_t turns = (P.rows + G::kTeams - 1) / G::kTeams;               \
-    launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T, TL, W, R>),    \
+    launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T, TL, W, R, Even>),    \
                   dim3((unsigned)std::min(most, turns), (unsigned)P.batch),   \
                   dim3(G::kThreads), 0, stream, P, x, counts, stats, totals,  \
                   g_loss, g_mean, g);                                         \
@@ -645,6 +647,22 @@ int backward_of(const BalanceParams& P, const void* logits, const int32_t* count
 #undef GS_BWD
 }
 #undef GS_TEAMS
+
+template <typename T>
+int backward_of(const BalanceParams& P, const void* logits, const int32_t* counts,
+                const float2* stats, const int4* totals, const float* g_loss,
+                const float* g_mean, void* g_logits, hipStream_t stream) {
+  const T* x = static_cast<const T*>(logits);
+  T* g = static_cast<T*>(g_logits);
+  if (P.K <= kLongest)
+    return P.K % kVec<T> == 0
+               ? gradients_of<T, true>(P, x, counts, stats, totals, g_loss, g_mean, g, stream)
+               : gradients_of<T, false>(P, x, counts, stats, totals, g_loss, g_mean, g, stream);
+  launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T>),
+                dim3((unsigned)(P.rows * P.batch)), dim3(kThreads), 0, stream, P, x,
+                counts, stats, totals, g_loss, g_mean, g);
+  return check_launch("balance_long_bwd_kernel");
+}
 
 }  // namespace
 

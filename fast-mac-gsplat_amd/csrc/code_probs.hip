@@ -131,7 +131,7 @@ __device__ __forceinline__ void write_row(const ProbsOut& out, int64_t n, Part p
 
 // The elements that a thread of a team of TL holds: vectors r = 0..R-1 of the
 // team's rows of TL vectors.
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 struct Held {
   static constexpr int V = kVec<T>;
   vec_t<T> x[R];
@@ -140,7 +140,7 @@ struct Held {
     lane = lane_;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
+      x[r] = load_part<T, Even>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
   }
   __device__ __forceinline__ int column(int r, int v) const { return (r * TL + lane) * V + v; }
   __device__ __forceinline__ void forget() {
@@ -201,7 +201,7 @@ struct Held {
 
 // ---- rows of at most TL * kVec * R codes: a team of TL lanes per row
 
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out) {
   constexpr int kTeams = kThreads / TL;
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
   const bool active = n < P.rows;
   if (!active) n = P.rows - 1;  // (its lanes go along)
   const T* row = logits + n * P.stride;
-  Held<T, TL, R> x;
+  Held<T, TL, R, Even> x;
   x.load(row, lane, P.K);
   const int code = P.codes.p ? P.codes.at(n, P.K) : kNoCode;
   float most[R];  // of each vector
@@ -307,7 +307,7 @@ struct Split {
 
 constexpr int kFound = 256;  // logits collected for the best ones
 
-template <typename T, int W, int R>
+template <typename T, int W, int R, bool Even>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) void probs_parts_kernel(
     ProbsParams P, const T* __restrict__ logits, ProbsOut out, Split split) {
   constexpr int kThreads = 64 * W;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) voi
   const int len = min(split.length, P.K - first);
   const T* row = logits + n * P.stride;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  Held<T, kThreads, R> x;
+  Held<T, kThreads, R, Even> x;
   x.load(row + first, threadIdx.x, len);
   const int code = P.codes.p && split.parts == 1 ? P.codes.at(n, P.K) : kNoCode;
   float most[R];  // of each vector
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(64) void probs_join_kernel(
 // Exponent, and everything that is the same for the row is in two constants.
 // A team of TL lanes per part of a row of TL * kVec * R columns (`parts` of
 // them per row).
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     ProbsParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ top_codes, const float2* __restrict__ stats,
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   vec_t<T> x[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    x[r] = load_part<T>(row, first + (r * TL + lane) * V, P.K, static_cast<T>(-INFINITY));
+    x[r] = load_part<T, Even>(row, first + (r * TL + lane) * V, P.K, static_cast<T>(-INFINITY));
   const float2 st = stats[n];
   const bool some = st.y != INFINITY;  // (else p = 0 everywhere)
   const float ge = g_entropy && some ? g_entropy[n] : 0.0f;
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     vec_t<T> o;
 #pragma unroll
     for (int v = 0; v < V; ++v) o[v] = static_cast<T>(g[r * V + v]);
-    store_part<T>(out, first + (r * TL + lane) * V, P.K, o);
+    store_part<T, Even>(out, first + (r * TL + lane) * V, P.K, o);
   }
 }
 
@@ -565,7 +565,7 @@ Split split_of(const ProbsParams& P) {
   return s;
 }
 
-template <typename T>
+template <typename T, bool Even>
 int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
                void* workspace, hipStream_t stream) {
   const T* x = static_cast<const T*>(logits);
@@ -573,7 +573,7 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   const int vecs = (P.K + V - 1) / V;
 #define GS_ROWS(TL, R)                                                           \
   if (vecs <= TL * R) {                                                          \
-    launch_traced("probs_rows_kernel", (probs_rows_kernel<T, TL, R>),            \
+    launch_traced("probs_rows_kernel", (probs_rows_kernel<T, TL, R, Even>),            \
                   dim3((unsigned)((P.rows + kThreads / TL - 1) / (kThreads / TL))), \
                   dim3(kThreads), 0, stream, P, x, out);                         \
     return check_launch("probs_rows_kernel");                                    \
@@ -591,7 +591,7 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   const dim3 grid((unsigned)(P.rows * s.parts));
   const int len = (s.length + V - 1) / V;
 #define GS_PARTS(W, R)                                                         \
-  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, W, R>), grid,     \
+  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, W, R, Even>), grid,     \
                 dim3(64 * W), 0, stream, P, x, out, s)
   constexpr int kR = 16 / V;  // vectors of 16 elements
   if (len <= 256 * kR) GS_PARTS(4, kR);
@@ -605,7 +605,7 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   return check_launch("probs_join_kernel");
 }
 
-template <typename T>
+template <typename T, bool Even>
 int backward_of(const ProbsParams& P, const void* logits, const int32_t* top_codes,
                 const float2* stats, const float* entropy,
                 const float* g_log_probs, const float* g_entropy,
@@ -617,7 +617,7 @@ int backward_of(const ProbsParams& P, const void* logits, const int32_t* top_cod
   {                                                                            \
     const int parts = (vecs + TL * R - 1) / (TL * R);                          \
     const int64_t teams = P.rows * parts, per = kThreads / TL;                 \
-    launch_traced("probs_bwd_kernel", (probs_bwd_kernel<T, TL, R>),            \
+    launch_traced("probs_bwd_kernel", (probs_bwd_kernel<T, TL, R, Even>),            \
                   dim3((unsigned)((teams + per - 1) / per)), dim3(kThreads), 0, \
                   stream, P, x, top_codes, stats, entropy, g_log_probs,        \
                   g_entropy, g_top, g, parts);                                 \
@@ -648,9 +648,10 @@ int launch_probs_forward(const ProbsParams& P, const void* logits,
                          int32_t* top_codes, float2* stats, void* workspace,
                          hipStream_t stream) {
   if (P.rows == 0) return GSPLAT_OK;
-  auto f = P.dtype == GSPLAT_F32    ? forward_of<float>
-           : P.dtype == GSPLAT_BF16 ? forward_of<__bf16>
-                                    : forward_of<_Float16>;
+  const bool even = P.K % (P.dtype == GSPLAT_F32 ? 4 : 8) == 0;
+  auto f = P.dtype == GSPLAT_F32    ? (even ? forward_of<float, true> : forward_of<float, false>)
+           : P.dtype == GSPLAT_BF16 ? (even ? forward_of<__bf16, true> : forward_of<__bf16, false>)
+                                    : (even ? forward_of<_Float16, true> : forward_of<_Float16, false>);
   return f(P, logits, ProbsOut{log_probs, entropy, top_log_probs, top_codes, stats},
            workspace, stream);
 }
@@ -661,9 +662,10 @@ int launch_probs_backward(const ProbsParams& P, const void* logits,
                           const float* g_entropy, const float* g_top,
                           void* g_logits, hipStream_t stream) {
   if (P.rows == 0) return GSPLAT_OK;
-  auto f = P.dtype == GSPLAT_F32    ? backward_of<float>
-           : P.dtype == GSPLAT_BF16 ? backward_of<__bf16>
-                                    : backward_of<_Float16>;
+  const bool even = P.K % (P.dtype == GSPLAT_F32 ? 4 : 8) == 0;
+  auto f = P.dtype == GSPLAT_F32    ? (even ? backward_of<float, true> : backward_of<float, false>)
+           : P.dtype == GSPLAT_BF16 ? (even ? backward_of<__bf16, true> : backward_of<__bf16, false>)
+                                    : (even ? backward_of<_Float16, true> : backward_of<_Float16, false>);
   return f(P, logits, top_codes, stats, entropy, g_log_probs, g_entropy, g_top,
            g_logits, stream);
 }

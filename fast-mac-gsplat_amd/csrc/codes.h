@@ -108,21 +108,25 @@ __device__ __forceinline__ void forget(vec_t<T>& v) {
   }
 }
 
-// Elements i .. i + kVec - 1 of a row of n, `fill` past its end.
-template <typename T>
+// Elements i .. i + kVec - 1 of a row of n, `fill` past its end.  Even: n is a
+// multiple of kVec, and a vector is in the row or past it (otherwise the
+// addresses of a last vector's single elements cost a kernel that loops over
+// rows half as many registers again).
+template <typename T, bool Even = false>
 __device__ __forceinline__ vec_t<T> load_part(const T* row, int i, int n, T fill) {
-  if (i + kVec<T> <= n) return load_vec(row + i);
+  if (Even ? i < n : i + kVec<T> <= n) return load_vec(row + i);
   vec_t<T> v;
 #pragma unroll
-  for (int j = 0; j < kVec<T>; ++j) v[j] = i + j < n ? row[i + j] : fill;
+  for (int j = 0; j < kVec<T>; ++j) v[j] = !Even && i + j < n ? row[i + j] : fill;
   return v;
 }
-template <typename T>
+template <typename T, bool Even = false>
 __device__ __forceinline__ void store_part(T* row, int i, int n, vec_t<T> v) {
-  if (i + kVec<T> <= n) {
+  if (Even ? i < n : i + kVec<T> <= n) {
     store_vec(row + i, v);
     return;
   }
+  if (Even) return;
 #pragma unroll
   for (int j = 0; j < kVec<T>; ++j)
     if (i + j < n) row[i + j] = v[j];
