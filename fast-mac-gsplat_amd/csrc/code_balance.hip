@@ -383,7 +383,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
           const int j = r * V + v;
           o[v] = static_cast<T>(p[j] * __builtin_fmaf(a[j], f, less));
         }
-        store_part<T, Even>(out, G::column(r), P.K, o);
+        store_part<T, Even, true>(out, G::column(r), P.K, o);
       }
     }
   }

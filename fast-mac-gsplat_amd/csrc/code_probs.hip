@@ -158,9 +158,9 @@ struct Held {
   __device__ __forceinline__ Part part(const Exponent& e) {
     Part p{e.m, 0.0f, 0.0f};
     auto sum = [&](auto exponent) {
-      forget();
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        gs::forget<T>(x[r]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float t = exponent(to_float(x[r][v]));
@@ -168,6 +168,7 @@ struct Held {
           p.s += y;
           p.st = __builtin_fmaf(y, bounded(t), p.st);
         }
+      }
     };
     if (e.plain)
       sum([&](float x) { return e.fast(x); });
@@ -187,15 +188,23 @@ struct Held {
       }
     return k;
   }
-  // The lowest column whose logit equals m.
-  __device__ __forceinline__ uint32_t first_equal(float m) const {
+  // The team's lowest column whose logit equals m; most[r]: max_of(r).  Vectors
+  // are in the order of the columns: those after the first that holds m are
+  // not looked at (by a wavefront as a whole).
+  __device__ __forceinline__ uint32_t first_equal(float m, const float (&most)[R]) const {
     uint32_t i = ~0u;
 #pragma unroll
-    for (int r = R - 1; r >= 0; --r)
+    for (int r = 0; r < R; ++r) {
+      const bool hit = most[r] == m && i == ~0u;
+      if (__ballot(hit) == 0) continue;
+      uint32_t j = ~0u;
 #pragma unroll
       for (int v = V - 1; v >= 0; --v)
-        if (to_float(x[r][v]) == m) i = column(r, v);
-    return i;
+        if (to_float(x[r][v]) == m) j = column(r, v);
+      if (hit) i = j;
+      if (TL == 64) break;
+    }
+    return team_min<TL>(i);
   }
 };
 
@@ -245,7 +254,7 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
   const bool plain = p.s == p.s;  // (no NaN)
   if (plain) {
     // the best: the first column that has the maximum
-    const uint32_t i = team_min<TL>(x.first_equal(p.m));
+    const uint32_t i = x.first_equal(p.m, most);
     if (lane == 0) put(0, i, p.m);
     from = 1;
   }
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
     }
   }
   uint64_t last = ~0ull;
-  if (plain) last = rank_key(p.m, team_min<TL>(x.first_equal(p.m)));
+  if (plain) last = rank_key(p.m, x.first_equal(p.m, most));
   for (int j = from; j < top; ++j) {
     last = team_best<TL>(x.best_below(last));
     const uint32_t i = ~(uint32_t)last;
@@ -346,7 +355,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) voi
   if ((lane & (W - 1)) == 0) groups[threadIdx.x / W] = group;
   if (lane == 0) parts[w] = p;
   if (threadIdx.x == 0) total = 0;
-  x.forget();
   __syncthreads();
   // (joined by teams of W lanes, each lane a wavefront's part)
   p = parts[lane & (W - 1)];
@@ -379,6 +387,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) voi
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (most[r] < bound) continue;
+      gs::forget<T>(x.x[r]);
 #pragma unroll
       for (int v = 0; v < kVec<T>; ++v) {
         const float f = to_float(x.x[r][v]);
@@ -533,12 +542,18 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   else
     products([&](float x) { return e.slow(x); });
   auto add = [&](int col, float w) {
-    if ((unsigned)(col - first) >= (unsigned)kSpan) return;
+    const unsigned rel = (unsigned)(col - first);
+    if (rel >= (unsigned)kSpan) return;
+    // (of a wavefront's row the place is the same for all lanes: one vector's
+    // elements are looked at)
+    const float mine = lane == (int)(rel / V & (TL - 1)) ? w : 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      const unsigned in = rel - r * (V * TL);
+      if (R > 1 && in >= (unsigned)(V * TL)) continue;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        g[r * V + v] += col - first == (r * TL + lane) * V + v ? w : 0.0f;
+      for (int v = 0; v < V; ++v) g[r * V + v] += in % V == (unsigned)v ? mine : 0.0f;
+    }
   };
   if (code >= 0) add(code, gl);
   for (int j = 0; j < top; ++j) add(tc[j], gt[j] * P.inv_t);
@@ -547,7 +562,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     vec_t<T> o;
 #pragma unroll
     for (int v = 0; v < V; ++v) o[v] = static_cast<T>(g[r * V + v]);
-    store_part<T, Even>(out, first + (r * TL + lane) * V, P.K, o);
+    store_part<T, Even, true>(out, first + (r * TL + lane) * V, P.K, o);
   }
 }
 
@@ -578,6 +593,14 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
                   dim3(kThreads), 0, stream, P, x, out);                         \
     return check_launch("probs_rows_kernel");                                    \
   }
+  // With no more than the best code wanted, teams as narrow as 32 elements a
+  // lane of 16 bits allow: what a row costs beside its elements is then shared
+  // by more of them.  More codes are found by a whole wavefront's ballots.
+  if constexpr (sizeof(T) == 2)
+    if (P.top <= 1) {
+      GS_ROWS(2, 1) GS_ROWS(4, 2) GS_ROWS(8, 2) GS_ROWS(16, 2) GS_ROWS(32, 2)
+      GS_ROWS(32, 4) GS_ROWS(64, 4)
+    }
   GS_ROWS(2, 1) GS_ROWS(4, 1) GS_ROWS(8, 1) GS_ROWS(16, 1) GS_ROWS(32, 1)
   GS_ROWS(64, 1) GS_ROWS(64, 2) GS_ROWS(64, 4)
 #undef GS_ROWS

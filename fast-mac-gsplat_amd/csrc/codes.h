@@ -120,10 +120,11 @@ __device__ __forceinline__ vec_t<T> load_part(const T* row, int i, int n, T fill
   for (int j = 0; j < kVec<T>; ++j) v[j] = !Even && i + j < n ? row[i + j] : fill;
   return v;
 }
-template <typename T, bool Even = false>
+template <typename T, bool Even = false, bool Stream = false>
 __device__ __forceinline__ void store_part(T* row, int i, int n, vec_t<T> v) {
   if (Even ? i < n : i + kVec<T> <= n) {
-    store_vec(row + i, v);
+    if (Stream) store_vec_stream(row + i, v);
+    else store_vec(row + i, v);
     return;
   }
   if (Even) return;
