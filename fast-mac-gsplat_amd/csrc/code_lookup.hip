@@ -135,10 +135,11 @@ struct Columns {
   static constexpr int kTeams = kThreads / TL;
   static __device__ __forceinline__ int lane() { return threadIdx.x & (TL - 1); }
   static __device__ __forceinline__ int column(int c0, int r) { return c0 + (r * TL + lane()) * V; }
+  template <bool Stream = false>
   static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int c0, int D) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T>(row, column(c0, r), D, static_cast<T>(0.0f));
+      x[r] = load_part<T, false, Stream>(row, column(c0, r), D, static_cast<T>(0.0f));
   }
   static __device__ __forceinline__ void store(T* row, int c0, int D, const float (&a)[R * V],
                                                float f) {
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       s[u] = scales ? scales[n[u]] : 1.0f;
-      C::load(g[u], grad + (int64_t)n[u] * P.D, c0, P.D);
+      C::template load<true>(g[u], grad + (int64_t)n[u] * P.D, c0, P.D);
     }
     look(j0 + kRows);
     key[kRows] = key_next[0];

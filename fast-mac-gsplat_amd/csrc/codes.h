@@ -95,6 +95,12 @@ __device__ __forceinline__ void store_vec_stream(T* p, vec_t<T> v) {
   __builtin_nontemporal_store(__builtin_bit_cast(words, v), reinterpret_cast<words*>(p));
 }
 
+template <typename T>
+__device__ __forceinline__ vec_t<T> load_vec_stream(const T* p) {
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+  return __builtin_bit_cast(vec_t<T>, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+}
+
 // The same 16 bytes, of which the compiler no longer knows that it has them as
 // floats already: two passes over a row in registers convert its elements twice
 // rather than keep twice the registers.
@@ -112,9 +118,9 @@ __device__ __forceinline__ void forget(vec_t<T>& v) {
 // multiple of kVec, and a vector is in the row or past it (otherwise the
 // addresses of a last vector's single elements cost a kernel that loops over
 // rows half as many registers again).
-template <typename T, bool Even = false>
+template <typename T, bool Even = false, bool Stream = false>
 __device__ __forceinline__ vec_t<T> load_part(const T* row, int i, int n, T fill) {
-  if (Even ? i < n : i + kVec<T> <= n) return load_vec(row + i);
+  if (Even ? i < n : i + kVec<T> <= n) return Stream ? load_vec_stream(row + i) : load_vec(row + i);
   vec_t<T> v;
 #pragma unroll
   for (int j = 0; j < kVec<T>; ++j) v[j] = !Even && i + j < n ? row[i + j] : fill;
