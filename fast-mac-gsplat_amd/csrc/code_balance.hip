@@ -40,10 +40,11 @@ struct Team {
   static __device__ __forceinline__ int member() { return threadIdx.x & (TL * W - 1); }
   static __device__ __forceinline__ int wave() { return W > 1 ? (threadIdx.x >> 6) & (W - 1) : 0; }
   static __device__ __forceinline__ int column(int r) { return (r * TL * W + member()) * V; }
+  template <bool Stream = false>
   static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int K) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T, Even>(row, column(r), K, static_cast<T>(-INFINITY));
+      x[r] = load_part<T, Even, Stream>(row, column(r), K, static_cast<T>(-INFINITY));
   }
 };
 
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
   auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
   int64_t i = G::team();
   vec_t<T> x[R];
-  G::load(x, logits + row_of(i) * P.stride, P.K);
+  G::template load<true>(x, logits + row_of(i) * P.stride, P.K);
   float2 st = stats[row_of(i)];
   for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
     const int64_t r0 = row_of(i);
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
       products([&](float y) { return ex.slow(y); });
     if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
       const int64_t rn = row_of(i + G::kTeams);
-      G::load(x, logits + rn * P.stride, P.K);
+      G::template load<true>(x, logits + rn * P.stride, P.K);
       st = stats[rn];
     }
     dot = team_sum<TL>(dot) * down;

@@ -511,7 +511,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   vec_t<T> x[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    x[r] = load_part<T, Even>(row, first + (r * TL + lane) * V, P.K, static_cast<T>(-INFINITY));
+    x[r] = load_part<T, Even, true>(row, first + (r * TL + lane) * V, P.K, static_cast<T>(-INFINITY));
   const float2 st = stats[n];
   const bool some = st.y != INFINITY;  // (else p = 0 everywhere)
   const float ge = g_entropy && some ? g_entropy[n] : 0.0f;
