@@ -58,6 +58,7 @@ struct Partials {
   int4* totals;  // rows that take part, choices, bad codes
   float* loss;   // [batch][column groups]
   uint32_t* tickets;  // [batch], zeroed by the row pass
+  bool stream;  // past_caches
 };
 
 // The choices of a row (kept by the lanes of a wavefront): counts them.
@@ -101,12 +102,18 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
   for (int j = 0; j < R * V; ++j) acc[j] = 0.0f;
   int took = 0, given = 0, bad = 0;
   vec_t<T> x[R];
+  auto load = [&](const T* row) {
+    if (out.stream)
+      G::template load<true>(x, row, P.K);
+    else
+      G::load(x, row, P.K);
+  };
   const int64_t base_row = b * P.rows + first;
   auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
   int64_t i = G::team();
   int code = kNoCode;
   if (count > 0) {
-    G::load(x, logits + row_of(i) * P.stride, P.K);
+    load(logits + row_of(i) * P.stride);
     if (lane < S) code = P.codes.at(row_of(i) * S + lane, P.K);
   }
   // (every team makes the same number of turns; those past the rows count nothing)
@@ -152,7 +159,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
       powers([&](float y) { return ex.slow(y); });
     if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
       const int64_t rn = row_of(i + G::kTeams);
-      G::load(x, logits + rn * P.stride, P.K);
+      load(logits + rn * P.stride);
       code = lane < S ? P.codes.at(rn * S + lane, P.K) : kNoCode;
     }
     s = team_sum<TL>(s);
@@ -595,7 +602,8 @@ int forward_of(const BalanceParams& P, const void* logits, float* loss,
              reinterpret_cast<int32_t*>(ws + L.counts),
              reinterpret_cast<int4*>(ws + L.totals),
              reinterpret_cast<float*>(ws + L.loss),
-             reinterpret_cast<uint32_t*>(ws + L.tickets)};
+             reinterpret_cast<uint32_t*>(ws + L.tickets),
+             past_caches(P.rows * P.batch, P.K, P.dtype)};
   int rc;
   if (!is_long) {
     rc = P.K % kVec<T> == 0 ? rows_of<T, true>(P, x, stats, w, stream)

@@ -136,11 +136,12 @@ struct Held {
   static constexpr int V = kVec<T>;
   vec_t<T> x[R];
   int lane;
+  template <bool Stream = false>
   __device__ __forceinline__ void load(const T* row, int lane_, int n) {
     lane = lane_;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T, Even>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
+      x[r] = load_part<T, Even, Stream>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
   }
   __device__ __forceinline__ int column(int r, int v) const { return (r * TL + lane) * V + v; }
   __device__ __forceinline__ void forget() {
@@ -312,6 +313,7 @@ struct Split {
   int length;   // elements of a part (the last may be shorter)
   Part* stats;  // [rows][parts]
   uint64_t* best;  // [rows][parts][top]
+  bool stream;     // past_caches
 };
 
 constexpr int kFound = 256;  // logits collected for the best ones
@@ -332,7 +334,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(5))) voi
   const T* row = logits + n * P.stride;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   Held<T, kThreads, R, Even> x;
-  x.load(row + first, threadIdx.x, len);
+  if (split.stream)
+    x.template load<true>(row + first, threadIdx.x, len);
+  else
+    x.load(row + first, threadIdx.x, len);
   const int code = P.codes.p && split.parts == 1 ? P.codes.at(n, P.K) : kNoCode;
   float most[R];  // of each vector
 #pragma unroll
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
 constexpr int kPartLong = 16384;
 
 Split split_of(const ProbsParams& P) {
-  Split s{1, P.K, nullptr, nullptr};
+  Split s{1, P.K, nullptr, nullptr, past_caches(P.rows, P.K, P.dtype)};
   if (P.K <= kPartLong) return s;
   // Few rows: shorter parts, until there is one for each of 512 workgroups.
   int64_t length = kPartLong;
