@@ -582,3 +582,54 @@ def test_inputs_that_are_not_plain(gpu):
     assert all(torch.equal(torch.Tensor(u) if u.is_floating_point() else u, v) for u, v in zip(a, b))
     a, b = gs.code_balance(x.as_subclass(Sub), codes), gs.code_balance(x, codes)
     assert torch.equal(a.counts, b.counts) and torch.equal(torch.Tensor(a.mean_probs), b.mean_probs)
+
+
+def test_example_fits_a_scene(gpu):
+    """examples/train_coded_scene.py: the three operators around the rasterizer, a scene that gets better."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_coded_scene.py")
+    spec = importlib.util.spec_from_file_location("train_coded_scene", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    history, stored = example.train(steps=60, splats=1500, codes=32, size=128)
+    assert bool(torch.isfinite(history["loss"]).all())
+    assert float(history["mse"][-5:].mean()) < 0.3 * float(history["mse"][0])
+    assert stored["codebook"].shape == (32, 3) and stored["codes"].shape == (1500,)
+    assert int(history["used"][-1]) >= 4
+
+
+def test_graph_capture(gpu):
+    """All three, forward and backward, in a captured graph, replayed with new values between eager work."""
+    x = torch.randn(3000, 200, device=gpu, requires_grad=True)
+    book = torch.randn(200, 16, device=gpu, requires_grad=True)
+    codes = torch.randint(-1, 200, (3000,), device=gpu)
+    many = torch.randint(-1, 200, (20000,), device=gpu)
+
+    def step():
+        o, b = gs.code_log_probs(x, codes, top=3), gs.code_balance(x, codes)
+        out, more = gs.lookup_codes(codes, book), gs.lookup_codes(many, book)
+        outs = [o.log_probs, o.entropy, o.top_log_probs, b.loss, b.mean_probs, out, more]
+        gx, gb = torch.autograd.grad(outs, [x, book], [torch.ones_like(t) for t in outs])
+        return [*outs, o.top_codes, b.counts, gx, gb]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(3000, 200, generator=_gen(k)))
+            codes.copy_(torch.randint(-1, 200, (3000,), generator=_gen(k + 9)))
+            many.copy_(torch.randint(-1, 200, (20000,), generator=_gen(k + 19)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.detach().clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b.detach())
