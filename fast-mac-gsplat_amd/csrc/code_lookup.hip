@@ -34,8 +34,8 @@ __device__ __forceinline__ float nan_for(int c) {
 
 // Each thread writes kUnroll vectors of 16 bytes of the output, taken as one
 // array; block b starts at element b * kThreads * V * kUnroll.  div: the
-// quotient of a 32-bit offset by D (below).
-constexpr int kUnroll = 4;
+// quotient of a 32-bit offset by D (below).  Four vectors keep four chains of
+// loads (code, row) on their way; one where that leaves CUs without work.
 
 // n / d for n < 2^31 by one 32 x 32 multiplication: floor(n m / 2^(32 + s))
 // with m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1 (exact for n < 2^31: the
@@ -52,7 +52,7 @@ struct Divide {
   }
 };
 
-template <typename T, bool Rows>
+template <typename T, bool Rows, int kUnroll>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     LookupParams P, Divide div, const T* __restrict__ codebook,
     const float* __restrict__ scales, T* __restrict__ out) {
@@ -616,18 +616,20 @@ Layout layout(const LookupParams& P) {
 template <typename T>
 int forward_of(const LookupParams& P, const void* codebook, const float* scales,
                void* out, hipStream_t stream) {
-  const int64_t total = P.rows * P.D;
-  const int64_t per = kThreads * kVec<T> * kUnroll;
-  const dim3 grid((unsigned)((total + per - 1) / per));
+  const int64_t vecs = (P.rows * P.D + kVec<T> - 1) / kVec<T>;
   const T* book = static_cast<const T*>(codebook);
   T* o = static_cast<T*>(out);
   const Divide div((uint32_t)P.D);
-  if (P.D % kVec<T> == 0)
-    launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, true>), grid,
-                  dim3(kThreads), 0, stream, P, div, book, scales, o);
-  else
-    launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, false>), grid,
-                  dim3(kThreads), 0, stream, P, div, book, scales, o);
+#define GS_LOOKUP(ROWS, U)                                                      \
+  launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, ROWS, U>),           \
+                dim3((unsigned)((vecs + kThreads * U - 1) / (kThreads * U))),   \
+                dim3(kThreads), 0, stream, P, div, book, scales, o)
+  const bool rows = P.D % kVec<T> == 0, many = vecs >= (int64_t)kThreads * 4 * 1024;
+  if (rows && many) GS_LOOKUP(true, 4);
+  else if (rows) GS_LOOKUP(true, 1);
+  else if (many) GS_LOOKUP(false, 4);
+  else GS_LOOKUP(false, 1);
+#undef GS_LOOKUP
   return check_launch("lookup_fwd_kernel");
 }
 
