@@ -128,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 // ---- backward
 
 // A team of TL lanes holds R vectors per lane of a row's columns from c0 on.
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 struct Columns {
   static constexpr int V = kVec<T>;
   static constexpr int kWidth = TL * V * R;
@@ -139,7 +139,7 @@ struct Columns {
   static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int c0, int D) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      x[r] = load_part<T, false, Stream>(row, column(c0, r), D, static_cast<T>(0.0f));
+      x[r] = load_part<T, Even, Stream>(row, column(c0, r), D, static_cast<T>(0.0f));
   }
   static __device__ __forceinline__ void store(T* row, int c0, int D, const float (&a)[R * V],
                                                float f) {
@@ -148,7 +148,7 @@ struct Columns {
       vec_t<T> o;
 #pragma unroll
       for (int v = 0; v < V; ++v) o[v] = static_cast<T>(a[r * V + v] * f);
-      if (column(c0, r) < D) store_part<T>(row, column(c0, r), D, o);
+      if (column(c0, r) < D) store_part<T, Even>(row, column(c0, r), D, o);
     }
   }
   static __device__ __forceinline__ void load_sums(float (&a)[R * V], const float* row, int c0,
@@ -179,12 +179,12 @@ struct Columns {
 constexpr int kList = 256;
 constexpr int kCodes = 4;  // per wavefront
 
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
     LookupParams P, const T* __restrict__ grad, const T* __restrict__ codebook,
     const float* __restrict__ scales, T* __restrict__ g_codebook,
     float* __restrict__ g_scales) {
-  using C = Columns<T, TL, R>;
+  using C = Columns<T, TL, R, Even>;
   constexpr int V = C::V, kT = 64 / TL;
   __shared__ uint16_t lists[kThreads / 64][kCodes][kList];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -300,12 +300,13 @@ struct Sorted {
   float* out;
 };
 
-template <typename T, int TL, int R>
-__global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
+template <typename T, int TL, int R, bool Even>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && R == 1 ? (Even ? 6 : 5) : 4))) void
+lookup_runs_kernel(
     LookupParams P, Sorted S, const T* __restrict__ grad,
     const T* __restrict__ codebook, const float* __restrict__ scales,
     T* __restrict__ g_codebook, float* __restrict__ g_scales) {
-  using C = Columns<T, TL, R>;
+  using C = Columns<T, TL, R, Even>;
   constexpr int V = C::V, kTeams = C::kTeams, kRows = R > 1 ? 2 : 4;
   __shared__ float open[kTeams][C::kWidth + 1];  // (+ 1: teams of one lane)
   __shared__ uint8_t ended[kTeams];
@@ -461,10 +462,10 @@ __global__ __launch_bounds__(kThreads) void lookup_runs_kernel(
 // on after its positions, that run's partial rows are added up (teams take
 // every kTeams-th row, then the teams in order).  A sort that gave up makes
 // the gradient NaN.
-template <typename T, int TL, int R>
+template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void lookup_join_kernel(
     LookupParams P, Sorted S, T* __restrict__ g_codebook) {
-  using C = Columns<T, TL, R>;
+  using C = Columns<T, TL, R, Even>;
   constexpr int V = C::V, kTeams = C::kTeams;
   __shared__ float sums[kTeams][C::kWidth + 1];
   __shared__ int ends[kThreads / 64];
@@ -633,7 +634,7 @@ int forward_of(const LookupParams& P, const void* codebook, const float* scales,
   return check_launch("lookup_fwd_kernel");
 }
 
-template <typename T>
+template <typename T, bool Even>
 int backward_of(const LookupParams& P, const void* grad_out, const void* codebook,
                 const float* scales, void* g_codebook, float* g_scales,
                 void* workspace, hipStream_t stream) {
@@ -657,7 +658,7 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
     const dim3 grid((unsigned)((P.K + per - 1) / per), tiles);
 #define GS_SCAN(TL, R)                                                          \
   {                                                                             \
-    launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R>), grid,   \
+    launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R, Even>), grid,   \
                   dim3(kThreads), 0, stream, P, grad, book, scales, g_book,     \
                   g_scales);                                                    \
     return check_launch("lookup_scan_kernel");                                  \
@@ -689,12 +690,12 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
   const dim3 grid((unsigned)L.blocks, tiles);
 #define GS_RUNS(TL, R)                                                          \
   {                                                                             \
-    launch_traced("lookup_runs_kernel", (lookup_runs_kernel<T, TL, R>), grid,   \
+    launch_traced("lookup_runs_kernel", (lookup_runs_kernel<T, TL, R, Even>), grid,   \
                   dim3(kThreads), 0, stream, P, S, grad, book, scales, g_book,  \
                   g_scales);                                                    \
     rc = check_launch("lookup_runs_kernel");                                    \
     if (rc) return rc;                                                          \
-    launch_traced("lookup_join_kernel", (lookup_join_kernel<T, TL, R>), grid,   \
+    launch_traced("lookup_join_kernel", (lookup_join_kernel<T, TL, R, Even>), grid,   \
                   dim3(kThreads), 0, stream, P, S, g_book);                     \
     return check_launch("lookup_join_kernel");                                  \
   }
@@ -723,14 +724,11 @@ int launch_lookup_backward(const LookupParams& P, const void* grad_out,
                            const void* codebook, const float* scales,
                            void* g_codebook, float* g_scales, void* workspace,
                            hipStream_t stream) {
-  if (P.dtype == GSPLAT_F32)
-    return backward_of<float>(P, grad_out, codebook, scales, g_codebook, g_scales,
-                              workspace, stream);
-  if (P.dtype == GSPLAT_BF16)
-    return backward_of<__bf16>(P, grad_out, codebook, scales, g_codebook, g_scales,
-                               workspace, stream);
-  return backward_of<_Float16>(P, grad_out, codebook, scales, g_codebook, g_scales,
-                               workspace, stream);
+  const bool even = P.D % vec_of(P) == 0;
+  auto f = P.dtype == GSPLAT_F32    ? (even ? backward_of<float, true> : backward_of<float, false>)
+           : P.dtype == GSPLAT_BF16 ? (even ? backward_of<__bf16, true> : backward_of<__bf16, false>)
+                                    : (even ? backward_of<_Float16, true> : backward_of<_Float16, false>);
+  return f(P, grad_out, codebook, scales, g_codebook, g_scales, workspace, stream);
 }
 
 }  // namespace gs
