@@ -358,7 +358,9 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int j = r * V + v;
-          const float t = exponent(to_float(x[r][v]));
+          // (a NaN in a row that takes no part is no part of it; one that does
+          // has a NaN in its constants)
+          const float t = fmaxf(exponent(to_float(x[r][v])), -1000.0f);
           p[j] = sizeof(T) == 2 ? exp2_fast(t) : exp2_full(t);
           dot = __builtin_fmaf(p[j], a[j], dot);
         }
@@ -404,7 +406,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 
 __device__ __forceinline__ float prob(float x, float2 st) {
-  return exp2_full((x - st.x) * kLog2e - st.y);
+  return st.y == INFINITY ? 0.0f : exp2_full((x - st.x) * kLog2e - st.y);
 }
 
 // A workgroup per row.  The only counts and totals of an image: zero on entry.

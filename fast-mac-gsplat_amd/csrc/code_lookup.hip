@@ -7,8 +7,8 @@
 // The gradient of the codebook is a sum by code, in an order that does not
 // depend on the run (no atomics: the same inputs give the same bits).
 //
-// Few splats: a wavefront takes four codes, reads every splat's code, lists
-// those that name one of the four and adds up their rows (one launch).
+// Few splats: a workgroup takes one to four codes, reads every splat's code,
+// lists those that name one of its own and adds up their rows (one launch).
 //
 // More splats: they are sorted by code (stable), so that a code's splats are
 // one run of the sorted positions.  A team of lanes adds up `piece` positions,
@@ -173,97 +173,132 @@ struct Columns {
   }
 };
 
-// Few splats.  Wavefront w takes codes 4w .. 4w + 3.  The splats are read
-// kList at a time; per code the rows found are shared out over the wavefront's
-// teams, whose sums are added in the order of the teams.
-constexpr int kList = 256;
-constexpr int kCodes = 4;  // per wavefront
+// Few splats.  A workgroup takes Q codes.  Its wavefronts each read a quarter of
+// kRowsAtOnce splats' codes and list the splats of the workgroup's codes, in
+// order; the rows listed for a code are shared out over the workgroup's teams,
+// four on their way at a time, and the teams' sums are added in their order.
+constexpr int kRowsAtOnce = 2048;
+constexpr int kQuarter = kRowsAtOnce / 4;
 
-template <typename T, int TL, int R, bool Even>
+template <typename T, int TL, int R, int Q, bool Even>
 __global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
     LookupParams P, const T* __restrict__ grad, const T* __restrict__ codebook,
     const float* __restrict__ scales, T* __restrict__ g_codebook,
     float* __restrict__ g_scales) {
   using C = Columns<T, TL, R, Even>;
-  constexpr int V = C::V, kT = 64 / TL;
-  __shared__ uint16_t lists[kThreads / 64][kCodes][kList];
+  constexpr int V = C::V, kTeams = C::kTeams, kAhead = 4;
+  __shared__ uint16_t lists[Q][4][kQuarter];
+  __shared__ int counts[Q][4];
+  __shared__ float sums[4][C::kWidth];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int team = lane / TL;
-  const int first = ((int)blockIdx.x * (kThreads / 64) + w) * kCodes;
-  if (first >= P.K) return;
+  const int team = threadIdx.x / TL;
+  const int first = (int)blockIdx.x * Q;
   const int c0 = blockIdx.y * C::kWidth;
   const bool dots = g_scales != nullptr;
-  float acc[kCodes][R * V];
+  float acc[Q][R * V];
 #pragma unroll
-  for (int q = 0; q < kCodes; ++q)
+  for (int q = 0; q < Q; ++q)
 #pragma unroll
     for (int j = 0; j < R * V; ++j) acc[q][j] = 0.0f;
-  for (int64_t base = 0; base < P.rows; base += kList) {
-    int found[kCodes] = {0, 0, 0, 0};
-    int mine[kList / 64];
+  for (int64_t base = 0; base < P.rows; base += kRowsAtOnce) {
+    int mine[kQuarter / 64];
 #pragma unroll
-    for (int u = 0; u < kList / 64; ++u) {
-      const int64_t n = base + u * 64 + lane;
+    for (int u = 0; u < kQuarter / 64; ++u) {
+      const int64_t n = base + w * kQuarter + u * 64 + lane;
       mine[u] = n < P.rows ? P.codes.at(n, P.K) : kNoCode;
       if (dots && first == 0 && n < P.rows && mine[u] < 0) g_scales[n] = nan_for(mine[u]);
     }
+    int found[Q];
 #pragma unroll
-    for (int u = 0; u < kList / 64; ++u) {
+    for (int q = 0; q < Q; ++q) found[q] = 0;
+#pragma unroll
+    for (int u = 0; u < kQuarter / 64; ++u) {
       const unsigned rel = (unsigned)(mine[u] - first);
-      if (__ballot(rel < (unsigned)kCodes) == 0) continue;
+      if (__ballot(rel < (unsigned)Q) == 0) continue;
 #pragma unroll
-      for (int q = 0; q < kCodes; ++q) {
+      for (int q = 0; q < Q; ++q) {
         const uint64_t hit = __ballot(rel == (unsigned)q);
         if (rel == (unsigned)q)
-          lists[w][q][found[q] + __builtin_amdgcn_mbcnt_hi(
+          lists[q][w][found[q] + __builtin_amdgcn_mbcnt_hi(
                                      (uint32_t)(hit >> 32),
                                      __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0))] =
-              (uint16_t)(u * 64 + lane);
+              (uint16_t)(w * kQuarter + u * 64 + lane);
         found[q] += __popcll(hit);
       }
     }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (lane == 0)
 #pragma unroll
-    for (int q = 0; q < kCodes; ++q) {
-      if (found[q] == 0) continue;
+      for (int q = 0; q < Q; ++q) counts[q][w] = found[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      // (the lists of the four wavefronts, one after another)
+      const int e0 = counts[q][0], e1 = e0 + counts[q][1], e2 = e1 + counts[q][2],
+                total = e2 + counts[q][3];
+      if (total == 0) continue;
       vec_t<T> row[R];
       if (dots) C::load(row, codebook + (int64_t)(first + q) * P.stride, c0, P.D);
       // (every team makes the same number of turns: the sums of a row's
       // products run over whole teams)
-      for (int i0 = 0; i0 < found[q]; i0 += kT) {
-        const int i = i0 + team;
-        const bool here = i < found[q];
-        const int64_t n = base + lists[w][q][here ? i : 0];
-        vec_t<T> g[R];
-        C::load(g, grad + n * P.D, c0, P.D);
-        const float s = !here ? 0.0f : scales ? scales[n] : 1.0f;
-        float dot = 0.0f;
+      for (int i0 = 0; i0 < total; i0 += kAhead * kTeams) {
+        int64_t n[kAhead];
+        float s[kAhead];
+        vec_t<T> g[kAhead][R];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = min(i0 + u * kTeams + team, total - 1);
+          const int from = (i >= e0) + (i >= e1) + (i >= e2);
+          n[u] = base + lists[q][from][i - (from == 0 ? 0 : from == 1 ? e0 : from == 2 ? e1 : e2)];
+          s[u] = scales ? scales[n[u]] : 1.0f;
+          C::load(g[u], grad + n[u] * P.D, c0, P.D);
+        }
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float x = to_float(g[r][v]);
-            if (here) acc[q][r * V + v] = __builtin_fmaf(x, s, acc[q][r * V + v]);
-            if (dots) dot = __builtin_fmaf(x, to_float(row[r][v]), dot);
+        for (int u = 0; u < kAhead; ++u) {
+          if (i0 + u * kTeams >= total) break;
+          const bool here = i0 + u * kTeams + team < total;
+          float dot = 0.0f;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              const float x = to_float(g[u][r][v]);
+              if (here) acc[q][r * V + v] = __builtin_fmaf(x, s[u], acc[q][r * V + v]);
+              if (dots) dot = __builtin_fmaf(x, to_float(row[r][v]), dot);
+            }
+          if (dots) {
+            dot = team_sum<TL>(dot);
+            if (here && C::lane() == 0) g_scales[n[u]] = dot * P.factor;
           }
-        if (dots) {
-          dot = team_sum<TL>(dot);
-          if (here && C::lane() == 0) g_scales[n] = dot * P.factor;
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    __syncthreads();
   }
   if (g_codebook == nullptr) return;
 #pragma unroll
-  for (int q = 0; q < kCodes; ++q) {
+  for (int q = 0; q < Q; ++q) {
     if (first + q >= P.K) return;
 #pragma unroll
     for (int j = 0; j < R * V; ++j)
 #pragma unroll
       for (int d = TL; d < 64; d <<= 1) acc[q][j] += __shfl_xor(acc[q][j], d, 64);
-    if (team == 0) C::store(g_codebook + (int64_t)(first + q) * P.D, c0, P.D, acc[q], P.factor);
+    if (lane < TL)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v) sums[w][(r * TL + lane) * V + v] = acc[q][r * V + v];
+    __syncthreads();
+    if (threadIdx.x < TL) {
+#pragma unroll
+      for (int t = 1; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            acc[q][r * V + v] += sums[t][(r * TL + lane) * V + v];
+      C::store(g_codebook + (int64_t)(first + q) * P.D, c0, P.D, acc[q], P.factor);
+    }
+    __syncthreads();
   }
 }
 
@@ -568,7 +603,11 @@ int lanes_of(const LookupParams& P) {
   return tl;
 }
 
-// The one-launch way reads all codes once for each four of the codebook.
+// The one-launch way reads all codes once for each code (or four) of the
+// codebook.  Kernels of both ways, rows of 64 floats: 8192 splats and 256 codes
+// 13 us against 28 sorted, 8192 x 4096 25 against 29, 4096 x 16384 27 against
+// 28, 8192 x 16384 44 against 29, 16384 x 16 43 against 24; the sort's five to
+// six launches cost the host 20 us more.
 bool few(const LookupParams& P) {
   return P.rows <= 8192 && P.rows * P.K <= (int64_t(1) << 26);
 }
@@ -654,17 +693,20 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
   }
   if (!g_book) return GSPLAT_OK;
   if (few(P)) {
-    const int per = kThreads / 64 * kCodes;
-    const dim3 grid((unsigned)((P.K + per - 1) / per), tiles);
+    // (four codes a workgroup where that leaves 1024 of them)
+#define GS_SCAN_OF(TL, R, Q)                                                      \
+    launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R, Q, Even>),  \
+                  dim3((unsigned)((P.K + Q - 1) / Q), tiles), dim3(kThreads), 0,  \
+                  stream, P, grad, book, scales, g_book, g_scales)
 #define GS_SCAN(TL, R)                                                          \
   {                                                                             \
-    launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R, Even>), grid,   \
-                  dim3(kThreads), 0, stream, P, grad, book, scales, g_book,     \
-                  g_scales);                                                    \
+    if (P.K >= 4096) GS_SCAN_OF(TL, R, 4);                                      \
+    else GS_SCAN_OF(TL, R, 1);                                                  \
     return check_launch("lookup_scan_kernel");                                  \
   }
     GS_WIDTHS(GS_SCAN)
 #undef GS_SCAN
+#undef GS_SCAN_OF
   }
   const Layout L = layout(P);
   char* w = static_cast<char*>(workspace);

@@ -63,7 +63,7 @@ struct Exponent {
     const float back = k - hi;
     const float rest = (hi - (k - back)) + (l - back);
     plain = __builtin_fabsf(k) < 1e30f;
-    shift = plain ? -(lo + rest) : 0.0f;
+    shift = plain ? -(lo + rest) : l == l ? 0.0f : l;  // (a NaN row's is NaN)
   }
   __device__ __forceinline__ float fast(float x) const { return __builtin_fmaf(x, c, -k); }
   __device__ __forceinline__ float slow(float x) const { return (x - m) * c - l; }

@@ -419,6 +419,43 @@ def test_balance_masks_nan_and_bad_codes(gpu):
         R.check(getattr(o, k), want[k], k)
 
 
+@pytest.mark.parametrize("K", [30, 700, 3001, 20000])
+def test_balance_gradient_of_rows_without_part(gpu, K):
+    """NaN and infinities in rows without a code reach nothing; a NaN in a row with one makes its row NaN."""
+    for dtype in (F32, BF16):
+        x = _logits((9,), K, dtype, seed=K)
+        codes = torch.randint(0, K, (9,), generator=_gen(K))
+        codes[2] = codes[3] = codes[4] = -1
+        x[2, 1] = math.nan
+        x[3, 2] = math.inf
+        x[4] = -math.inf
+        x[5] = -math.inf
+        _check_balance(gpu, x, codes, what=f"no part K={K} {dtype}")
+        g_loss = torch.ones(())
+        x[6, 3] = math.nan
+        want = R.balance(x, codes, g_loss, torch.zeros(K))["g_logits"]
+        xg = x.to(gpu).requires_grad_(True)
+        o = gs.code_balance(xg, codes.to(gpu))
+        got, = torch.autograd.grad(o.loss, xg, torch.ones((), device=gpu))
+        R.check(got, want, f"NaN row K={K} {dtype}")
+
+
+@pytest.mark.parametrize("N", [700, 9000])
+def test_lookup_gradients_of_splats_without_code(gpu, N):
+    """NaN and infinities in the gradient of splats without a code reach no row of the codebook."""
+    codes, book, s, grad = _lookup_inputs((N,), 50, 12, F32, seed=N)
+    none = codes < 0
+    clean = grad.clone()
+    clean[none] = 0.0
+    grad[none] = math.nan
+    grad[none.nonzero()[0]] = math.inf
+    want = R.lookup(codes, book, s, 1.0, clean)
+    b, sg = book.to(gpu).requires_grad_(True), s.to(gpu).requires_grad_(True)
+    gb, g_s = torch.autograd.grad(gs.lookup_codes(codes.to(gpu), b, sg), [b, sg], grad.to(gpu))
+    R.check(gb, want["g_codebook"], "g_codebook")
+    R.check(g_s, want["g_scales"], "g_scales")
+
+
 def test_balance_layouts_and_empty(gpu):
     x = _logits((2, 60), 19, F32, seed=4)
     codes = torch.randint(-1, 19, (2, 60), generator=_gen(5))
