@@ -232,25 +232,27 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
   if (threadIdx.x == 0) out.totals[at] = make_int4(sum4[0], sum4[1], sum4[2], 0);
 }
 
-// ---- the workgroups' sums joined: 64 columns of an image per workgroup, 16
-// wavefronts that each take every 16th of them.  The image's last workgroup
-// adds up the loss.
+// ---- the workgroups' sums joined: 16 columns of an image per workgroup, 64
+// slices that each take every 64th of them.  The image's last workgroup adds up
+// the loss.
 
-constexpr int kJoinWaves = 16;
+constexpr int kJoinColumns = 16;
+constexpr int kJoinSlices = 64;
+constexpr int kJoinThreads = kJoinColumns * kJoinSlices;
 
-__global__ __launch_bounds__(64 * kJoinWaves) void balance_join_kernel(
+__global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
     BalanceParams P, Partials in, float* __restrict__ loss,
     int32_t* __restrict__ counts, float* __restrict__ mean,
     int4* __restrict__ totals) {
-  __shared__ float sums[kJoinWaves][64];
-  __shared__ int nums[kJoinWaves][64];
+  __shared__ float sums[kJoinThreads];
+  __shared__ int nums[kJoinThreads];
   __shared__ int all[3];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b = blockIdx.y;
-  const int k = blockIdx.x * 64 + lane;
+  const int slice = threadIdx.x / kJoinColumns, b = blockIdx.y;
+  const int k = blockIdx.x * kJoinColumns + threadIdx.x % kJoinColumns;
   if (threadIdx.x < 3) all[threadIdx.x] = 0;
   __syncthreads();
   int4 t = make_int4(0, 0, 0, 0);
-  for (int i = threadIdx.x; i < in.count_blocks; i += 64 * kJoinWaves) {
+  for (int i = threadIdx.x; i < in.count_blocks; i += kJoinThreads) {
     const int4 q = in.totals[(int64_t)b * in.count_blocks + i];
     t.x += q.x;
     t.y += q.y;
@@ -262,43 +264,64 @@ __global__ __launch_bounds__(64 * kJoinWaves) void balance_join_kernel(
   float s = 0.0f;
   int n = 0;
   if (k < P.K) {
+    // (eight of each on their way: with loads waited for one after another the
+    // launch is latency)
     const float* ps = in.sums + (int64_t)b * in.blocks * P.K + k;
-#pragma unroll 4
-    for (int i = w; i < in.blocks; i += kJoinWaves) s += ps[(int64_t)i * P.K];
     const int32_t* pn = in.counts + (int64_t)b * in.count_blocks * P.K + k;
-#pragma unroll 4
-    for (int i = w; i < in.count_blocks; i += kJoinWaves) n += pn[(int64_t)i * P.K];
-  }
-  sums[w][lane] = s;
-  nums[w][lane] = n;
-  __syncthreads();
-  if (w != 0) return;
+    const int last = max(in.blocks, in.count_blocks);
+    for (int i0 = slice; i0 < last; i0 += 8 * kJoinSlices) {
+      float x[8];
+      int y[8];
 #pragma unroll
-  for (int j = 1; j < kJoinWaves; ++j) {
-    s += sums[j][lane];
-    n += nums[j][lane];
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kJoinSlices;
+        x[u] = i < in.blocks ? ps[(int64_t)i * P.K] : 0.0f;
+        y[u] = i < in.count_blocks ? pn[(int64_t)i * P.K] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        s += x[u];
+        n += y[u];
+      }
+    }
+  }
+  sums[threadIdx.x] = s;
+  nums[threadIdx.x] = n;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  // one wavefront: each quarter of its lanes takes every fourth slice
+  const int lane = threadIdx.x;
+  for (int j = lane + 64; j < kJoinThreads; j += 64) {
+    s += sums[j];
+    n += nums[j];
+  }
+#pragma unroll
+  for (int d = kJoinColumns; d < 64; d <<= 1) {
+    s += __shfl_xor(s, d, 64);
+    n += __shfl_xor(n, d, 64);
   }
   const float mu = s / (float)max(all[0], 1);
-  if (k < P.K) {
+  const bool mine = lane < kJoinColumns && k < P.K;
+  if (mine) {
     counts[(int64_t)b * P.K + k] = n;
     mean[(int64_t)b * P.K + k] = mu;
   }
   if (blockIdx.x == 0 && lane == 0) totals[b] = make_int4(all[0], all[1], all[2], 0);
   // (an image with nothing counted: 0, whatever the means are)
-  float l = wave_sum(n ? (float)n * mu : 0.0f);
+  float l = wave_sum(mine && n ? (float)n * mu : 0.0f);
   const float factor = (float)P.K / (float)max(all[1], 1);
   if (gridDim.x > 1) {
-    float* mine = in.loss + (int64_t)b * gridDim.x;
+    float* parts = in.loss + (int64_t)b * gridDim.x;
     uint32_t ticket = 0;
     if (lane == 0) {
-      __hip_atomic_store(&mine[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&parts[blockIdx.x], l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       ticket = __hip_atomic_fetch_add(&in.tickets[b], 1u, __ATOMIC_ACQ_REL,
                                       __HIP_MEMORY_SCOPE_AGENT);
     }
     if ((uint32_t)__builtin_amdgcn_readfirstlane((int)ticket) != gridDim.x - 1) return;
     l = 0.0f;
     for (unsigned i = lane; i < gridDim.x; i += 64)
-      l += __hip_atomic_load(&mine[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      l += __hip_atomic_load(&parts[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     l = wave_sum(l);
   }
   if (lane == 0) loss[b] = all[2] ? __builtin_nanf("") : l * factor;
@@ -530,7 +553,9 @@ int blocks_of(const BalanceParams& P) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, P.rows / least));
 }
 
-int column_groups(const BalanceParams& P) { return (P.K + 63) / 64; }
+int column_groups(const BalanceParams& P) {
+  return (P.K + kJoinColumns - 1) / kJoinColumns;
+}
 
 struct Layout {
   size_t sums, counts, totals, loss, tickets, total;
@@ -633,7 +658,7 @@ int forward_of(const BalanceParams& P, const void* logits, float* loss,
   if (rc) return rc;
   launch_traced("balance_join_kernel", balance_join_kernel,
                 dim3((unsigned)column_groups(P), (unsigned)P.batch),
-                dim3(64 * kJoinWaves), 0, stream, P, w, loss, counts, mean,
+                dim3(kJoinThreads), 0, stream, P, w, loss, counts, mean,
                 reinterpret_cast<int4*>(totals));
   return check_launch("balance_join_kernel");
 }
