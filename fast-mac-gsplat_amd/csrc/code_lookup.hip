@@ -17,6 +17,16 @@
 // what runs over the workgroup's ends goes to two partial rows, which a second
 // launch adds up.  Every workgroup has the same work however the splats are
 // spread over the codes.  The splats' rows are read once, for both gradients.
+//
+// What bounds it, on an MI355X: the forward of a million splats x 128 floats
+// over 16384 codes (8 MB of codebook, twice an XCD's L2) takes 120 us, 4.6 TB/s
+// of codes read and rows written, 6 TB/s with the codebook's misses; the
+// output's stores stream past the caches (165 us without).  Its backward: 45 us
+// of sorting (two passes of 16 us and two of 5 to 8, latency), 130 us of runs
+// (rows in sorted order are gathers of 512 bytes: 4.2 TB/s), 10 us of joining.
+// 262144 splats x 48 values: 9 us forward, and in the backward seven launches
+// of 5 to 19 us, each a chain of dependent loads, beside which the host's
+// launches and torch's autograd call take as long.
 #include <algorithm>
 
 #include "codes.h"

@@ -35,6 +35,9 @@ implementation expresses as an unbacked size.  Without the state
 (save_state=False, the eval path) render_forward returns empty final_T,
 last, tile_stop and workspace tensors.  Every op raises RuntimeError with the
 C ABI's message on failure, like the reference's TORCH_CHECK.
+
+The operators of scenes in codes (lookup_codes, code_log_probs, code_balance
+and their backwards, no counterpart in the reference) are in codes.py.
 """
 from __future__ import annotations
 
