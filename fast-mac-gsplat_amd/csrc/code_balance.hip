@@ -239,12 +239,12 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
   if (threadIdx.x == 0) out.totals[at] = make_int4(sum3[0], sum3[1], sum3[2], 0);
 }
 
-// ---- the workgroups' sums joined: 16 columns of an image per workgroup, 64
-// slices that each take every 64th of them.  The image's last workgroup adds up
+// ---- the workgroups' sums joined: 32 columns of an image per workgroup, 32
+// slices that each take every 32nd of them.  The image's last workgroup adds up
 // the loss.
 
-constexpr int kJoinColumns = 16;
-constexpr int kJoinSlices = 64;
+constexpr int kJoinColumns = 32;
+constexpr int kJoinSlices = 32;
 constexpr int kJoinThreads = kJoinColumns * kJoinSlices;
 
 __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
   nums[threadIdx.x] = n;
   __syncthreads();
   if (threadIdx.x >= 64) return;
-  // one wavefront: each quarter of its lanes takes every fourth slice
+  // one wavefront: each half of its lanes takes every second slice
   const int lane = threadIdx.x;
   for (int j = lane + 64; j < kJoinThreads; j += 64) {
     s += sums[j];
