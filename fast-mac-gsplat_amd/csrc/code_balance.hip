@@ -507,41 +507,68 @@ __global__ __launch_bounds__(kThreads) void balance_columns_kernel(
     if (k + v < P.K) to[k + v] = acc[v];
 }
 
+// Four rows of an image per workgroup, so that the columns' weights are read
+// once for four elements.
+constexpr int kLongRows = 4;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void balance_long_bwd_kernel(
     BalanceParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ counts, const float2* __restrict__ stats,
     const int4* __restrict__ totals, const float* __restrict__ g_loss,
     const float* __restrict__ g_mean, T* __restrict__ g_logits) {
+  constexpr int V = kVec<T>;
   __shared__ float red[kWaves];
-  const int64_t r = blockIdx.x;
-  const int b = (int)(r / P.rows);
-  const T* row = logits + r * P.stride;
-  T* out = g_logits + r * P.K;
-  const float2 st = stats[r];
+  const int b = blockIdx.y;
+  const int64_t first = (int64_t)blockIdx.x * kLongRows;
+  const int rows = (int)min((int64_t)kLongRows, P.rows - first);
   const int4 tot = totals[b];
   const float per_row = 1.0f / (float)max(tot.x, 1);
   const float per_count = g_loss ? g_loss[b] * ((float)P.K / (float)max(tot.y, 1)) : 0.0f;
-  auto a_of = [&](int k) {
-    if (k >= P.K) return 0.0f;
-    const float f = per_count * (float)counts[(int64_t)b * P.K + k];
-    return g_mean ? f + g_mean[(int64_t)b * P.K + k] : f;
+  const int32_t* count = counts + (int64_t)b * P.K;
+  const float* mean = g_mean ? g_mean + (int64_t)b * P.K : nullptr;
+  auto weights = [&](int k, float (&a)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      a[v] = k + v < P.K ? per_count * (float)count[k + v] : 0.0f;
+      if (mean && k + v < P.K) a[v] += mean[k + v];
+    }
   };
-  float dot = 0.0f;
-  for (int k = threadIdx.x * kVec<T>; k < P.K; k += kThreads * kVec<T>) {
-    const vec_t<T> x = load_part<T>(row, k, P.K, static_cast<T>(-INFINITY));
+  const T* x[kLongRows];
+  float2 st[kLongRows];
+  float dot[kLongRows];
 #pragma unroll
-    for (int v = 0; v < kVec<T>; ++v)
-      dot = __builtin_fmaf(prob(to_float(x[v]), st), a_of(k + v), dot);
+  for (int q = 0; q < kLongRows; ++q) {
+    const int64_t r = b * P.rows + first + min(q, rows - 1);
+    x[q] = logits + r * P.stride;
+    st[q] = stats[r];
+    dot[q] = 0.0f;
   }
-  dot = block_sum<kWaves>(dot, red);
-  for (int k = threadIdx.x * kVec<T>; k < P.K; k += kThreads * kVec<T>) {
-    const vec_t<T> x = load_part<T>(row, k, P.K, static_cast<T>(-INFINITY));
-    vec_t<T> o;
+  for (int k = threadIdx.x * V; k < P.K; k += kThreads * V) {
+    float a[V];
+    weights(k, a);
 #pragma unroll
-    for (int v = 0; v < kVec<T>; ++v)
-      o[v] = static_cast<T>(prob(to_float(x[v]), st) * (a_of(k + v) - dot) * per_row);
-    store_part<T>(out, k, P.K, o);
+    for (int q = 0; q < kLongRows; ++q) {
+      const vec_t<T> y = load_part<T>(x[q], k, P.K, static_cast<T>(-INFINITY));
+#pragma unroll
+      for (int v = 0; v < V; ++v) dot[q] = __builtin_fmaf(prob(to_float(y[v]), st[q]), a[v], dot[q]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kLongRows; ++q) dot[q] = block_sum<kWaves>(dot[q], red);
+  for (int k = threadIdx.x * V; k < P.K; k += kThreads * V) {
+    float a[V];
+    weights(k, a);
+#pragma unroll
+    for (int q = 0; q < kLongRows; ++q) {
+      if (q >= rows) break;
+      const vec_t<T> y = load_part<T>(x[q], k, P.K, static_cast<T>(-INFINITY));
+      vec_t<T> o;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        o[v] = static_cast<T>(prob(to_float(y[v]), st[q]) * (a[v] - dot[q]) * per_row);
+      store_part<T, false, true>(g_logits + (b * P.rows + first + q) * P.K, k, P.K, o);
+    }
   }
 }
 
@@ -702,8 +729,8 @@ int backward_of(const BalanceParams& P, const void* logits, const int32_t* count
                ? gradients_of<T, true>(P, x, counts, stats, totals, g_loss, g_mean, g, stream)
                : gradients_of<T, false>(P, x, counts, stats, totals, g_loss, g_mean, g, stream);
   launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T>),
-                dim3((unsigned)(P.rows * P.batch)), dim3(kThreads), 0, stream, P, x,
-                counts, stats, totals, g_loss, g_mean, g);
+                dim3((unsigned)((P.rows + kLongRows - 1) / kLongRows), (unsigned)P.batch),
+                dim3(kThreads), 0, stream, P, x, counts, stats, totals, g_loss, g_mean, g);
   return check_launch("balance_long_bwd_kernel");
 }
 

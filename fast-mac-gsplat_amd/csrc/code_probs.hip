@@ -108,6 +108,72 @@ __device__ __forceinline__ int place_among(uint64_t k, int n) {
   return place;
 }
 
+// Keys of ranks, the larger the better: for 16-bit logits and columns below 2^16
+// one word, the logit's bits in their order above the column's complement; for
+// floats rank_key.
+template <typename T>
+struct Rank {
+  using Key = uint64_t;
+  static __device__ __forceinline__ Key of(T x, uint32_t i) { return rank_key(x, i); }
+  static __device__ __forceinline__ uint32_t column(Key k) { return ~(uint32_t)k; }
+  static __device__ __forceinline__ float logit(Key k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+  }
+  template <int L>
+  static __device__ __forceinline__ Key best(Key k) { return team_best<L>(k); }
+};
+template <typename T>
+struct Rank16 {
+  using Key = uint32_t;
+  static __device__ __forceinline__ Key of(T x, uint32_t i) {
+    uint32_t u = __builtin_bit_cast(uint16_t, x);
+    if (x == static_cast<T>(0.0f)) u = 0;
+    if (!(x == x)) u = 0x7fff;
+    return (u & 0x8000u ? ~u << 16 : (u | 0x8000u) << 16) | (0xffffu - i);
+  }
+  static __device__ __forceinline__ uint32_t column(Key k) { return 0xffffu - (k & 0xffffu); }
+  static __device__ __forceinline__ float logit(Key k) {
+    const uint32_t u = k >> 16;
+    return to_float(__builtin_bit_cast(T, (uint16_t)(u & 0x8000u ? u ^ 0x8000u : ~u)));
+  }
+  template <int L>
+  static __device__ __forceinline__ Key best(Key k) { return team_umax<L>(k); }
+};
+template <>
+struct Rank<__bf16> : Rank16<__bf16> {};
+template <>
+struct Rank<_Float16> : Rank16<_Float16> {};
+
+// A lane's E keys (4 or 8), the best first: an odd-even merge network.
+template <int E, typename Key>
+__device__ __forceinline__ void sort_keys(Key (&k)[E]) {
+  auto order = [&](int a, int b) {
+    const Key hi = k[a] > k[b] ? k[a] : k[b], lo = k[a] > k[b] ? k[b] : k[a];
+    k[a] = hi;
+    k[b] = lo;
+  };
+#pragma unroll
+  for (int h = 0; h < E; h += 4) {
+    order(h, h + 1);
+    order(h + 2, h + 3);
+    order(h, h + 2);
+    order(h + 1, h + 3);
+    order(h + 1, h + 2);
+  }
+  if constexpr (E == 8) {
+    order(0, 4);
+    order(1, 5);
+    order(2, 6);
+    order(3, 7);
+    order(2, 4);
+    order(3, 5);
+    order(1, 2);
+    order(3, 4);
+    order(5, 6);
+  }
+}
+
 struct ProbsOut {
   float* log_probs;
   float* entropy;
@@ -263,6 +329,33 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
       out.top_log_probs[n * top + j] = e.log_prob(v);
     }
   };
+  if constexpr (TL < 64 && R == 1) {
+    // Several codes of a narrow team: every lane sorts its keys, and in each
+    // turn the team's best head is taken and its lane goes on to its next.
+    if (top > 1) {
+      using K = Rank<T>;
+      constexpr int V = kVec<T>;
+      typename K::Key k[V], mine_key = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) k[v] = K::of(x.x[0][v], x.column(0, v));
+      sort_keys<V>(k);
+      for (int j = 0; j < top; ++j) {
+        const typename K::Key best = K::template best<TL>(k[0]);
+        if (k[0] == best) {
+#pragma unroll
+          for (int v = 0; v + 1 < V; ++v) k[v] = k[v + 1];
+          k[V - 1] = 0;
+        }
+        if (lane == (j & (TL - 1))) mine_key = best;
+        // (as many as the team has lanes are written at once)
+        if ((j & (TL - 1)) == TL - 1 || j == top - 1) {
+          const int at = (j & ~(TL - 1)) + lane;
+          if (at <= j) put(at, K::column(mine_key), K::logit(mine_key));
+        }
+      }
+      return;
+    }
+  }
   int from = 0;
   const bool plain = p.s == p.s;  // (no NaN)
   if (plain) {
@@ -521,6 +614,10 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     const float* __restrict__ g_entropy, const float* __restrict__ g_top,
     T* __restrict__ g_logits, int parts) {
   constexpr int kTeams = kThreads / TL, V = kVec<T>, kSpan = TL * V * R;
+  // Gradients of single columns: rows of one team add them up in LDS, a lane per
+  // alternative (R = 4: rows of several parts, whose few columns are compared).
+  constexpr bool kSpread = R < 4;
+  __shared__ alignas(16) float spread[kSpread ? kThreads * V * R : 1];
   const int lane = threadIdx.x & (TL - 1);
   const int team = TL == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TL) : threadIdx.x / TL;
   const int64_t i = (int64_t)blockIdx.x * kTeams + team;
@@ -546,7 +643,27 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   const int top = g_top && some ? P.top : 0;
   const float* gt = g_top + n * P.top;
   const int32_t* tc = top_codes + n * P.top;
-  for (int j = 0; j < top; ++j) total += gt[j];
+  float* mine = spread + (threadIdx.x - lane) * (V * R);  // (the team's columns)
+  if constexpr (kSpread) {
+    if (top > 0) {
+#pragma unroll
+      for (int v = 0; v < V * R; v += 4)
+        *reinterpret_cast<float4*>(&mine[lane * (V * R) + v]) = make_float4(0, 0, 0, 0);
+      __builtin_amdgcn_wave_barrier();
+      float sum = 0.0f;
+      for (int j = lane; j < top; j += TL) {
+        const float w = gt[j];
+        const unsigned col = (unsigned)(tc[j] - first);
+        sum += w;
+        // (a column may also be the code's: two additions, in either order)
+        if (col < (unsigned)kSpan) atomicAdd(&mine[col], w * P.inv_t);
+      }
+      total += team_sum<TL>(sum);
+      __builtin_amdgcn_wave_barrier();
+    }
+  } else {
+    for (int j = 0; j < top; ++j) total += gt[j];
+  }
   // 16 bits of a result: exponents 32 up, so that probabilities that the
   // hardware's exponential flushes are far below the type's smallest step (the
   // exponents' own steps, 4e-6 there, are lost in 16 bits).  32 bits: exp2_full.
@@ -578,17 +695,31 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     if (rel >= (unsigned)kSpan) return;
     // (of a wavefront's row the place is the same for all lanes: one vector's
     // elements are looked at)
-    const float mine = lane == (int)(rel / V & (TL - 1)) ? w : 0.0f;
+    const float own = lane == (int)(rel / V & (TL - 1)) ? w : 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const unsigned in = rel - r * (V * TL);
       if (R > 1 && in >= (unsigned)(V * TL)) continue;
 #pragma unroll
-      for (int v = 0; v < V; ++v) g[r * V + v] += in % V == (unsigned)v ? mine : 0.0f;
+      for (int v = 0; v < V; ++v) g[r * V + v] += in % V == (unsigned)v ? own : 0.0f;
     }
   };
   if (code >= 0) add(code, gl);
-  for (int j = 0; j < top; ++j) add(tc[j], gt[j] * P.inv_t);
+  if constexpr (kSpread) {
+    if (top > 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; v += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(&mine[(r * TL + lane) * V + v]);
+          g[r * V + v] += w.x;
+          g[r * V + v + 1] += w.y;
+          g[r * V + v + 2] += w.z;
+          g[r * V + v + 3] += w.w;
+        }
+  } else {
+    for (int j = 0; j < top; ++j) add(tc[j], gt[j] * P.inv_t);
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     vec_t<T> o;
