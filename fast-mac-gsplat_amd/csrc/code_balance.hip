@@ -507,11 +507,9 @@ __global__ __launch_bounds__(kThreads) void balance_columns_kernel(
     if (k + v < P.K) to[k + v] = acc[v];
 }
 
-// Four rows of an image per workgroup, so that the columns' weights are read
-// once for four elements.
-constexpr int kLongRows = 4;
-
-template <typename T>
+// kLongRows rows of an image per workgroup, so that the columns' weights are
+// read once for as many elements.
+template <typename T, int kLongRows>
 __global__ __launch_bounds__(kThreads) void balance_long_bwd_kernel(
     BalanceParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ counts, const float2* __restrict__ stats,
@@ -578,7 +576,8 @@ constexpr int kLongest = 16384;  // codes of a row that a workgroup holds
 
 // Workgroups per image of the row pass.  A workgroup leaves 8 bytes per code,
 // so it takes at least 32 bytes of every column (a quarter of that again); 1024
-// workgroups in all keep the GPU busy.
+// workgroups in all keep the GPU busy (200K rows x 4096 368 us, with 512 476,
+// with 2048 371; four images x 256 54, 60, 59).
 int blocks_of(const BalanceParams& P) {
   if (P.rows == 0) return 1;
   if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
@@ -728,9 +727,17 @@ int backward_of(const BalanceParams& P, const void* logits, const int32_t* count
     return P.K % kVec<T> == 0
                ? gradients_of<T, true>(P, x, counts, stats, totals, g_loss, g_mean, g, stream)
                : gradients_of<T, false>(P, x, counts, stats, totals, g_loss, g_mean, g, stream);
-  launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T>),
-                dim3((unsigned)((P.rows + kLongRows - 1) / kLongRows), (unsigned)P.batch),
-                dim3(kThreads), 0, stream, P, x, counts, stats, totals, g_loss, g_mean, g);
+#define GS_LONG(Q)                                                              \
+  launch_traced("balance_long_bwd_kernel", (balance_long_bwd_kernel<T, Q>),     \
+                dim3((unsigned)((P.rows + Q - 1) / Q), (unsigned)P.batch),      \
+                dim3(kThreads), 0, stream, P, x, counts, stats, totals, g_loss, \
+                g_mean, g)
+  // (4096 rows of 32768: 430 us in 32 bits with four rows, 602 with one, 281 and
+  // 915 in 16; 1342 rows of 100000: 909, 859 and 706 us in 32 bits with four, two
+  // and one, 577, 619 and 1061 in 16)
+  if (sizeof(T) == 2 || P.rows * P.batch >= 4096) GS_LONG(4);
+  else GS_LONG(1);
+#undef GS_LONG
   return check_launch("balance_long_bwd_kernel");
 }
 

@@ -44,8 +44,7 @@ __device__ __forceinline__ float nan_for(int c) {
 
 // Each thread writes kUnroll vectors of 16 bytes of the output, taken as one
 // array; block b starts at element b * kThreads * V * kUnroll.  div: the
-// quotient of a 32-bit offset by D (below).  Four vectors keep four chains of
-// loads (code, row) on their way; one where that leaves CUs without work.
+// quotient of a 32-bit offset by D (below).
 
 // n / d for n < 2^31 by one 32 x 32 multiplication: floor(n m / 2^(32 + s))
 // with m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1 (exact for n < 2^31: the
@@ -71,9 +70,8 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
   const int64_t start = (int64_t)blockIdx.x * (kThreads * V * kUnroll);
   const int64_t row0 = start / P.D;
   const uint32_t skip = (uint32_t)(start - row0 * P.D);
-  int64_t at[kUnroll];
+  int64_t at[kUnroll], n[kUnroll];
   uint32_t d[kUnroll];
-  int64_t n[kUnroll];
   int c[kUnroll];
   float s[kUnroll];
 #pragma unroll
@@ -88,12 +86,12 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     s[u] = P.factor;
     if (scales && in) s[u] *= scales[n[u]];
   }
-  vec_t<T> x[kUnroll];
+  vec_t<T> y[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const T* row = codebook + (int64_t)max(c[u], 0) * P.stride;
     if (Rows || d[u] + V <= (uint32_t)P.D) {
-      x[u] = load_vec(row + d[u]);
+      y[u] = load_vec(row + d[u]);
     } else {
       // the vector goes on in the next rows
       uint32_t e = d[u];
@@ -102,9 +100,9 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
       float f = s[u];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float y = nan_for(k);
-        if (k >= 0) y = to_float(codebook[(int64_t)k * P.stride + e]) * f;
-        x[u][v] = static_cast<T>(y);
+        float z = nan_for(k);
+        if (k >= 0) z = to_float(codebook[(int64_t)k * P.stride + e]) * f;
+        y[u][v] = static_cast<T>(z);
         if (++e == (uint32_t)P.D) {
           e = 0;
           ++r;
@@ -119,18 +117,16 @@ __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     if (at[u] >= total) continue;
-    vec_t<T> y = x[u];
-    if (Rows || d[u] + V <= (uint32_t)P.D) {
+    if (Rows || d[u] + V <= (uint32_t)P.D)
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        y[v] = static_cast<T>(c[u] >= 0 ? to_float(x[u][v]) * s[u] : nan_for(c[u]));
-    }
+        y[u][v] = static_cast<T>(c[u] >= 0 ? to_float(y[u][v]) * s[u] : nan_for(c[u]));
     if (at[u] + V <= total) {
-      store_vec_stream(out + at[u], y);
+      store_vec_stream(out + at[u], y[u]);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (at[u] + v < total) out[at[u] + v] = y[v];
+        if (at[u] + v < total) out[at[u] + v] = y[u][v];
     }
   }
 }
@@ -670,14 +666,20 @@ int forward_of(const LookupParams& P, const void* codebook, const float* scales,
   const T* book = static_cast<const T*>(codebook);
   T* o = static_cast<T*>(out);
   const Divide div((uint32_t)P.D);
+  // Four vectors a thread, with as many chains of loads on their way, where the
+  // codebook does not fit an XCD's 4 MB of L2 (a million splats x 128 floats over
+  // 16384 codes: 120 us against 133); one where it does (over 4096 codes 82
+  // against 88, 262144 x 48 6.3 against 7.0, 64K x 11 4.2 against 7.8).
+  const bool missing = (int64_t)P.K * P.D * sizeof(T) > (int64_t(4) << 20) &&
+                       vecs >= (int64_t)kThreads * 4 * 1024;
 #define GS_LOOKUP(ROWS, U)                                                      \
   launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, ROWS, U>),           \
                 dim3((unsigned)((vecs + kThreads * U - 1) / (kThreads * U))),   \
                 dim3(kThreads), 0, stream, P, div, book, scales, o)
-  const bool rows = P.D % kVec<T> == 0, many = vecs >= (int64_t)kThreads * 4 * 1024;
-  if (rows && many) GS_LOOKUP(true, 4);
+  const bool rows = P.D % kVec<T> == 0;
+  if (rows && missing) GS_LOOKUP(true, 4);
   else if (rows) GS_LOOKUP(true, 1);
-  else if (many) GS_LOOKUP(false, 4);
+  else if (missing) GS_LOOKUP(false, 4);
   else GS_LOOKUP(false, 1);
 #undef GS_LOOKUP
   return check_launch("lookup_fwd_kernel");
@@ -703,7 +705,8 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
   }
   if (!g_book) return GSPLAT_OK;
   if (few(P)) {
-    // (four codes a workgroup where that leaves 1024 of them)
+    // (four codes a workgroup where that leaves 1024 of them: 1024 splats x 64,
+    // 16384 codes 16 us against 25 with one, 4096 codes 8 against 9)
 #define GS_SCAN_OF(TL, R, Q)                                                      \
     launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R, Q, Even>),  \
                   dim3((unsigned)((P.K + Q - 1) / Q), tiles), dim3(kThreads), 0,  \

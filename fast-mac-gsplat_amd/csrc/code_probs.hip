@@ -735,7 +735,8 @@ constexpr int kPartLong = 16384;
 Split split_of(const ProbsParams& P) {
   Split s{1, P.K, nullptr, nullptr, past_caches(P.rows, P.K, P.dtype)};
   if (P.K <= kPartLong) return s;
-  // Few rows: shorter parts, until there is one for each of 512 workgroups.
+  // Few rows: shorter parts, until there is one for each of 512 workgroups (one
+  // row of 131072: 8.0 us against 9.6, 64 rows of 32768 8.7 against 10.1).
   int64_t length = kPartLong;
   while (length > 2048 && P.rows * ((P.K + length - 1) / length) < 512) length /= 2;
   s.length = (int)length;
