@@ -20,6 +20,7 @@
 // (6 TB/s); 200K rows x 4096 in bf16 358 us (4.6 TB/s, VALU issue beside HBM)
 // and 635 us (5.2 TB/s).
 #include <algorithm>
+#include <type_traits>
 
 #include "codes.h"
 
@@ -93,9 +94,6 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
   int32_t* hist = lds;
   float* sums = reinterpret_cast<float*>(lds + P.K);
   const int b = blockIdx.y;
-  const int64_t per = (P.rows + out.blocks - 1) / out.blocks;
-  const int64_t first = blockIdx.x * per;
-  const int64_t count = max((int64_t)0, min(per, P.rows - first));
   for (int k = threadIdx.x; k < P.K; k += G::kThreads) hist[k] = 0;
   if (threadIdx.x < 3) sum3[threadIdx.x] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) out.tickets[b] = 0;
@@ -115,18 +113,19 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
     else
       G::load(x, row, P.K);
   };
-  const int64_t base_row = b * P.rows + first;
-  auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
-  int64_t i = G::team();
+  const int64_t base_row = b * P.rows, step = (int64_t)gridDim.x * G::kTeams;
+  auto row_of = [&](int64_t i) { return base_row + min(i, P.rows - 1); };
+  int64_t from = (int64_t)blockIdx.x * G::kTeams;  // the workgroup's first row of a turn
+  int64_t i = from + G::team();
   int code = kNoCode;
-  if (count > 0) {
+  if (from < P.rows) {
     load(logits + row_of(i) * P.stride);
     if (lane < S) code = P.codes.at(row_of(i) * S + lane, P.K);
   }
   // (every team makes the same number of turns; those past the rows count nothing)
-  for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
+  for (int turn = 0; from < P.rows; turn ^= 1, from += step, i += step) {
     const int64_t r0 = row_of(i);
-    const bool here = i < count;
+    const bool here = i < P.rows;
     Choices mine;
     if (here) {
       int32_t* h = w == 0 ? hist : nullptr;
@@ -164,8 +163,8 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
       powers([&](float y) { return ex.fast(y); });
     else
       powers([&](float y) { return ex.slow(y); });
-    if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
-      const int64_t rn = row_of(i + G::kTeams);
+    if (from + step < P.rows) {  // (x is free: the next row)
+      const int64_t rn = row_of(i + step);
       load(logits + rn * P.stride);
       code = lane < S ? P.codes.at(rn * S + lane, P.K) : kNoCode;
     }
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
     // (the powers lack ex.shift: it cancels from e / s, not from log2 s)
     float base = ex.m, shift = ex.shift, f = 1.0f;
     if constexpr (W > 1) {  // (two sets of slots: one barrier a row)
-      float2* slot = slots[turn & 1][W > 1 ? G::team() : 0];
+      float2* slot = slots[turn][W > 1 ? G::team() : 0];
       if (lane == 0) slot[w] = make_float2(m, s * exp2_fast(shift));
       __syncthreads();
       const float2 q = slot[lane & (W - 1)];
@@ -216,46 +215,52 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
     for (int q = 0; q < G::kThreads / (64 * W); ++q) {
       if (group == q && (threadIdx.x & 63) < TL)
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+          const int k = G::column(r);
+          if (k >= P.K) continue;
+          float had[V];  // (reads, then writes: both in whole vectors)
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const int k = G::column(r) + v;
-            if (k < P.K) sums[k] = q == 0 ? acc[r * V + v] : sums[k] + acc[r * V + v];
-          }
+          for (int v = 0; v < V; ++v) had[v] = q == 0 || (!Even && k + v >= P.K) ? 0.0f : sums[k + v];
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (Even || k + v < P.K) sums[k + v] = had[v] + acc[r * V + v];
+        }
       __syncthreads();
     }
     for (int k = threadIdx.x; k < P.K; k += G::kThreads) out.sums[at * P.K + k] = sums[k];
   } else {
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      const int k = G::column(r);
+      float* to = out.sums + at * P.K + k;
+      if (k >= P.K) continue;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int k = G::column(r) + v;
-        if (k < P.K) out.sums[at * P.K + k] = acc[r * V + v];
-      }
+      for (int v = 0; v < V; ++v)
+        if (Even || k + v < P.K) to[v] = acc[r * V + v];
+    }
   }
   for (int k = threadIdx.x; k < P.K; k += G::kThreads) out.counts[at * P.K + k] = hist[k];
   if (threadIdx.x == 0) out.totals[at] = make_int4(sum3[0], sum3[1], sum3[2], 0);
 }
 
-// ---- the workgroups' sums joined: 32 columns of an image per workgroup, 32
-// slices that each take every 32nd of them.  The image's last workgroup adds up
-// the loss.
+// ---- the workgroups' sums joined: Columns (32 or 64) columns of an image per
+// workgroup, whole cache lines, in slices that each take every so many-th of the
+// sums.  The image's last workgroup adds up the loss.
 
-constexpr int kJoinColumns = 32;
-constexpr int kJoinSlices = 32;
-constexpr int kJoinThreads = kJoinColumns * kJoinSlices;
+constexpr int kJoinThreads = 1024;
 
+template <int Columns>
 __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
     BalanceParams P, Partials in, float* __restrict__ loss,
     int32_t* __restrict__ counts, float* __restrict__ mean,
     int4* __restrict__ totals) {
+  constexpr int kSlices = kJoinThreads / Columns;
   __shared__ float sums[kJoinThreads];
   __shared__ int nums[kJoinThreads];
   __shared__ int all[3];
-  const int slice = threadIdx.x / kJoinColumns, b = blockIdx.y;
-  const int k = blockIdx.x * kJoinColumns + threadIdx.x % kJoinColumns;
+  const int slice = threadIdx.x / Columns, b = blockIdx.y;
+  const int k = blockIdx.x * Columns + threadIdx.x % Columns;
   if (threadIdx.x < 3) all[threadIdx.x] = 0;
   __syncthreads();
   int4 t = make_int4(0, 0, 0, 0);
@@ -276,12 +281,12 @@ __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
     const float* ps = in.sums + (int64_t)b * in.blocks * P.K + k;
     const int32_t* pn = in.counts + (int64_t)b * in.count_blocks * P.K + k;
     const int last = max(in.blocks, in.count_blocks);
-    for (int i0 = slice; i0 < last; i0 += 8 * kJoinSlices) {
+    for (int i0 = slice; i0 < last; i0 += 8 * kSlices) {
       float x[8];
       int y[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * kJoinSlices;
+        const int i = i0 + u * kSlices;
         x[u] = i < in.blocks ? ps[(int64_t)i * P.K] : 0.0f;
         y[u] = i < in.count_blocks ? pn[(int64_t)i * P.K] : 0;
       }
@@ -296,19 +301,19 @@ __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
   nums[threadIdx.x] = n;
   __syncthreads();
   if (threadIdx.x >= 64) return;
-  // one wavefront: each half of its lanes takes every second slice
+  // one wavefront: its lanes take every slice, or each half of them every second
   const int lane = threadIdx.x;
   for (int j = lane + 64; j < kJoinThreads; j += 64) {
     s += sums[j];
     n += nums[j];
   }
 #pragma unroll
-  for (int d = kJoinColumns; d < 64; d <<= 1) {
+  for (int d = Columns; d < 64; d <<= 1) {
     s += __shfl_xor(s, d, 64);
     n += __shfl_xor(n, d, 64);
   }
   const float mu = s / (float)max(all[0], 1);
-  const bool mine = lane < kJoinColumns && k < P.K;
+  const bool mine = lane < Columns && k < P.K;
   if (mine) {
     counts[(int64_t)b * P.K + k] = n;
     mean[(int64_t)b * P.K + k] = mu;
@@ -336,7 +341,7 @@ __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(
 
 // ---- backward
 
-template <typename T, int TL, int W, int R, bool Even>
+template <typename T, int TL, int W, int R, bool Even, bool Past>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_kernel(
     BalanceParams P, const T* __restrict__ logits,
     const int32_t* __restrict__ counts, const float2* __restrict__ stats,
@@ -347,34 +352,34 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
   constexpr float kUp = sizeof(T) == 2 ? 32.0f : 0.0f;
   __shared__ float slots[2][G::kTeams][W];
   const int b = blockIdx.y;
-  const int64_t per = (P.rows + gridDim.x - 1) / gridDim.x;
-  const int64_t first = blockIdx.x * per;
-  const int64_t count = min(per, P.rows - first);
-  if (count <= 0) return;
   const int lane = threadIdx.x & (TL - 1), w = G::wave();
   const int4 tot = totals[b];
   const float per_row = 1.0f / (float)max(tot.x, 1);
   const float per_count = g_loss ? g_loss[b] * ((float)P.K / (float)max(tot.y, 1)) : 0.0f;
   float a[R * V];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) {
+    // (without a branch, and in whole vectors where the rows are)
+    const int k = G::column(r), last = k < P.K ? k : 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int k = G::column(r) + v;
-      float f = 0.0f;
-      if (k < P.K) {
-        f = per_count * (float)counts[(int64_t)b * P.K + k];
-        if (g_mean) f += g_mean[(int64_t)b * P.K + k];
-      }
-      a[r * V + v] = f;
-    }
-  const int64_t base_row = b * P.rows + first;
-  auto row_of = [&](int64_t i) { return base_row + min(i, count - 1); };
-  int64_t i = G::team();
+    for (int v = 0; v < V; ++v)
+      a[r * V + v] = per_count * (float)(counts + (int64_t)b * P.K)[Even ? last + v : min(k + v, P.K - 1)];
+    if (g_mean)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        a[r * V + v] += (g_mean + (int64_t)b * P.K)[Even ? last + v : min(k + v, P.K - 1)];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (k + v >= P.K) a[r * V + v] = 0.0f;
+  }
+  const int64_t base_row = b * P.rows, step = (int64_t)gridDim.x * G::kTeams;
+  auto row_of = [&](int64_t i) { return base_row + min(i, P.rows - 1); };
+  int64_t from = (int64_t)blockIdx.x * G::kTeams;  // the workgroup's first row of a turn
+  int64_t i = from + G::team();
   vec_t<T> x[R];
   G::template load<true>(x, logits + row_of(i) * P.stride, P.K);
   float2 st = stats[row_of(i)];
-  for (int64_t turn = 0; turn * G::kTeams < count; ++turn, i += G::kTeams) {
+  for (int turn = 0; from < P.rows; turn ^= 1, from += step, i += step) {
     const int64_t r0 = row_of(i);
     // p = 2^(t + down) with t from Exponent (16 bits: exponents 32 up, as in
     // code_probs.hip); a row that takes no part has log2 s = inf and p = 0.
@@ -400,19 +405,19 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
       products([&](float y) { return ex.fast(y); });
     else
       products([&](float y) { return ex.slow(y); });
-    if ((turn + 1) * G::kTeams < count) {  // (x is free: the next row)
-      const int64_t rn = row_of(i + G::kTeams);
+    if (from + step < P.rows) {  // (x is free: the next row)
+      const int64_t rn = row_of(i + step);
       G::template load<true>(x, logits + rn * P.stride, P.K);
       st = stats[rn];
     }
     dot = team_sum<TL>(dot) * down;
     if constexpr (W > 1) {
-      float* slot = slots[turn & 1][W > 1 ? G::team() : 0];
+      float* slot = slots[turn][W > 1 ? G::team() : 0];
       if (lane == 0) slot[w] = dot;
       __syncthreads();
       dot = team_sum<W>(slot[lane & (W - 1)]);
     }
-    if (i < count) {
+    if (i < P.rows) {
       T* out = g_logits + r0 * P.K;
       const float f = down * per_row, less = -dot * f;
 #pragma unroll
@@ -423,7 +428,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
           const int j = r * V + v;
           o[v] = static_cast<T>(p[j] * __builtin_fmaf(a[j], f, less));
         }
-        store_part<T, Even, true>(out, G::column(r), P.K, o);
+        store_part<T, Even, Past>(out, G::column(r), P.K, o);
       }
     }
   }
@@ -578,16 +583,34 @@ constexpr int kLongest = 16384;  // codes of a row that a workgroup holds
 // so it takes at least 32 bytes of every column (a quarter of that again); 1024
 // workgroups in all keep the GPU busy (200K rows x 4096 368 us, with 512 476,
 // with 2048 371; four images x 256 54, 60, 59).
+// Teams of a workgroup of the kernel that GS_TEAMS takes.
+int teams_of(const BalanceParams& P) {
+  const int per = P.dtype != GSPLAT_F32 && P.K > 1024 && P.K % 8 == 0 ? 32 : 16;
+  int threads = 2;
+  while (threads * per < P.K) threads *= 2;
+  return std::max(1, 256 / threads);
+}
+
 int blocks_of(const BalanceParams& P) {
   if (P.rows == 0) return 1;
   if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
-  const int64_t least = P.dtype == GSPLAT_F32 ? 8 : 16;
+  // two rows for each team, at least: what a workgroup costs at its start and
+  // end, and the join its sums, is then worth it (16384 rows of 64 floats: 14 us,
+  // 17 with eight rows a workgroup; 1024 of 4096 in bf16 20 and 27)
+  const int64_t least = 2 * teams_of(P);
   const int64_t most = std::max<int64_t>(1, (P.K > 8192 ? 256 : P.K > 4096 ? 512 : 1024) / P.batch);
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, P.rows / least));
 }
 
+// (The tickets of an image's workgroups are taken one after another, 33 ns each:
+// above 4096 columns in all, half as many workgroups.  Four images of 8192 codes
+// 18 us and 37, of 2048 11 and 13; one of 4096 17.5 and 15.)
+int join_columns(const BalanceParams& P) {
+  return (int64_t)P.K * P.batch > 4096 ? 64 : 32;
+}
+
 int column_groups(const BalanceParams& P) {
-  return (P.K + kJoinColumns - 1) / kJoinColumns;
+  return (P.K + join_columns(P) - 1) / join_columns(P);
 }
 
 struct Layout {
@@ -689,7 +712,8 @@ int forward_of(const BalanceParams& P, const void* logits, float* loss,
     }
   }
   if (rc) return rc;
-  launch_traced("balance_join_kernel", balance_join_kernel,
+  launch_traced("balance_join_kernel",
+                join_columns(P) == 64 ? balance_join_kernel<64> : balance_join_kernel<32>,
                 dim3((unsigned)column_groups(P), (unsigned)P.batch),
                 dim3(kJoinThreads), 0, stream, P, w, loss, counts, mean,
                 reinterpret_cast<int4*>(totals));
@@ -701,15 +725,29 @@ int gradients_of(const BalanceParams& P, const T* x, const int32_t* counts,
                  const float2* stats, const int4* totals, const float* g_loss,
                  const float* g_mean, T* g, hipStream_t stream) {
   const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
+  // Gradients go past the caches where they are more than the last one holds and
+  // what a store writes of a row is whole lines, or long: 512 MiB of rows of
+  // 1024 floats 188 us so and 201 through the caches, 256 MiB 96 and 87; 1M rows
+  // of 100 floats (128 bytes of a row per store, anywhere in its lines) 276 and
+  // 188, of 32 (half a line) 140 and 81.
+  const bool large = P.rows * P.batch * P.K * (int64_t)sizeof(T) > (int64_t(256) << 20);
+  const bool whole = P.K * sizeof(T) % 128 == 0;
 #define GS_BWD(TL, W, R)                                                      \
   {                                                                           \
     using G = Team<T, TL, W, R, Even>;                                              \
     const int64_t most = std::max(1, (W > 4 ? 4096 / W : 1024) / P.batch);         \
     const int64_t turns = (P.rows + G::kTeams - 1) / G::kTeams;               \
-    launch_traced("balance_bwd_kernel", (balance_bwd_kernel<T, TL, W, R, Even>),    \
-                  dim3((unsigned)std::min(most, turns), (unsigned)P.batch),   \
-                  dim3(G::kThreads), 0, stream, P, x, counts, stats, totals,  \
-                  g_loss, g_mean, g);                                         \
+    auto launch = [&](auto past) {                                            \
+      launch_traced("balance_bwd_kernel",                                     \
+                    (balance_bwd_kernel<T, TL, W, R, Even, past.value>),      \
+                    dim3((unsigned)std::min(most, turns), (unsigned)P.batch), \
+                    dim3(G::kThreads), 0, stream, P, x, counts, stats,        \
+                    totals, g_loss, g_mean, g);                               \
+    };                                                                        \
+    if (TL >= 8 && large && (TL >= 32 || whole))                              \
+      launch(std::integral_constant<bool, (TL >= 8)>{});                      \
+    else                                                                      \
+      launch(std::false_type{});                                              \
     return check_launch("balance_bwd_kernel");                                \
   }
   GS_TEAMS(GS_BWD)
