@@ -28,12 +28,15 @@ namespace gs {
 namespace {
 
 // A team reads a row once and holds it in registers: TL lanes of one wavefront
-// (W = 1), or W wavefronts.  A thread holds R vectors, 16 elements of most rows
-// and 32 of those above 1024 codes in 16 bits, of the row at hand, its probabilities and
+// (W = 1), or W wavefronts.  A thread holds R vectors (12 or 16 floats, 16 or 24
+// elements of 16 bits, 32 of long rows) of the row at hand, its probabilities and
 // (forward) its columns' sums or (backward) its columns' a; the next row is
 // loaded once its probabilities are there.  What a row costs besides its elements
 // (reductions, its choices) is the same for a lane with 4 elements and one
-// with 32, so teams are as narrow as that allows.
+// with 32, so teams are as narrow as that allows.  The workgroups take rows in
+// turn, so that all of them together move through the logits from front to back
+// (each in a range of its own: 512K rows of 256 floats 122 us forward and 208
+// backward; in turn 113 and 186).
 //
 // (Four wavefronts per SIMD: the compiler would otherwise take more registers
 // than it needs with 32 elements a lane.)
@@ -48,11 +51,20 @@ struct Team {
   static __device__ __forceinline__ int member() { return threadIdx.x & (TL * W - 1); }
   static __device__ __forceinline__ int wave() { return W > 1 ? (threadIdx.x >> 6) & (W - 1) : 0; }
   static __device__ __forceinline__ int column(int r) { return (r * TL * W + member()) * V; }
-  template <bool Stream = false>
+  // (Late: fix is called once the vectors are there.  The backward of 32 bits is
+  // better without: 522K rows of 257 floats 245 us, 263 with.)
+  template <bool Stream, bool Late = true>
   static __device__ __forceinline__ void load(vec_t<T> (&x)[R], const T* row, int K) {
+    const T fill = static_cast<T>(-INFINITY);
+    if constexpr (Late) {
+      load_row<T, R, Even, Stream>(x, row, column(0), TL * W * V, K, fill);
+    } else {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      x[r] = load_part<T, Even, Stream>(row, column(r), K, static_cast<T>(-INFINITY));
+      for (int r = 0; r < R; ++r) x[r] = load_part<T, Even, Stream>(row, column(r), K, fill);
+    }
+  }
+  static __device__ __forceinline__ void fix(vec_t<T> (&x)[R], int K) {
+    fix_row<T, R, Even>(x, column(0), TL * W * V, K, static_cast<T>(-INFINITY));
   }
 };
 
@@ -111,7 +123,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
     if (out.stream)
       G::template load<true>(x, row, P.K);
     else
-      G::load(x, row, P.K);
+      G::template load<false>(x, row, P.K);
   };
   const int64_t base_row = b * P.rows, step = (int64_t)gridDim.x * G::kTeams;
   auto row_of = [&](int64_t i) { return base_row + min(i, P.rows - 1); };
@@ -124,6 +136,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_rows_ke
   }
   // (every team makes the same number of turns; those past the rows count nothing)
   for (int turn = 0; from < P.rows; turn ^= 1, from += step, i += step) {
+    G::fix(x, P.K);
     const int64_t r0 = row_of(i);
     const bool here = i < P.rows;
     Choices mine;
@@ -377,9 +390,10 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
   int64_t from = (int64_t)blockIdx.x * G::kTeams;  // the workgroup's first row of a turn
   int64_t i = from + G::team();
   vec_t<T> x[R];
-  G::template load<true>(x, logits + row_of(i) * P.stride, P.K);
+  G::template load<true, sizeof(T) == 2>(x, logits + row_of(i) * P.stride, P.K);
   float2 st = stats[row_of(i)];
   for (int turn = 0; from < P.rows; turn ^= 1, from += step, i += step) {
+    if (sizeof(T) == 2) G::fix(x, P.K);
     const int64_t r0 = row_of(i);
     // p = 2^(t + down) with t from Exponent (16 bits: exponents 32 up, as in
     // code_probs.hip); a row that takes no part has log2 s = inf and p = 0.
@@ -407,7 +421,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) GS_WAVES void balance_bwd_ker
       products([&](float y) { return ex.slow(y); });
     if (from + step < P.rows) {  // (x is free: the next row)
       const int64_t rn = row_of(i + step);
-      G::template load<true>(x, logits + rn * P.stride, P.K);
+      G::template load<true, sizeof(T) == 2>(x, logits + rn * P.stride, P.K);
       st = stats[rn];
     }
     dot = team_sum<TL>(dot) * down;
@@ -585,9 +599,11 @@ constexpr int kLongest = 16384;  // codes of a row that a workgroup holds
 // with 2048 371; four images x 256 54, 60, 59).
 // Teams of a workgroup of the kernel that GS_TEAMS takes.
 int teams_of(const BalanceParams& P) {
-  const int per = P.dtype != GSPLAT_F32 && P.K > 1024 && P.K % 8 == 0 ? 32 : 16;
+  const bool narrow = P.dtype != GSPLAT_F32;
   int threads = 2;
-  while (threads * per < P.K) threads *= 2;
+  while (threads < 64 && threads * (narrow ? 24 : 16) < P.K) threads *= 2;
+  if (threads * (narrow ? 24 : 16) < P.K)
+    while (threads * (narrow && P.K % 8 == 0 ? 32 : 16) < P.K) threads *= 2;
   return std::max(1, 256 / threads);
 }
 
@@ -635,26 +651,37 @@ Layout layout(const BalanceParams& P) {
   return L;
 }
 
-// The kernel for rows of K codes: CALL(TL, W, R).
-#define GS_TEAMS(CALL)                                              \
-  constexpr int kR = 16 / kVec<T>;                                  \
-  if (vecs <= 2) CALL(2, 1, 1);                                     \
-  if (vecs <= 2 * kR) CALL(2, 1, kR);                               \
-  if (vecs <= 4 * kR) CALL(4, 1, kR);                               \
-  if (vecs <= 8 * kR) CALL(8, 1, kR);                               \
-  if (vecs <= 16 * kR) CALL(16, 1, kR);                             \
-  if (vecs <= 32 * kR) CALL(32, 1, kR);                             \
-  if (vecs <= 64 * kR) CALL(64, 1, kR);                             \
-  if constexpr (sizeof(T) == 2 && Even) {                           \
-    if (vecs <= 128 * kR) CALL(64, 1, 2 * kR);                      \
-    if (vecs <= 256 * kR) CALL(64, 2, 2 * kR);                      \
-    if (vecs <= 512 * kR) CALL(64, 4, 2 * kR);                      \
-    CALL(64, 8, 2 * kR);                                            \
-  } else {                                                          \
-    if (vecs <= 128 * kR) CALL(64, 2, kR);                          \
-    if (vecs <= 256 * kR) CALL(64, 4, kR);                          \
-    if (vecs <= 512 * kR) CALL(64, 8, kR);                          \
-    CALL(64, 16, kR);                                               \
+// The kernel for rows of K codes: CALL(TL, W, R).  Three vectors a lane between
+// the powers of two (672K rows of 192 in bf16: 73 us forward, with lanes half idle
+// 99; 512K of 257 floats 151 and 161), in 16 bits from LEAST lanes on: a backward's
+// stores of a narrower team are parts of lines (1M rows of 48: 56 us, and 43
+// with two vectors).
+#define GS_TEAMS(CALL, LEAST)                                               \
+  constexpr int kR = 16 / kVec<T>;                                          \
+  constexpr int kA = sizeof(T) == 2 ? kR : 3, kB = sizeof(T) == 2 ? 3 : kR; \
+  if (vecs <= 2) CALL(2, 1, 1);                                             \
+  if (vecs <= 2 * kA) CALL(2, 1, kA);                                       \
+  if (vecs <= 2 * kB && (kB > 3 || 2 >= LEAST)) CALL(2, 1, kB);             \
+  if (vecs <= 4 * kA) CALL(4, 1, kA);                                       \
+  if (vecs <= 4 * kB && (kB > 3 || 4 >= LEAST)) CALL(4, 1, kB);             \
+  if (vecs <= 8 * kA) CALL(8, 1, kA);                                       \
+  if (vecs <= 8 * kB) CALL(8, 1, kB);                                       \
+  if (vecs <= 16 * kA) CALL(16, 1, kA);                                     \
+  if (vecs <= 16 * kB) CALL(16, 1, kB);                                     \
+  if (vecs <= 32 * kA) CALL(32, 1, kA);                                     \
+  if (vecs <= 32 * kB) CALL(32, 1, kB);                                     \
+  if (vecs <= 64 * kA) CALL(64, 1, kA);                                     \
+  if (vecs <= 64 * kB) CALL(64, 1, kB);                                     \
+  if constexpr (sizeof(T) == 2 && Even) {                                   \
+    if (vecs <= 128 * kR) CALL(64, 1, 2 * kR);                              \
+    if (vecs <= 256 * kR) CALL(64, 2, 2 * kR);                              \
+    if (vecs <= 512 * kR) CALL(64, 4, 2 * kR);                              \
+    CALL(64, 8, 2 * kR);                                                    \
+  } else {                                                                  \
+    if (vecs <= 128 * kR) CALL(64, 2, kR);                                  \
+    if (vecs <= 256 * kR) CALL(64, 4, kR);                                  \
+    if (vecs <= 512 * kR) CALL(64, 8, kR);                                  \
+    CALL(64, 16, kR);                                                       \
   }
 
 template <typename T, bool Even>
@@ -669,7 +696,7 @@ int rows_of(const BalanceParams& P, const T* x, float2* stats, const Partials& w
                   (size_t)P.K * (G::kTeams > 1 ? 8 : 4), stream, P, x, stats, w); \
     return check_launch("balance_rows_kernel");                               \
   }
-  GS_TEAMS(GS_ROWS)
+  GS_TEAMS(GS_ROWS, 2)
 #undef GS_ROWS
 }
 
@@ -725,12 +752,12 @@ int gradients_of(const BalanceParams& P, const T* x, const int32_t* counts,
                  const float2* stats, const int4* totals, const float* g_loss,
                  const float* g_mean, T* g, hipStream_t stream) {
   const int vecs = (P.K + kVec<T> - 1) / kVec<T>;
-  // Gradients go past the caches where they are more than the last one holds and
-  // what a store writes of a row is whole lines, or long: 512 MiB of rows of
-  // 1024 floats 188 us so and 201 through the caches, 256 MiB 96 and 87; 1M rows
-  // of 100 floats (128 bytes of a row per store, anywhere in its lines) 276 and
-  // 188, of 32 (half a line) 140 and 81.
-  const bool large = P.rows * P.batch * P.K * (int64_t)sizeof(T) > (int64_t(256) << 20);
+  // Gradients go past the caches, which are left to the logits (forward and
+  // backward of 256 MiB of rows of 1024 floats 146 us so and 184 through the
+  // caches, of 128 MiB 84 and 86; the backward alone, of logits that nothing read
+  // before, 96 and 87), where a store writes whole lines of a row, or many: 1M
+  // rows of 100 floats (128 bytes of a row per store, anywhere in its lines) 276
+  // us so and 188 through the caches, of 32 (half a line) 140 and 81.
   const bool whole = P.K * sizeof(T) % 128 == 0;
 #define GS_BWD(TL, W, R)                                                      \
   {                                                                           \
@@ -744,13 +771,13 @@ int gradients_of(const BalanceParams& P, const T* x, const int32_t* counts,
                     dim3(G::kThreads), 0, stream, P, x, counts, stats,        \
                     totals, g_loss, g_mean, g);                               \
     };                                                                        \
-    if (TL >= 8 && large && (TL >= 32 || whole))                              \
+    if (TL >= 32 || (TL >= 8 && whole))                                       \
       launch(std::integral_constant<bool, (TL >= 8)>{});                      \
     else                                                                      \
       launch(std::false_type{});                                              \
     return check_launch("balance_bwd_kernel");                                \
   }
-  GS_TEAMS(GS_BWD)
+  GS_TEAMS(GS_BWD, 8)
 #undef GS_BWD
 }
 #undef GS_TEAMS

@@ -214,9 +214,15 @@ struct Held {
   template <bool Stream = false>
   __device__ __forceinline__ void load(const T* row, int lane_, int n) {
     lane = lane_;
+    constexpr bool kFix = R <= 8;  // (more vectors: fix_row's registers are not there)
+    const T fill = static_cast<T>(-INFINITY);
+    if constexpr (kFix || Even) {
+      load_row<T, R, Even, Stream>(x, row, lane * V, TL * V, n, fill);
+      fix_row<T, R, Even>(x, lane * V, TL * V, n, fill);
+    } else {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      x[r] = load_part<T, Even, Stream>(row, (r * TL + lane) * V, n, static_cast<T>(-INFINITY));
+      for (int r = 0; r < R; ++r) x[r] = load_part<T, Even, Stream>(row, (r * TL + lane) * V, n, fill);
+    }
   }
   __device__ __forceinline__ int column(int r, int v) const { return (r * TL + lane) * V + v; }
   __device__ __forceinline__ void forget() {
@@ -286,8 +292,12 @@ struct Held {
 
 // ---- rows of at most TL * kVec * R codes: a team of TL lanes per row
 //
-// (64K rows of 1024 in bf16: 33 us with 32 elements a lane, 38 with 16; a
-// million rows of 512 floats: 382 us.)
+// 12 to 32 elements a lane, in steps of a third or a half between the powers of
+// two, where no more than the best code is wanted: what a row costs beside its
+// elements is shared by more of them, and fewer lanes idle.  (64K rows of 1024 in
+// bf16: 33 us with 32 elements a lane, 38 with 16; 1M rows of 104 floats 92 us
+// with 16, 182 with 4; 1M of 130 in bf16 82 with 24, 123 with 16 and half the
+// lanes idle.)
 
 template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
@@ -329,22 +339,22 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
       out.top_log_probs[n * top + j] = e.log_prob(v);
     }
   };
-  if constexpr (TL < 64 && R == 1) {
+  if constexpr (TL < 64 && R * kVec<T> <= 8) {
     // Several codes of a narrow team: every lane sorts its keys, and in each
     // turn the team's best head is taken and its lane goes on to its next.
     if (top > 1) {
       using K = Rank<T>;
-      constexpr int V = kVec<T>;
-      typename K::Key k[V], mine_key = 0;
+      constexpr int V = kVec<T>, E = R * V;
+      typename K::Key k[E], mine_key = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) k[v] = K::of(x.x[0][v], x.column(0, v));
-      sort_keys<V>(k);
+      for (int v = 0; v < E; ++v) k[v] = K::of(x.x[v / V][v % V], x.column(v / V, v % V));
+      sort_keys<E>(k);
       for (int j = 0; j < top; ++j) {
         const typename K::Key best = K::template best<TL>(k[0]);
         if (k[0] == best) {
 #pragma unroll
-          for (int v = 0; v + 1 < V; ++v) k[v] = k[v + 1];
-          k[V - 1] = 0;
+          for (int v = 0; v + 1 < E; ++v) k[v] = k[v + 1];
+          k[E - 1] = 0;
         }
         if (lane == (j & (TL - 1))) mine_key = best;
         // (as many as the team has lanes are written at once)
@@ -605,7 +615,8 @@ __global__ __launch_bounds__(64) void probs_join_kernel(
 // exponential and a product: p = 2^(t + down), log p = (t + down) ln 2 with t from
 // Exponent, and everything that is the same for the row is in two constants.
 // A team of TL lanes per part of a row of TL * kVec * R columns (`parts` of
-// them per row).
+// them per row).  (Two or three vectors a lane: 1M rows of 104 floats 277 us with
+// one, 186 with two; of 96 in bf16 139 and, with three, 97.)
 template <typename T, int TL, int R, bool Even>
 __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
     ProbsParams P, const T* __restrict__ logits,
@@ -627,9 +638,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   const T* row = logits + n * P.stride;
   T* out = g_logits + n * P.K;
   vec_t<T> x[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    x[r] = load_part<T, Even, true>(row, first + (r * TL + lane) * V, P.K, static_cast<T>(-INFINITY));
+  load_row<T, R, Even, true>(x, row, first + lane * V, TL * V, P.K, static_cast<T>(-INFINITY));
   const float2 st = stats[n];
   const bool some = st.y != INFINITY;  // (else p = 0 everywhere)
   const float ge = g_entropy && some ? g_entropy[n] : 0.0f;
@@ -667,6 +676,7 @@ __global__ __launch_bounds__(kThreads) void probs_bwd_kernel(
   // 16 bits of a result: exponents 32 up, so that probabilities that the
   // hardware's exponential flushes are far below the type's smallest step (the
   // exponents' own steps, 4e-6 there, are lost in 16 bits).  32 bits: exp2_full.
+  fix_row<T, R, Even>(x, first + lane * V, TL * V, P.K, static_cast<T>(-INFINITY));
   constexpr float kUp = sizeof(T) == 2 ? 32.0f : 0.0f;
   const Exponent e(st.x, st.y - kUp, P.inv_t * kLog2e);
   const float down = e.shift - kUp;
@@ -757,15 +767,24 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
                   dim3(kThreads), 0, stream, P, x, out);                         \
     return check_launch("probs_rows_kernel");                                    \
   }
-  // With no more than the best code wanted, teams as narrow as 32 elements a
-  // lane of 16 bits allow: what a row costs beside its elements is then shared
-  // by more of them.  More codes are found by a whole wavefront's ballots.
-  if constexpr (sizeof(T) == 2)
-    if (P.top <= 1) {
-      GS_ROWS(2, 1) GS_ROWS(4, 2) GS_ROWS(8, 2) GS_ROWS(16, 2) GS_ROWS(32, 2)
-      GS_ROWS(32, 4) GS_ROWS(64, 4)
+  // (several codes of rows above 128 floats or 256 elements of 16 bits are found by
+  // a whole wavefront's ballots: 524K rows of 256 floats, 8 best, 245 us so and 268 from
+  // teams of 32 lanes' sorted keys)
+  if (P.top <= 1) {
+    GS_ROWS(2, 1)
+    if constexpr (sizeof(T) == 2) {
+      GS_ROWS(2, 3) GS_ROWS(4, 2) GS_ROWS(4, 3) GS_ROWS(8, 2) GS_ROWS(8, 3) GS_ROWS(16, 2)
+      GS_ROWS(16, 3) GS_ROWS(32, 2) GS_ROWS(32, 3) GS_ROWS(32, 4) GS_ROWS(64, 3) GS_ROWS(64, 4)
+    } else {
+      GS_ROWS(2, 2) GS_ROWS(2, 3) GS_ROWS(4, 2) GS_ROWS(4, 3) GS_ROWS(4, 4) GS_ROWS(8, 3) GS_ROWS(8, 4)
+      GS_ROWS(16, 3) GS_ROWS(16, 4) GS_ROWS(32, 3) GS_ROWS(32, 4) GS_ROWS(64, 3) GS_ROWS(64, 4)
     }
-  GS_ROWS(2, 1) GS_ROWS(4, 1) GS_ROWS(8, 1) GS_ROWS(16, 1) GS_ROWS(32, 1)
+  }
+  if constexpr (sizeof(T) == 2) {
+    GS_ROWS(2, 1) GS_ROWS(4, 1) GS_ROWS(8, 1) GS_ROWS(16, 1) GS_ROWS(32, 1)
+  } else {
+    GS_ROWS(2, 1) GS_ROWS(2, 2) GS_ROWS(4, 2) GS_ROWS(8, 2) GS_ROWS(16, 2)
+  }
   GS_ROWS(64, 1) GS_ROWS(64, 2) GS_ROWS(64, 4)
 #undef GS_ROWS
   Split s = split_of(P);
@@ -813,10 +832,14 @@ int backward_of(const ProbsParams& P, const void* logits, const int32_t* top_cod
   if (vecs <= 2) GS_BWD(2, 1)
   if (vecs <= 4) GS_BWD(4, 1)
   if (vecs <= 8) GS_BWD(8, 1)
-  if (vecs <= 16) GS_BWD(16, 1)
-  if (vecs <= 32) GS_BWD(32, 1)
-  if (vecs <= 64) GS_BWD(64, 1)
+  if (vecs <= 16) GS_BWD(8, 2)
+  if (vecs <= 24) GS_BWD(8, 3)
+  if (vecs <= 32) GS_BWD(16, 2)
+  if (vecs <= 48) GS_BWD(16, 3)
+  if (vecs <= 64) GS_BWD(32, 2)
+  if (vecs <= 96) GS_BWD(32, 3)
   if (vecs <= 128) GS_BWD(64, 2)
+  if (vecs <= 192) GS_BWD(64, 3)
   GS_BWD(64, 4)
 #undef GS_BWD
 }

@@ -123,6 +123,11 @@ __device__ __forceinline__ void forget(vec_t<T>& v) {
   }
 }
 
+// A vector's bytes.
+struct Words {
+  uint64_t lo, hi;
+};
+
 // Elements i .. i + kVec - 1 of a row of n, `fill` past its end.  Even: n is a
 // multiple of kVec, and a vector is in the row or past it (otherwise the
 // addresses of a last vector's single elements cost a kernel that loops over
@@ -142,10 +147,77 @@ __device__ __forceinline__ void store_part(T* row, int i, int n, vec_t<T> v) {
     else store_vec(row + i, v);
     return;
   }
-  if (Even) return;
+  if (Even || i >= n) return;
+  // a last vector's elements by the binary digits of their number
+  const int m = n - i;
+  const Words w = __builtin_bit_cast(Words, v);
+  T* to = row + i;
+  uint64_t u = w.lo;
+  if (m * sizeof(T) & 8) {
+    __builtin_memcpy(to, &u, 8);
+    to += 8 / sizeof(T);
+    u = w.hi;
+  }
+  if (m * sizeof(T) & 4) {
+    const uint32_t low = (uint32_t)u;
+    __builtin_memcpy(to, &low, 4);
+    to += 4 / sizeof(T);
+    u >>= 32;
+  }
+  if (sizeof(T) == 2 && (m & 1)) {
+    const uint16_t low = (uint16_t)u;
+    __builtin_memcpy(to, &low, 2);
+  }
+}
+
+// A thread's R vectors of a row of n: those at first, first + step, ...  Where
+// rows are not whole vectors (and not shorter than one), a last vector is read as
+// the row's last kVec elements, one load like the others, and fix_row brings
+// them to their place once they are there.  (1M rows of 101 in bf16, the
+// balance's backward: element by element 157 us, so 118.)
+template <typename T, int R, bool Even, bool Stream>
+__device__ __forceinline__ void load_row(vec_t<T> (&x)[R], const T* row, int first, int step, int n, T fill) {
+  constexpr int V = kVec<T>;
+  if (Even || n < V) {
 #pragma unroll
-  for (int j = 0; j < kVec<T>; ++j)
-    if (i + j < n) row[i + j] = v[j];
+    for (int r = 0; r < R; ++r) x[r] = load_part<T, Even, Stream>(row, first + r * step, n, fill);
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = first + r * step;
+    if (i < n) {
+      const T* from = row + min(i, n - V);
+      x[r] = Stream ? load_vec_stream(from) : load_vec(from);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[r][v] = fill;
+    }
+  }
+}
+template <typename T, int R, bool Even>
+__device__ __forceinline__ void fix_row(vec_t<T> (&x)[R], int first, int step, int n, T fill) {
+  constexpr int V = kVec<T>;
+  if (Even || n < V) return;
+  vec_t<T> fills;
+#pragma unroll
+  for (int v = 0; v < V; ++v) fills[v] = fill;
+  const uint64_t more = __builtin_bit_cast(Words, fills).lo;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = first + r * step, past = i + V - n;  // elements to leave out
+    if (past <= 0 || past >= V) continue;
+    Words w = __builtin_bit_cast(Words, x[r]);
+    int bits = past * (int)sizeof(T) * 8;
+    if (bits >= 64) {
+      w.lo = w.hi;
+      w.hi = more;
+      bits -= 64;
+    }
+    w.lo = (w.lo >> bits) | (w.hi << 1) << (63 - bits);
+    w.hi = (w.hi >> bits) | (more << 1) << (63 - bits);
+    x[r] = __builtin_bit_cast(vec_t<T>, w);
+  }
 }
 
 // Reductions over teams of L consecutive lanes (a power of two up to the
