@@ -183,6 +183,10 @@ struct Columns {
 // kRowsAtOnce splats' codes and list the splats of the workgroup's codes, in
 // order; the rows listed for a code are shared out over the workgroup's teams,
 // four on their way at a time, and the teams' sums are added in their order.
+//
+// Where one code's splats could be too many for a workgroup, blockIdx.z takes
+// `span` splats, leaves its sums in partial[z][K][D], and lookup_scan_join_kernel
+// adds those up in order.
 constexpr int kRowsAtOnce = 2048;
 constexpr int kQuarter = kRowsAtOnce / 4;
 
@@ -190,7 +194,7 @@ template <typename T, int TL, int R, int Q, bool Even>
 __global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
     LookupParams P, const T* __restrict__ grad, const T* __restrict__ codebook,
     const float* __restrict__ scales, T* __restrict__ g_codebook,
-    float* __restrict__ g_scales) {
+    float* __restrict__ g_scales, float* __restrict__ partial, int64_t span) {
   using C = Columns<T, TL, R, Even>;
   constexpr int V = C::V, kTeams = C::kTeams, kAhead = 4;
   __shared__ uint16_t lists[Q][4][kQuarter];
@@ -206,13 +210,14 @@ __global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
   for (int q = 0; q < Q; ++q)
 #pragma unroll
     for (int j = 0; j < R * V; ++j) acc[q][j] = 0.0f;
-  for (int64_t base = 0; base < P.rows; base += kRowsAtOnce) {
+  const int64_t from_row = blockIdx.z * span, to_row = min(from_row + span, P.rows);
+  for (int64_t base = from_row; base < to_row; base += kRowsAtOnce) {
     int mine[kQuarter / 64];
 #pragma unroll
     for (int u = 0; u < kQuarter / 64; ++u) {
       const int64_t n = base + w * kQuarter + u * 64 + lane;
-      mine[u] = n < P.rows ? P.codes.at(n, P.K) : kNoCode;
-      if (dots && first == 0 && n < P.rows && mine[u] < 0) g_scales[n] = nan_for(mine[u]);
+      mine[u] = n < to_row ? P.codes.at(n, P.K) : kNoCode;
+      if (dots && first == 0 && n < to_row && mine[u] < 0) g_scales[n] = nan_for(mine[u]);
     }
     int found[Q];
 #pragma unroll
@@ -302,10 +307,25 @@ __global__ __launch_bounds__(kThreads) void lookup_scan_kernel(
 #pragma unroll
           for (int v = 0; v < V; ++v)
             acc[q][r * V + v] += sums[t][(r * TL + lane) * V + v];
-      C::store(g_codebook + (int64_t)(first + q) * P.D, c0, P.D, acc[q], P.factor);
+      if (partial)
+        C::store_sums(partial + ((int64_t)blockIdx.z * P.K + first + q) * P.D, c0, P.D, acc[q]);
+      else
+        C::store(g_codebook + (int64_t)(first + q) * P.D, c0, P.D, acc[q], P.factor);
     }
     __syncthreads();
   }
+}
+
+// A value of the codebook's gradient per thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void lookup_scan_join_kernel(
+    LookupParams P, const float* __restrict__ partial, int chunks, T* __restrict__ g_codebook) {
+  const int64_t values = (int64_t)P.K * P.D, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= values) return;
+  float a = 0.0f;
+#pragma unroll 16
+  for (int z = 0; z < chunks; ++z) a += partial[z * values + i];
+  g_codebook[i] = static_cast<T>(a * P.factor);
 }
 
 // Keys of the sort (K for splats without a code: after all others), and zeros
@@ -609,16 +629,42 @@ int lanes_of(const LookupParams& P) {
   return tl;
 }
 
-// The one-launch way reads all codes once for each code (or four) of the
-// codebook.  Kernels of both ways, rows of 64 floats: 8192 splats and 256 codes
-// 13 us against 28 sorted, 8192 x 4096 25 against 29, 4096 x 16384 27 against
-// 28, 8192 x 16384 44 against 29, 16384 x 16 43 against 24; the sort's five to
-// six launches cost the host 20 us more.
-bool few(const LookupParams& P) {
-  return P.rows <= 8192 && P.rows * P.K <= (int64_t(1) << 26);
+// Chunks of the splats that the scan takes, or 0: sorted.  The scan reads all codes
+// once for each code (or four) of the codebook.  Kernels of both ways, rows of 64
+// floats: 8192 splats and 256 codes 13 us against 28 sorted, 8192 x 4096 25 against
+// 29, 4096 x 16384 27 against 28, 8192 x 16384 44 against 29, 16384 x 16 43 against
+// 24; the sort's five to six launches cost the host 20 us more.
+// Chunks bound what one code that many splats share takes: where a chunk's splats
+// are all of one code, kMostTurns turns of a workgroup's loads (8192 splats x 700 in
+// bf16, 64 codes, 80% of the splats on eight of them: 144 us of kernels forward and
+// backward as one chunk, 36 in eight).  Their sums cost a uniform choice of codes
+// time: 16 MB of them 20 us.
+// Narrow rows, of which a workgroup takes 256 and more at once, go this way up to 64K
+// splats (kernels forward and backward, 65536 x 3 floats of 64 codes 17 us and 32
+// sorted, 16384 of 512 codes 22 and 36, 32768 x 16 of 512 codes 26 and 32; at 2^25
+// splats x codes 39 to 56 and 30 to 41).
+constexpr int kMostTurns = 64;
+int chunks_of(const LookupParams& P) {
+  const int64_t work = P.rows * P.K;
+  if (P.rows <= 8192 ? work > int64_t(1) << 26
+                     : vecs_of(P) > 4 || P.rows > 65536 || work > int64_t(1) << 24)
+    return 0;
+  // (sums of 8 MB at most)
+  const int64_t limit = std::clamp<int64_t>((int64_t(1) << 21) / ((int64_t)P.K * P.D), 1, 64);
+  const int64_t most = kMostTurns * 4 * (kThreads / lanes_of(P));  // splats of a chunk
+  const int64_t chunks = std::max<int64_t>(1, (P.rows + most - 1) / most);
+  if (P.rows > 8192) {
+    const int64_t wide = std::max(chunks, (P.rows + kRowsAtOnce - 1) / kRowsAtOnce);
+    return wide <= limit ? (int)wide : 0;
+  }
+  // (more than the limit: larger chunks, up to four times, where a workgroup has one
+  // code; else sorted: 4096 splats x 700 in bf16, 80% of them on eight of 8192
+  // codes, 337 us a pass as one chunk and 63 sorted)
+  return chunks <= (P.K >= 4096 ? 1 : 4) * limit ? (int)std::min(chunks, limit) : 0;
 }
 
 struct Layout {
+  int chunks;  // of the one-launch way, or 0: sorted
   RadixPlan sort;
   int piece, span, blocks;
   size_t ctl, buffers, keys, sorted, order, out_key, in, out, total;
@@ -626,7 +672,9 @@ struct Layout {
 
 Layout layout(const LookupParams& P) {
   Layout L{};
-  if (few(P)) return L;
+  L.chunks = chunks_of(P);
+  if (L.chunks > 1) L.total = (size_t)L.chunks * P.K * P.D * 4;
+  if (L.chunks > 0) return L;
   int bits = 1;
   while (bits < 32 && (int64_t(1) << bits) <= P.K) ++bits;
   L.sort = radix_plan(P.rows, 1, 0, bits);
@@ -669,17 +717,19 @@ int forward_of(const LookupParams& P, const void* codebook, const float* scales,
   // Four vectors a thread, with as many chains of loads on their way, where the
   // codebook does not fit an XCD's 4 MB of L2 (a million splats x 128 floats over
   // 16384 codes: 120 us against 133); one where it does (over 4096 codes 82
-  // against 88, 262144 x 48 6.3 against 7.0, 64K x 11 4.2 against 7.8).
+  // against 88, 262144 x 48 6.3 against 7.0, 64K x 11 4.2 against 7.8).  A launch
+  // has fewer than 2^32 threads: outputs of 32 GiB and more take four too.
   const bool missing = (int64_t)P.K * P.D * sizeof(T) > (int64_t(4) << 20) &&
                        vecs >= (int64_t)kThreads * 4 * 1024;
+  const bool four = missing || vecs >= int64_t(1) << 31;
 #define GS_LOOKUP(ROWS, U)                                                      \
   launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, ROWS, U>),           \
                 dim3((unsigned)((vecs + kThreads * U - 1) / (kThreads * U))),   \
                 dim3(kThreads), 0, stream, P, div, book, scales, o)
   const bool rows = P.D % kVec<T> == 0;
-  if (rows && missing) GS_LOOKUP(true, 4);
+  if (rows && four) GS_LOOKUP(true, 4);
   else if (rows) GS_LOOKUP(true, 1);
-  else if (missing) GS_LOOKUP(false, 4);
+  else if (four) GS_LOOKUP(false, 4);
   else GS_LOOKUP(false, 1);
 #undef GS_LOOKUP
   return check_launch("lookup_fwd_kernel");
@@ -704,24 +754,35 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
     g_scales = nullptr;
   }
   if (!g_book) return GSPLAT_OK;
-  if (few(P)) {
+  const Layout L = layout(P);
+  if (L.chunks > 0) {
+    float* partial = L.chunks > 1 ? static_cast<float*>(workspace) : nullptr;
+    const int64_t span = (P.rows + L.chunks - 1) / L.chunks;
     // (four codes a workgroup where that leaves 1024 of them: 1024 splats x 64,
-    // 16384 codes 16 us against 25 with one, 4096 codes 8 against 9)
+    // 16384 codes 16 us against 25 with one, 4096 codes 8 against 9.  Not for the
+    // chunks of wide rows: 80% of 8192 splats x 700 in bf16 on eight of 1024 codes
+    // 175 us a pass with four, 72 with one)
+    const bool four = P.K >= 4096 || (vecs <= 4 && P.K * L.chunks >= 4096);
 #define GS_SCAN_OF(TL, R, Q)                                                      \
     launch_traced("lookup_scan_kernel", (lookup_scan_kernel<T, TL, R, Q, Even>),  \
-                  dim3((unsigned)((P.K + Q - 1) / Q), tiles), dim3(kThreads), 0,  \
-                  stream, P, grad, book, scales, g_book, g_scales)
+                  dim3((unsigned)((P.K + Q - 1) / Q), tiles, (unsigned)L.chunks), \
+                  dim3(kThreads), 0, stream, P, grad, book, scales, g_book,       \
+                  g_scales, partial, span)
 #define GS_SCAN(TL, R)                                                          \
   {                                                                             \
-    if (P.K >= 4096) GS_SCAN_OF(TL, R, 4);                                      \
+    if (four) GS_SCAN_OF(TL, R, 4);                                             \
     else GS_SCAN_OF(TL, R, 1);                                                  \
-    return check_launch("lookup_scan_kernel");                                  \
+    const int rc = check_launch("lookup_scan_kernel");                          \
+    if (rc || !partial) return rc;                                              \
+    launch_traced("lookup_scan_join_kernel", (lookup_scan_join_kernel<T>),      \
+                  dim3((unsigned)(((int64_t)P.K * P.D + kThreads - 1) / kThreads)), \
+                  dim3(kThreads), 0, stream, P, partial, L.chunks, g_book);     \
+    return check_launch("lookup_scan_join_kernel");                             \
   }
     GS_WIDTHS(GS_SCAN)
 #undef GS_SCAN
 #undef GS_SCAN_OF
   }
-  const Layout L = layout(P);
   char* w = static_cast<char*>(workspace);
   auto* keys = reinterpret_cast<uint32_t*>(w + L.keys);
   auto* sorted = reinterpret_cast<uint32_t*>(w + L.sorted);

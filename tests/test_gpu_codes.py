@@ -670,3 +670,15 @@ def test_graph_capture(gpu):
         got = [t.detach().clone() for t in held]
         for a, b in zip(got, step()):
             assert torch.equal(a, b.detach())
+
+
+def test_lookup_of_more_vectors_than_a_launch_has_threads(gpu):
+    """An output of 72 GiB: 2^32 vectors of 16 bytes and more."""
+    N, D = 1 << 29, 72
+    book = torch.randn(64, D, device=gpu).to(BF16)
+    codes = torch.randint(0, 64, (N,), device=gpu, dtype=torch.int32)
+    out = gs.lookup_codes(codes, book)
+    for a in (0, N // 2 - 500, N // 9 * 8 - 500, N - 1000):
+        assert torch.equal(out[a:a + 1000], book[codes[a:a + 1000].long()])
+    del out
+    torch.cuda.empty_cache()

@@ -1,9 +1,10 @@
-"""Rows of logits at the widths where the kernels of code_log_probs and code_balance change: whole
-teams of 2 to 64 lanes with 1 to 4 vectors a lane, one element less and one more, the next whole vector."""
+"""Rows of logits at the widths where the kernels of code_log_probs and code_balance change: whole teams of
+2 to 64 lanes with 1 to 4 vectors a lane, one element less and one more, the next whole vector.  The codebook's
+gradient where its splats are sorted, and where chunks of them are added up."""
 import pytest
 import torch
 
-from test_gpu_codes import BF16, F16, F32, _check_balance, _check_probs, _gen, _logits
+from test_gpu_codes import BF16, F16, F32, _check_balance, _check_lookup, _check_probs, _gen, _logits, _lookup_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,21 @@ def test_widths_of_columns(gpu, dtype, K):
     _check_probs(gpu, x, codes, 1, what=f"K={K} {dtype}", view=columns)
     _check_probs(gpu, x, codes, 3, what=f"K={K} {dtype}", view=columns)
     _check_balance(gpu, x, codes, what=f"K={K} {dtype}", view=columns)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [1, 3, 4, 5, 8, 16, 17, 31, 33, 64])
+def test_lookup_of_many_splats_and_codes(gpu, dtype, D):
+    """Narrow rows above the sizes that are not sorted: runs within and over the teams' pieces."""
+    _check_lookup(gpu, *_lookup_inputs((30011 + D,), 9001, D, dtype, skew=D % 2 == 0, seed=D), what=f"D={D} {dtype}")
+
+
+@pytest.mark.parametrize("D,dtype", [(1, F32), (3, F32), (16, F32), (30, BF16), (32, F16), (64, F32), (130, BF16), (513, F32), (1040, F16)])
+@pytest.mark.parametrize("N", [255, 511, 2047, 2049, 4100, 8192, 8193, 20001, 65536, 65537])
+def test_lookup_of_few_codes(gpu, N, D, dtype):
+    """Splats in chunks whose sums are joined: one code of most splats, of all, chunks without any code."""
+    codes, book, s, grad = _lookup_inputs((min(N, 9000) if D > 32 else N,), 37, D, dtype, skew=True, seed=N)
+    _check_lookup(gpu, codes, book, s, grad, factor=0.5, what=f"N={N} D={D}")
+    _check_lookup(gpu, torch.where(torch.arange(len(codes)) > len(codes) // 3, -torch.ones_like(codes), codes), book, None, grad,
+                  what=f"N={N} D={D} pruned")
+    _check_lookup(gpu, torch.full_like(codes, 36), book, s, grad, what=f"N={N} D={D} one code")
