@@ -8,7 +8,8 @@
 // depend on the run (no atomics: the same inputs give the same bits).
 //
 // Few splats: a workgroup takes one to four codes, reads every splat's code,
-// lists those that name one of its own and adds up their rows (one launch).
+// lists those that name one of its own and adds up their rows (one launch, or two
+// where the splats are taken in chunks: chunks_of below).
 //
 // More splats: they are sorted by code (stable), so that a code's splats are
 // one run of the sorted positions.  A team of lanes adds up `piece` positions,
