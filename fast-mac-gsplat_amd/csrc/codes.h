@@ -4,6 +4,9 @@
 
 #include "gs_internal.h"
 
+#define GS_HD __device__ __forceinline__
+#include "exponent.h"
+
 namespace gs {
 
 // Codebooks and logits are float, __bf16 or _Float16 (GSPLAT_F32 / _BF16 /
@@ -46,28 +49,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-
-// Exponents (x - m) c - l of a row's elements in one fused multiply-add: t(x) =
-// x c - k with k = m c + l rounded, and what the rounding of k took, the same
-// for all the row's elements: the exponent is t + shift.  Rows whose k is past
-// 1e30 (a largest logit near the type's limits, no probabilities at all) are
-// not `plain` and take slow(x), whose shift is 0.
-struct Exponent {
-  float m, l, c, k, shift;
-  bool plain;
-  __device__ __forceinline__ Exponent(float m_, float l_, float c_) : m(m_), l(l_), c(c_) {
-#pragma clang fp contract(off)
-    const float hi = m * c;
-    const float lo = __builtin_fmaf(m, c, -hi);
-    k = hi + l;
-    const float back = k - hi;
-    const float rest = (hi - (k - back)) + (l - back);
-    plain = __builtin_fabsf(k) < 1e30f;
-    shift = plain ? -(lo + rest) : l == l ? 0.0f : l;  // (a NaN row's is NaN)
-  }
-  __device__ __forceinline__ float fast(float x) const { return __builtin_fmaf(x, c, -k); }
-  __device__ __forceinline__ float slow(float x) const { return (x - m) * c - l; }
-};
 
 // 16 bytes of elements, loaded and stored at any multiple of the element size
 // (rows of logits start anywhere; the memory pipeline takes dwordx4 accesses
