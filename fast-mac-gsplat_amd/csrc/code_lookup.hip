@@ -648,9 +648,12 @@ int lanes_of(const LookupParams& P) {
 // splats (kernels forward and backward, 65536 x 3 floats of 64 codes 17 us and 32
 // sorted, 16384 of 512 codes 22 and 36, 32768 x 16 of 512 codes 26 and 32; at 2^25
 // splats x codes 39 to 56 and 30 to 41).
+// Codebooks of 2^26 codes are sorted whatever the splats: four codes a workgroup are
+// as many threads as a launch does not have.
 constexpr int kMostTurns = 64;
 int chunks_of(const LookupParams& P) {
   const int64_t work = P.rows * P.K;
+  if (P.K >= 1 << 26) return 0;
   if (P.rows <= 8192 ? work > int64_t(1) << 26
                      : vecs_of(P) > 4 || P.rows > 65536 || work > int64_t(1) << 24)
     return 0;
@@ -677,6 +680,7 @@ struct Layout {
 
 Layout layout(const LookupParams& P) {
   Layout L{};
+  if (P.rows == 0) return L;  // (zeros)
   L.chunks = chunks_of(P);
   if (L.chunks > 1) L.total = (size_t)L.chunks * P.K * P.D * 4;
   if (L.chunks > 0) return L;
@@ -759,6 +763,16 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
     g_scales = nullptr;
   }
   if (!g_book) return GSPLAT_OK;
+  const int64_t zero_bytes = (int64_t)P.K * P.D * sizeof(T);
+  auto prepare = [&](uint32_t* keys, uint32_t* ctl, int64_t ctl_words) {
+    const int64_t most = std::max(P.rows, zero_bytes / 16) / kThreads + 1;
+    launch_traced("lookup_keys_kernel", lookup_keys_kernel,
+                  dim3((unsigned)std::min<int64_t>(most, 2048)), dim3(kThreads), 0,
+                  stream, P, keys, ctl, ctl_words, reinterpret_cast<char*>(g_book),
+                  zero_bytes);
+    return check_launch("lookup_keys_kernel");
+  };
+  if (P.rows == 0) return prepare(nullptr, nullptr, 0);
   const Layout L = layout(P);
   if (L.chunks > 0) {
     float* partial = L.chunks > 1 ? static_cast<float*>(workspace) : nullptr;
@@ -793,13 +807,7 @@ int backward_of(const LookupParams& P, const void* grad_out, const void* codeboo
   auto* sorted = reinterpret_cast<uint32_t*>(w + L.sorted);
   auto* order = reinterpret_cast<uint32_t*>(w + L.order);
   const RadixCtl C = radix_ctl_at(L.sort, w + L.ctl);
-  const int64_t zero_bytes = (int64_t)P.K * P.D * sizeof(T);
-  const int64_t most = std::max(P.rows, zero_bytes / 16) / kThreads + 1;
-  launch_traced("lookup_keys_kernel", lookup_keys_kernel,
-                dim3((unsigned)std::min<int64_t>(most, 2048)), dim3(kThreads), 0,
-                stream, P, keys, C.ghist, (int64_t)radix_ctl_bytes(L.sort) / 4,
-                reinterpret_cast<char*>(g_book), zero_bytes);
-  int rc = check_launch("lookup_keys_kernel");
+  int rc = prepare(keys, C.ghist, (int64_t)radix_ctl_bytes(L.sort) / 4);
   if (!rc) rc = radix_global_hist(L.sort, C, keys, nullptr, stream);
   if (!rc)
     rc = radix_passes(L.sort, C, w + L.buffers, keys, nullptr, nullptr, sorted,

@@ -41,3 +41,23 @@ def test_scales_alone_of_many_splats(gpu):
     for a, b in _slices(N, 1 << 26):
         want = R.lookup(codes[a:b].cpu(), book.cpu(), scales[a:b].detach().cpu(), 1.5, grad[a:b].cpu())
         R.check(got[a:b], want["g_scales"], f"rows from {a}")
+
+
+@pytest.mark.parametrize("N", [0, 1, 3001])
+def test_lookup_of_few_splats_in_a_huge_codebook(gpu, N):
+    """Every row of the codebook's gradient is written, however few splats there are."""
+    K = (1 << 26) + 5
+    _room(3)
+    book = torch.ones(K, 1, device=gpu, requires_grad=True)
+    codes = torch.randint(0, K - 2, (N,), generator=torch.Generator().manual_seed(N)).to(gpu)
+    if N:
+        codes[0] = K - 2
+        codes[N // 2] = K - 2
+    junk = torch.full((K, 1), 7.0, device=gpu)  # (what the gradient's memory may hold)
+    del junk
+    out = gs.lookup_codes(codes, book, None, 3.0)
+    g, = torch.autograd.grad(out, book, torch.full((N, 1), 2.0, device=gpu))
+    assert out.shape == (N, 1) and bool((out == 3.0).all())
+    where, counts = codes.unique(return_counts=True)
+    assert torch.equal(g[where, 0], 6.0 * counts)
+    assert int(g.count_nonzero()) == where.numel()
