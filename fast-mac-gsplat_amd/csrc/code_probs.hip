@@ -180,7 +180,20 @@ struct ProbsOut {
   float* top_log_probs;
   int32_t* top_codes;
   float2* stats;
+  // Those of rows n on.
+  ProbsOut from(int64_t n, int top) const {
+    return ProbsOut{log_probs ? log_probs + n : nullptr, entropy + n,
+                    top_log_probs ? top_log_probs + n * top : nullptr,
+                    top_codes ? top_codes + n * top : nullptr, stats ? stats + n : nullptr};
+  }
 };
+
+// The call's rows first .. first + rows - 1.
+ProbsParams rows_of(ProbsParams P, int64_t first, int64_t rows) {
+  P.rows = rows;
+  P.codes = P.codes.from(first);
+  return P;
+}
 
 // What a row's statistics say about one of its logits.
 struct RowEnd {
@@ -762,10 +775,14 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
   const int vecs = (P.K + V - 1) / V;
 #define GS_ROWS(TL, R)                                                           \
   if (vecs <= TL * R) {                                                          \
-    launch_traced("probs_rows_kernel", (probs_rows_kernel<T, TL, R, Even>),            \
-                  dim3((unsigned)((P.rows + kThreads / TL - 1) / (kThreads / TL))), \
-                  dim3(kThreads), 0, stream, P, x, out);                         \
-    return check_launch("probs_rows_kernel");                                    \
+    constexpr int kTeams = kThreads / TL;                                        \
+    return in_launches(P.rows, kMostBlocks * kTeams, [&](int64_t n, int64_t rows) { \
+      launch_traced("probs_rows_kernel", (probs_rows_kernel<T, TL, R, Even>),    \
+                    dim3((unsigned)((rows + kTeams - 1) / kTeams)),              \
+                    dim3(kThreads), 0, stream, rows_of(P, n, rows),              \
+                    x + n * P.stride, out.from(n, P.top));                       \
+      return check_launch("probs_rows_kernel");                                  \
+    });                                                                          \
   }
   // (several codes of rows above 128 floats or 256 elements of 16 bits are found by
   // a whole wavefront's ballots: 524K rows of 256 floats, 8 best, 245 us so and 268 from
@@ -794,21 +811,26 @@ int forward_of(const ProbsParams& P, const void* logits, const ProbsOut& out,
         static_cast<char*>(workspace) +
         align_up((size_t)P.rows * s.parts * sizeof(Part), 256));
   }
-  const dim3 grid((unsigned)(P.rows * s.parts));
   const int len = (s.length + V - 1) / V;
-#define GS_PARTS(W, R)                                                         \
-  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, W, R, Even>), grid,     \
-                dim3(64 * W), 0, stream, P, x, out, s)
   constexpr int kR = 16 / V;  // vectors of 16 elements
-  if (len <= 256 * kR) GS_PARTS(4, kR);
-  else if (len <= 512 * kR) GS_PARTS(4, 2 * kR);
-  else GS_PARTS(4, 4 * kR);
+  // (launches of one after another use the same workspace)
+  return in_launches(P.rows, kMostBlocks / s.parts, [&](int64_t n, int64_t rows) {
+    const ProbsParams Q = rows_of(P, n, rows);
+    const T* from = x + n * P.stride;
+    const ProbsOut to = out.from(n, P.top);
+#define GS_PARTS(W, R)                                                         \
+  launch_traced("probs_parts_kernel", (probs_parts_kernel<T, W, R, Even>),     \
+                dim3((unsigned)(rows * s.parts)), dim3(64 * W), 0, stream, Q, from, to, s)
+    if (len <= 256 * kR) GS_PARTS(4, kR);
+    else if (len <= 512 * kR) GS_PARTS(4, 2 * kR);
+    else GS_PARTS(4, 4 * kR);
 #undef GS_PARTS
-  const int rc = check_launch("probs_parts_kernel");
-  if (rc || s.parts == 1) return rc;
-  launch_traced("probs_join_kernel", (probs_join_kernel<T>), dim3((unsigned)P.rows),
-                dim3(64), 0, stream, P, x, out, s);
-  return check_launch("probs_join_kernel");
+    const int rc = check_launch("probs_parts_kernel");
+    if (rc || s.parts == 1) return rc;
+    launch_traced("probs_join_kernel", (probs_join_kernel<T>), dim3((unsigned)rows),
+                  dim3(64), 0, stream, Q, from, to, s);
+    return check_launch("probs_join_kernel");
+  });
 }
 
 template <typename T, bool Even>

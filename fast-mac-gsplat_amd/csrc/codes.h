@@ -29,7 +29,23 @@ struct Codes {
     if (c >= 0 && c < K) return (int)c;
     return c == -1 ? kNoCode : kBadCode;
   }
+  // Those of rows n on.
+  Codes from(int64_t n) const {
+    return Codes{p ? static_cast<const char*>(p) + n * (wide ? 8 : 4) : nullptr, wide};
+  }
 };
+
+// A launch has fewer than 2^32 threads: rows go in as many launches as that
+// takes, `most` rows each.  launch(first, rows) returns a status.
+template <typename Launch>
+int in_launches(int64_t rows, int64_t most, Launch launch) {
+  for (int64_t first = 0; first < rows; first += most) {
+    const int rc = launch(first, rows - first < most ? rows - first : most);
+    if (rc) return rc;
+  }
+  return GSPLAT_OK;
+}
+constexpr int64_t kMostBlocks = (1 << 24) - 1;  // of 256 threads
 
 // 2^t with denormal results kept (the hardware's base-2 exponential flushes
 // them): gradients go down to the type's smallest values.

@@ -61,3 +61,36 @@ def test_lookup_of_few_splats_in_a_huge_codebook(gpu, N):
     where, counts = codes.unique(return_counts=True)
     assert torch.equal(g[where, 0], 6.0 * counts)
     assert int(g.count_nonzero()) == where.numel()
+
+
+def _rows_check(gpu, N, K, launch, top, train):
+    x = torch.empty(N, K, device=gpu, dtype=BF16)
+    for a in range(0, N, 1 << 24):
+        x[a:a + (1 << 24)].normal_()
+    codes = torch.randint(-1, K, (N,), device=gpu, dtype=torch.int32)
+    x.requires_grad_(train)
+    o = gs.code_log_probs(x, codes, top=top)
+    ones = torch.ones(N, device=gpu) if train else None
+    g = torch.autograd.grad([o.log_probs, o.entropy], x, [ones, ones])[0] if train else None
+    for a, b in _slices(N, launch):
+        one = torch.ones(b - a)
+        want = R.probs(x[a:b].detach().cpu(), codes[a:b].cpu(), top, 1.0, one if train else None, one if train else None)
+        R.check(o.log_probs[a:b], want["log_probs"], f"log_probs from {a}")
+        R.check(o.entropy[a:b], want["entropy"], f"entropy from {a}")
+        if top:
+            R.check(o.top_codes[a:b], want["top_codes"], f"top_codes from {a}")
+            R.check(o.top_log_probs[a:b], want["top_log_probs"], f"top_log_probs from {a}")
+        if train:
+            R.check(g[a:b], want["g_logits"], f"g_logits from {a}")
+
+
+def test_probs_of_more_rows_than_a_launch_has_wavefronts(gpu):
+    """A wavefront a row: 2^26 rows and more."""
+    _room(40)
+    _rows_check(gpu, (1 << 26) + 1001, 257, 1 << 26, 2, False)
+
+
+def test_probs_of_more_rows_than_a_launch_has_workgroups(gpu):
+    """A workgroup a row: 2^24 rows and more."""
+    _room(75)
+    _rows_check(gpu, (1 << 24) + 1001, 2056, 1 << 24, 1, False)
