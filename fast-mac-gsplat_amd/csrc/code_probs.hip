@@ -844,12 +844,17 @@ int backward_of(const ProbsParams& P, const void* logits, const int32_t* top_cod
 #define GS_BWD(TL, R)                                                          \
   {                                                                            \
     const int parts = (vecs + TL * R - 1) / (TL * R);                          \
-    const int64_t teams = P.rows * parts, per = kThreads / TL;                 \
-    launch_traced("probs_bwd_kernel", (probs_bwd_kernel<T, TL, R, Even>),            \
-                  dim3((unsigned)((teams + per - 1) / per)), dim3(kThreads), 0, \
-                  stream, P, x, top_codes, stats, entropy, g_log_probs,        \
-                  g_entropy, g_top, g, parts);                                 \
-    return check_launch("probs_bwd_kernel");                                   \
+    constexpr int kTeams = kThreads / TL;                                      \
+    return in_launches(P.rows, kMostBlocks * kTeams / parts, [&](int64_t n, int64_t rows) { \
+      auto from = [&](const float* q, int per) { return q ? q + n * per : nullptr; }; \
+      launch_traced("probs_bwd_kernel", (probs_bwd_kernel<T, TL, R, Even>),    \
+                    dim3((unsigned)((rows * parts + kTeams - 1) / kTeams)),    \
+                    dim3(kThreads), 0, stream, rows_of(P, n, rows),            \
+                    x + n * P.stride, top_codes ? top_codes + n * P.top : nullptr, \
+                    stats + n, entropy + n, from(g_log_probs, 1),              \
+                    from(g_entropy, 1), from(g_top, P.top), g + n * P.K, parts); \
+      return check_launch("probs_bwd_kernel");                                 \
+    });                                                                        \
   }
   if (vecs <= 2) GS_BWD(2, 1)
   if (vecs <= 4) GS_BWD(4, 1)

@@ -94,3 +94,9 @@ def test_probs_of_more_rows_than_a_launch_has_workgroups(gpu):
     """A workgroup a row: 2^24 rows and more."""
     _room(75)
     _rows_check(gpu, (1 << 24) + 1001, 2056, 1 << 24, 1, False)
+
+
+def test_probs_gradient_of_more_rows_than_a_launch_has_teams(gpu):
+    """Eight lanes a row: 2^29 rows and more."""
+    _room(110)
+    _rows_check(gpu, (1 << 29) + 1001, 33, 1 << 29, 0, True)
