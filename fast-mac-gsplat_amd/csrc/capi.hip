@@ -17,6 +17,7 @@ namespace {
 thread_local char g_err[1024] = "";
 // armed launch timing (kTimeForward, kTimeBackward): start, stop
 thread_local hipEvent_t g_timing[2][2] = {{nullptr, nullptr}, {nullptr, nullptr}};
+thread_local bool g_too_large = false;  // a launch since the last check_launch
 }
 
 void set_launch_timing(int which, hipEvent_t start, hipEvent_t stop) {
@@ -58,7 +59,19 @@ void set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
+bool launch_fits(dim3 grid, dim3 block) {
+  const bool fits = ((uint64_t)grid.x * block.x | (uint64_t)grid.y * block.y |
+                     (uint64_t)grid.z * block.z) >> 32 == 0;
+  if (!fits) g_too_large = true;
+  return fits;
+}
+
 int check_launch(const char* what) {
+  if (g_too_large) {
+    g_too_large = false;
+    set_error("%s: more than 2^32 threads", what);
+    return GSPLAT_ERR_HIP;
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error("%s: %s", what, hipGetErrorString(e));

@@ -727,13 +727,14 @@ int forward_of(const LookupParams& P, const void* codebook, const float* scales,
   // codebook does not fit an XCD's 4 MB of L2 (a million splats x 128 floats over
   // 16384 codes: 120 us against 133); one where it does (over 4096 codes 82
   // against 88, 262144 x 48 6.3 against 7.0, 64K x 11 4.2 against 7.8).  A launch
-  // has fewer than 2^32 threads: outputs of 32 GiB and more take four too.
+  // has fewer than 2^32 threads: outputs of 32 GiB and more take four too (and those
+  // of 256 GiB, which no device holds, are refused by launch_traced).
   const bool missing = (int64_t)P.K * P.D * sizeof(T) > (int64_t(4) << 20) &&
                        vecs >= (int64_t)kThreads * 4 * 1024;
   const bool four = missing || vecs >= int64_t(1) << 31;
 #define GS_LOOKUP(ROWS, U)                                                      \
   launch_traced("lookup_fwd_kernel", (lookup_fwd_kernel<T, ROWS, U>),           \
-                dim3((unsigned)((vecs + kThreads * U - 1) / (kThreads * U))),   \
+                dim3((unsigned)std::min<int64_t>((vecs + kThreads * U - 1) / (kThreads * U), ~0u)), \
                 dim3(kThreads), 0, stream, P, div, book, scales, o)
   const bool rows = P.D % kVec<T> == 0;
   if (rows && four) GS_LOOKUP(true, 4);

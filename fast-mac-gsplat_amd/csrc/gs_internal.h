@@ -447,6 +447,12 @@ void take_launch_timing(int which, hipEvent_t& start, hipEvent_t& stop);
 constexpr int kTraceMax = 1024;  // GSPLAT_TRACE_MAX
 void trace_take(const char* name, hipEvent_t& start, hipEvent_t& stop);
 
+// Whether a launch has fewer than 2^32 threads an axis.  The runtime does not
+// refuse more: it cuts the grid, and what the missing workgroups would have
+// written stays as it was.  Such a launch is left out, and the check_launch
+// that follows fails.
+bool launch_fits(dim3 grid, dim3 block);
+
 // Every kernel launch of the library: with the trace's events when the
 // trace is armed (hipExtLaunchKernelGGL records them at the kernel's own
 // start and end, so they time the kernel alone).  The arguments are
@@ -455,6 +461,7 @@ template <typename... KArgs, typename... Args>
 inline void launch_traced(const char* name, void (*kernel)(KArgs...),
                           dim3 grid, dim3 block, size_t shmem,
                           hipStream_t stream, Args&&... args) {
+  if (!launch_fits(grid, block)) return;
   hipEvent_t t0 = nullptr, t1 = nullptr;
   trace_take(name, t0, t1);
   if (t0 != nullptr)
