@@ -29,9 +29,9 @@ int make(const gsplat_lookup_meta* m, const void* codes, gs::LookupParams& P,
          const char* what) {
   if (m == nullptr) return fail(what, "meta is NULL");
   if (m->rows < 0 || m->rows > (int64_t(1) << 29)) return fail(what, "rows must lie in [0, 2^29]");
-  if (m->num_codes < 1 || m->num_codes > (1 << 28))
+  if (m->num_codes < 1 || m->num_codes > GSPLAT_MAX_CODES)
     return fail(what, "num_codes must lie in [1, 2^28]");
-  if (m->width < 1 || m->width > (1 << 20)) return fail(what, "width must lie in [1, 2^20]");
+  if (m->width < 1 || m->width > GSPLAT_MAX_CODE_WIDTH) return fail(what, "width must lie in [1, 2^20]");
   if (m->stride < m->width || m->stride > (int64_t(1) << 40))
     return fail(what, "stride must be at least width");
   if (!dtype_ok(m->dtype)) return fail(what, "dtype must be GSPLAT_F32, _BF16 or _F16");
@@ -45,7 +45,7 @@ int make(const gsplat_probs_meta* m, const void* codes, gs::ProbsParams& P,
          const char* what) {
   if (m == nullptr) return fail(what, "meta is NULL");
   if (m->rows < 0 || m->rows > 0x7fffffffLL) return fail(what, "rows must lie in [0, 2^31)");
-  if (m->num_codes < 1 || m->num_codes > (1 << 28))
+  if (m->num_codes < 1 || m->num_codes > GSPLAT_MAX_CODES)
     return fail(what, "num_codes must lie in [1, 2^28]");
   if (m->top < 0 || m->top > GSPLAT_MAX_TOP || m->top > m->num_codes)
     return fail(what, "top must lie in [0, min(num_codes, 64)]");
@@ -64,11 +64,11 @@ int make(const gsplat_probs_meta* m, const void* codes, gs::ProbsParams& P,
 int make(const gsplat_balance_meta* m, const void* codes, gs::BalanceParams& P,
          const char* what) {
   if (m == nullptr) return fail(what, "meta is NULL");
-  if (m->batch < 1 || m->batch > 65535) return fail(what, "batch must lie in [1, 65535]");
-  if (m->choices < 1 || m->choices > (1 << 20)) return fail(what, "choices must lie in [1, 2^20]");
+  if (m->batch < 1 || m->batch > GSPLAT_MAX_BALANCE_IMAGES) return fail(what, "batch must lie in [1, 65535]");
+  if (m->choices < 1 || m->choices > GSPLAT_MAX_CHOICES) return fail(what, "choices must lie in [1, 2^20]");
   if (m->rows < 0 || m->rows > 0x7fffffffLL / m->batch / m->choices)
     return fail(what, "batch * rows * choices must lie in [0, 2^31)");
-  if (m->num_codes < 1 || m->num_codes > (1 << 24))
+  if (m->num_codes < 1 || m->num_codes > GSPLAT_MAX_BALANCE_CODES)
     return fail(what, "num_codes must lie in [1, 2^24]");
   if (m->stride < m->num_codes || m->stride > (int64_t(1) << 40))
     return fail(what, "stride must be at least num_codes");

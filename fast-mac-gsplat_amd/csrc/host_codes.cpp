@@ -178,6 +178,8 @@ py::object lookup(py::handle codes, py::handle codebook, py::handle scales, doub
   const Tensor s = scales.is_none() ? Tensor() : THPVariable_Unpack(scales.ptr());
   if (!codes_ok(c) || dtype_of(book) < 0 || book.dim() != 2 || book.numel() == 0)
     return py::none();
+  if (book.size(0) > GSPLAT_MAX_CODES || book.size(1) > GSPLAT_MAX_CODE_WIDTH)
+    return py::none();
   if (c.device() != book.device()) return py::none();
   if (s.defined() && (s.device() != c.device() || s.sizes() != c.sizes())) return py::none();
   const c10::DeviceGuard device(book.device());
@@ -295,7 +297,8 @@ py::object log_probs(py::handle logits, py::handle codes, int64_t top, double te
   const Tensor& x = THPVariable_Unpack(logits.ptr());
   const Tensor c = codes.is_none() ? Tensor() : THPVariable_Unpack(codes.ptr());
   const int64_t nd = x.dim();
-  if (dtype_of(x) < 0 || nd < 1 || x.size(nd - 1) == 0) return py::none();
+  if (dtype_of(x) < 0 || nd < 1 || x.size(nd - 1) == 0 || x.size(nd - 1) > GSPLAT_MAX_CODES)
+    return py::none();
   if (c.defined() && (!codes_ok(c) || c.device() != x.device() ||
                       c.sizes() != x.sizes().slice(0, nd - 1)))
     return py::none();
@@ -395,7 +398,9 @@ py::object balance(py::handle logits, py::handle codes) {
   const int64_t nd = x.dim();
   if (dtype_of(x) < 0 || !codes_ok(c) || (nd != 2 && nd != 3) || x.size(nd - 1) == 0)
     return py::none();
-  if (nd == 3 && (x.size(0) == 0 || x.size(0) > 65535)) return py::none();
+  if (x.size(nd - 1) > GSPLAT_MAX_BALANCE_CODES) return py::none();
+  if (nd == 3 && (x.size(0) == 0 || x.size(0) > GSPLAT_MAX_BALANCE_IMAGES)) return py::none();
+  if (c.dim() == nd && c.size(nd - 1) > GSPLAT_MAX_CHOICES) return py::none();
   if (c.device() != x.device()) return py::none();
   const auto rows = x.sizes().slice(0, nd - 1);
   if (c.sizes() != rows &&

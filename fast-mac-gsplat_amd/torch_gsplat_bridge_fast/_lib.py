@@ -27,6 +27,10 @@ HANDOFF_PAIRS = 128                       # GSPLAT_HANDOFF_PAIRS
 TIME_FORWARD, TIME_BACKWARD = 0, 1        # GSPLAT_TIME_FORWARD / _BACKWARD
 TRACE_MAX = 1024                          # GSPLAT_TRACE_MAX
 MAX_TOP = 64                              # GSPLAT_MAX_TOP
+MAX_CODES, MAX_CODE_WIDTH = 1 << 28, 1 << 20      # GSPLAT_MAX_CODES / _CODE_WIDTH
+MAX_BALANCE_CODES = 1 << 24               # GSPLAT_MAX_BALANCE_CODES
+MAX_BALANCE_IMAGES = 65535                # GSPLAT_MAX_BALANCE_IMAGES
+MAX_CHOICES = 1 << 20                     # GSPLAT_MAX_CHOICES
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GSPLAT_F32 / _BF16 / _F16
 
 _vp = ctypes.c_void_p

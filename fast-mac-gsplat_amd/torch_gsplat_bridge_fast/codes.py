@@ -310,11 +310,19 @@ def _check_dtype(name: str, t: Tensor) -> None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16")
 
 
+def _check_size(what: str, size: int, most: int) -> None:
+    """The C ABI's limits, on sizes that its 32-bit fields have not cut."""
+    if size > most:
+        raise ValueError(f"at most {most} {what} are supported, not {size}")
+
+
 def _check_lookup(codes: Tensor, codebook: Tensor, scales: Optional[Tensor]) -> None:
     _check_codes(codes)
     _check_dtype("codebook", codebook)
     if codebook.ndim != 2 or 0 in codebook.shape:
         raise ValueError("codebook must have shape [K,D] with K and D at least 1")
+    _check_size("codes", codebook.shape[0], _lib.MAX_CODES)
+    _check_size("values per code", codebook.shape[1], _lib.MAX_CODE_WIDTH)
     if scales is not None:
         if scales.dtype != torch.float32:
             raise ValueError("scales must be float32")
@@ -340,6 +348,7 @@ def _check_probs(logits: Tensor, codes: Optional[Tensor], top: int, temperature:
         raise ValueError(f"top must lie in [0, {most}] (at most the number of codes, and {_lib.MAX_TOP})")
     if not (1e-30 <= temperature <= 1e30):
         raise ValueError("temperature must lie in [1e-30, 1e30]")
+    _check_size("codes", logits.shape[-1], _lib.MAX_CODES)
     _check_device(logits=logits, codes=codes)
 
 
@@ -353,6 +362,11 @@ def _check_balance(logits: Tensor, codes: Tensor) -> None:
         raise ValueError("codes must have the shape of logits without its last axis, or with choices per splat in its place")
     if logits.ndim == 3 and logits.shape[0] == 0:
         raise ValueError("at least one image is required (B >= 1)")
+    _check_size("codes", logits.shape[-1], _lib.MAX_BALANCE_CODES)
+    if logits.ndim == 3:
+        _check_size("images", logits.shape[0], _lib.MAX_BALANCE_IMAGES)
+    if codes.ndim == logits.ndim:
+        _check_size("choices per splat", codes.shape[-1], _lib.MAX_CHOICES)
     _check_device(logits=logits, codes=codes)
 
 

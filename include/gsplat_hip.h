@@ -654,6 +654,14 @@ int gsplat_hip_tile_render(const gsplat_raster_meta* meta,
 #define GSPLAT_BF16 1
 #define GSPLAT_F16 2
 
+/* The largest sizes that the calls below take. */
+#define GSPLAT_MAX_CODES (1 << 28)         /* num_codes */
+#define GSPLAT_MAX_CODE_WIDTH (1 << 20)    /* width */
+#define GSPLAT_MAX_TOP 64                  /* top */
+#define GSPLAT_MAX_BALANCE_CODES (1 << 24) /* num_codes of the balance */
+#define GSPLAT_MAX_BALANCE_IMAGES 65535    /* batch */
+#define GSPLAT_MAX_CHOICES (1 << 20)       /* choices */
+
 /* Codes are int32 or int64 (code_bytes 4 or 8).  -1: the splat has no code.
  * Any other value outside [0, num_codes) is a mistake: nothing is read or
  * counted for it, and the outputs that depend on it are NaN. */
@@ -705,7 +713,6 @@ typedef struct gsplat_probs_meta {
   int32_t code_bytes;
   float temperature; /* T > 0 */
 } gsplat_probs_meta;
-#define GSPLAT_MAX_TOP 64
 
 size_t gsplat_hip_code_probs_workspace_bytes(const gsplat_probs_meta* meta);
 int gsplat_hip_code_probs_forward(const gsplat_probs_meta* meta,
@@ -736,7 +743,7 @@ typedef struct gsplat_balance_meta {
   int64_t rows;      /* per image; batch * rows * choices < 2^31 */
   int32_t batch;     /* 1 .. 65535 */
   int32_t num_codes; /* 1 .. 2^24 */
-  int32_t choices;   /* codes per row, >= 1 */
+  int32_t choices;   /* codes per row, 1 .. 2^20 */
   int32_t dtype;
   int64_t stride;
   int32_t code_bytes;

@@ -100,3 +100,16 @@ def test_probs_gradient_of_more_rows_than_a_launch_has_teams(gpu):
     """Eight lanes a row: 2^29 rows and more."""
     _room(110)
     _rows_check(gpu, (1 << 29) + 1001, 33, 1 << 29, 0, True)
+
+
+def test_sizes_past_32_bits_are_refused(gpu):
+    """On the host path too: one value broadcast to more than 2^32."""
+    past = (1 << 32) + 7
+    one, code = torch.zeros(1, 1, device=gpu, dtype=BF16), torch.zeros(1, device=gpu, dtype=torch.int32)
+    for f in (lambda x: gs.lookup_codes(code, x.expand(past, 1)), lambda x: gs.lookup_codes(code, x.expand(1, past)),
+              lambda x: gs.code_log_probs(x.expand(1, past), code), lambda x: gs.code_balance(x.expand(1, past), code),
+              lambda x: gs.code_balance(x[None].expand(past, 1, 1), code[None].expand(past, 1)),
+              lambda x: gs.code_balance(x, code[None].expand(1, past))):
+        for train in (False, True):
+            with pytest.raises(ValueError, match=r"are supported, not 4294967303"):
+                f(one.clone().requires_grad_(train))
