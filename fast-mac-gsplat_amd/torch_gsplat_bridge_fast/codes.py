@@ -103,6 +103,8 @@ def _(codes, codebook, scales, factor):
 @torch.library.custom_op(f"{_NS}::lookup_codes_backward", mutates_args=())
 def _lookup_backward(grad: Tensor, codes: Tensor, codebook: Tensor, scales: Optional[Tensor], factor: float,
                      need_codebook: bool, need_scales: bool) -> Tuple[Tensor, Tensor]:
+    _check_lookup(codes, codebook, scales)
+    _check_given("grad", grad, (*codes.shape, codebook.shape[1]), codebook.dtype, codes)
     book, c, g = _rows_of(codebook), codes.contiguous(), grad.contiguous()
     s = None if scales is None else scales.contiguous()
     meta = _lookup_meta(c, book, factor)
@@ -182,8 +184,17 @@ def _(logits, codes, top, temperature):
 def _probs_backward(g_log_probs: Optional[Tensor], g_entropy: Optional[Tensor], g_top: Optional[Tensor], logits: Tensor,
                     codes: Optional[Tensor], top_codes: Tensor, stats: Tensor, entropy: Tensor, temperature: float
                     ) -> Tensor:
+    shape, f32 = tuple(logits.shape[:-1]), torch.float32
+    _check_probs(logits, codes, top_codes.shape[-1] if top_codes.ndim else 0, temperature)
+    many = (*shape, top_codes.shape[-1] if top_codes.ndim else 0)
+    for name, t, given, dtype in (("g_log_probs", g_log_probs if codes is not None else None, shape, f32),
+                                  ("g_entropy", g_entropy, shape, f32), ("g_top", g_top, many, f32),
+                                  ("top_codes", top_codes, many, torch.int32), ("stats", stats, (*shape, 2), f32),
+                                  ("entropy", entropy, shape, f32)):
+        _check_given(name, t, given, dtype, logits)
     flat = _rows_of(logits)
     c = None if codes is None else codes.contiguous()
+    top_codes, stats, entropy = top_codes.contiguous(), stats.contiguous(), entropy.contiguous()
     g = [None if t is None else t.contiguous() for t in (g_log_probs if c is not None else None, g_entropy, g_top)]
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     top = top_codes.shape[-1]
@@ -258,8 +269,18 @@ def _(logits, codes):
 @torch.library.custom_op(f"{_NS}::code_balance_backward", mutates_args=())
 def _balance_backward(g_loss: Optional[Tensor], g_mean: Optional[Tensor], logits: Tensor, counts: Tensor, stats: Tensor,
                       totals: Tensor) -> Tensor:
+    _check_logits(logits)
+    _check_images(logits)
+    batch, K, f32 = tuple(logits.shape[:-2]), logits.shape[-1], torch.float32
+    for name, t, given, dtype in (("g_loss", g_loss, batch, f32), ("g_mean", g_mean, (*batch, K), f32),
+                                  ("counts", counts, (*batch, K), torch.int32),
+                                  ("stats", stats, (*logits.shape[:-1], 2), f32),
+                                  ("totals", totals, (batch[0] if batch else 1, 4), torch.int32)):
+        _check_given(name, t, given, dtype, logits)
+    _check_device(logits=logits)
     flat = _rows_of(logits)
     g = [None if t is None else t.contiguous() for t in (g_loss, g_mean)]
+    counts, stats, totals = counts.contiguous(), stats.contiguous(), totals.contiguous()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     with torch.cuda.device(flat.device), _timed("code_balance_backward"):
         check(_lib.lib().gsplat_hip_code_balance_backward(
@@ -316,6 +337,18 @@ def _check_size(what: str, size: int, most: int) -> None:
         raise ValueError(f"at most {most} {what} are supported, not {size}")
 
 
+def _check_given(name: str, t: Optional[Tensor], shape: Tuple[int, ...], dtype: torch.dtype, like: Tensor) -> None:
+    """A backward operator's input, as its forward made it or as autograd passes it."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {str(dtype)[6:]}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {list(shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on the other inputs' device")
+
+
 def _check_lookup(codes: Tensor, codebook: Tensor, scales: Optional[Tensor]) -> None:
     _check_codes(codes)
     _check_dtype("codebook", codebook)
@@ -352,19 +385,23 @@ def _check_probs(logits: Tensor, codes: Optional[Tensor], top: int, temperature:
     _check_device(logits=logits, codes=codes)
 
 
-def _check_balance(logits: Tensor, codes: Tensor) -> None:
-    _check_logits(logits)
-    _check_codes(codes)
+def _check_images(logits: Tensor) -> None:
     if logits.ndim not in (2, 3):
         raise ValueError("logits must have shape [G,K] or [B,G,K]")
-    if codes.shape != logits.shape[:-1] and (codes.ndim != logits.ndim or codes.shape[:-1] != logits.shape[:-1]
-                                             or codes.shape[-1] == 0):
-        raise ValueError("codes must have the shape of logits without its last axis, or with choices per splat in its place")
     if logits.ndim == 3 and logits.shape[0] == 0:
         raise ValueError("at least one image is required (B >= 1)")
     _check_size("codes", logits.shape[-1], _lib.MAX_BALANCE_CODES)
     if logits.ndim == 3:
         _check_size("images", logits.shape[0], _lib.MAX_BALANCE_IMAGES)
+
+
+def _check_balance(logits: Tensor, codes: Tensor) -> None:
+    _check_logits(logits)
+    _check_codes(codes)
+    _check_images(logits)
+    if codes.shape != logits.shape[:-1] and (codes.ndim != logits.ndim or codes.shape[:-1] != logits.shape[:-1]
+                                             or codes.shape[-1] == 0):
+        raise ValueError("codes must have the shape of logits without its last axis, or with choices per splat in its place")
     if codes.ndim == logits.ndim:
         _check_size("choices per splat", codes.shape[-1], _lib.MAX_CHOICES)
     _check_device(logits=logits, codes=codes)
