@@ -75,7 +75,8 @@ def train(steps=300, splats=4096, codes=64, size=256, rate=1e-4, even=1e-4, temp
             print(f"step {step:4d}  mse {float(mse.detach()):.5f}  bits per splat {float(cost.detach()):.2f}  "
                   f"codes in use {int(history['used'][-1])} of {codes}", flush=True)
     history = {k: torch.stack(v).float().cpu() for k, v in history.items()}
-    return history, {"codebook": book.detach(), "codes": chosen.to(torch.int16), "gains": gains.detach()}
+    small = torch.int16 if codes <= 1 << 15 else torch.int32  # (lookup_codes takes int32 and int64)
+    return history, {"codebook": book.detach(), "codes": chosen.to(small), "gains": gains.detach()}
 
 
 if __name__ == "__main__":
