@@ -277,12 +277,15 @@ struct Probs : torch::autograd::Function<Probs> {
       return out;
     const c10::DeviceGuard device(x.device());
     out[0] = at::empty(x.sizes(), plain_options(x));
+    // (saved-tensor hooks may give back another layout)
+    const Tensor best = top > 0 ? saved[2].contiguous() : Tensor();
+    const Tensor stats = saved[3].contiguous(), entropy = saved[4].contiguous();
     const auto meta = probs_meta(x, stride, c, top, ctx->saved_data["T"].toDouble());
     {
       const Timed timed("code_log_probs_backward");
       check(api.code_probs_backward(&meta, x.data_ptr(), pointer(c),
-                                    top > 0 ? i32(saved[2]) : nullptr, f32(saved[3]),
-                                    f32(saved[4]), f32_or_null(gl), f32_or_null(ge),
+                                    top > 0 ? i32(best) : nullptr, f32(stats),
+                                    f32(entropy), f32_or_null(gl), f32_or_null(ge),
                                     f32_or_null(gt), out[0].data_ptr(), stream_of(x)),
             "gsplat_hip_code_probs_backward");
     }
@@ -379,11 +382,13 @@ struct Balance : torch::autograd::Function<Balance> {
     const Tensor gm = grads[2].defined() ? grads[2].contiguous() : grads[2];
     const c10::DeviceGuard device(x.device());
     out[0] = at::empty(x.sizes(), plain_options(x));
+    const Tensor counts = saved[1].contiguous(), stats = saved[2].contiguous();
+    const Tensor totals = saved[3].contiguous();
     const auto meta = balance_meta(x, stride, 1, 4);
     {
       const Timed timed("code_balance_backward");
-      check(api.code_balance_backward(&meta, x.data_ptr(), i32(saved[1]), f32(saved[2]),
-                                      i32(saved[3]), f32_or_null(gl), f32_or_null(gm),
+      check(api.code_balance_backward(&meta, x.data_ptr(), i32(counts), f32(stats),
+                                      i32(totals), f32_or_null(gl), f32_or_null(gm),
                                       out[0].data_ptr(), stream_of(x)),
             "gsplat_hip_code_balance_backward");
     }
