@@ -30,6 +30,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream_of
@@ -331,6 +332,15 @@ def _check_dtype(name: str, t: Tensor) -> None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16")
 
 
+def _check_reverse(*tensors: Optional[Tensor]) -> None:
+    """The operators have no forward derivative; torch would leave a dual input's tangent out."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("scenes in codes have gradients in reverse mode only, not in forward mode")
+
+
 def _check_size(what: str, size: int, most: int) -> None:
     """The C ABI's limits, on sizes that its 32-bit fields have not cut."""
     if size > most:
@@ -419,6 +429,7 @@ def lookup_codes(codes: Tensor, codebook: Tensor, scales: Optional[Tensor] = Non
     out = _lib.host().lookup_codes(codes, codebook, scales, factor)
     if out is not None:
         return out
+    _check_reverse(codebook, scales)
     _check_lookup(codes, codebook, scales)
     return _lookup(codes, codebook, scales, float(factor))
 
@@ -434,6 +445,7 @@ def code_log_probs(logits: Tensor, codes: Optional[Tensor] = None, top: int = 0,
     out = _lib.host().code_log_probs(logits, codes, top, temperature)
     if out is not None:
         return CodeLogProbs(*out)
+    _check_reverse(logits)
     _check_probs(logits, codes, top, temperature)
     log_probs, entropy, top_log_probs, top_codes, _ = _probs(logits, codes, int(top), float(temperature))
     return CodeLogProbs(None if codes is None else log_probs, entropy, top_log_probs if top else None,
@@ -451,6 +463,7 @@ def code_balance(logits: Tensor, codes: Tensor) -> CodeBalance:
     out = _lib.host().code_balance(logits, codes)
     if out is not None:
         return CodeBalance(*out)
+    _check_reverse(logits)
     _check_balance(logits, codes)
     loss, counts, mean_probs, _, _ = _balance(logits, codes)
     return CodeBalance(loss, counts, mean_probs)

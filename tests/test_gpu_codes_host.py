@@ -98,6 +98,34 @@ def test_threads(gpu):
         raise errors[0]
 
 
+def test_forward_mode_is_refused(gpu):
+    """There is no forward derivative: a dual input raises, and no tangent gets lost."""
+    x, codes, book, scales = _inputs(gpu)
+    calls = (lambda x, b, s: gs.code_log_probs(x, codes).entropy, lambda x, b, s: gs.code_balance(x, codes).loss,
+             lambda x, b, s: gs.lookup_codes(codes, b), lambda x, b, s: gs.lookup_codes(codes, book, s))
+    for train in (False, True):
+        ts = [t.detach().clone().requires_grad_(train) for t in (x, book, scales)]
+        for f in calls:
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                with torch.autograd.forward_ad.dual_level():
+                    f(*(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in ts))
+    for f in calls:
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (x, book, scales), tuple(torch.ones_like(t) for t in (x, book, scales)))
+    # a level alone is nothing to refuse
+    with torch.autograd.forward_ad.dual_level():
+        _same(_all(x, codes, book, scales)[1], _grads(gpu)[:-3])
+
+
+def test_functional_gradients_are_refused(gpu):
+    """As the rasterizer's: torch.func's transforms of autograd need what an autograd node in C++ does not have."""
+    x, codes, book, scales = _inputs(gpu)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: gs.code_log_probs(t, codes).entropy.sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: gs.lookup_codes(codes, t).sum())(book)
+
+
 def test_vmap(gpu):
     parts = [_inputs(gpu, s) for s in range(3)]
     x, codes, book, scales = (torch.stack(t) for t in zip(*parts))
