@@ -593,10 +593,6 @@ __global__ __launch_bounds__(kThreads) void balance_long_bwd_kernel(
 
 constexpr int kLongest = 16384;  // codes of a row that a workgroup holds
 
-// Workgroups per image of the row pass.  A workgroup leaves 8 bytes per code,
-// so it takes at least 32 bytes of every column (a quarter of that again); 1024
-// workgroups in all keep the GPU busy (200K rows x 4096 368 us, with 512 476,
-// with 2048 371; four images x 256 54, 60, 59).
 // Teams of a workgroup of the kernel that GS_TEAMS takes.
 int teams_of(const BalanceParams& P) {
   const bool narrow = P.dtype != GSPLAT_F32;
@@ -607,9 +603,20 @@ int teams_of(const BalanceParams& P) {
   return std::max(1, 256 / threads);
 }
 
+// Workgroups per image of the row pass, each of which leaves its columns' sums
+// and counts, 8 bytes per code: 1024 in all keep the GPU busy (200K rows x 4096
+// 368 us, with 512 476, with 2048 371; four images x 256 54, 60, 59).
+// Above 16384 codes, chunks of an image's rows, whose columns are shared out over
+// further workgroups: eight rows at least, so that the sums are an eighth of the
+// logits in 32 bits, a quarter in 16 (forwards of 64 images of 256 rows x 32768 in
+// bf16 1457 us with 143 MB of sums, a chunk a row 3474 with 2156 MB; one of 100 x
+// 100000 79 and 110, of 4096 x 32768 191 and 190).
 int blocks_of(const BalanceParams& P) {
   if (P.rows == 0) return 1;
-  if (P.K > kLongest) return (int)std::min<int64_t>(P.rows, 256);
+  if (P.K > kLongest) {
+    const int64_t most = std::max(1, std::min(256, 1024 / P.batch));
+    return (int)std::clamp<int64_t>(P.rows / 8, 1, most);
+  }
   // two rows for each team, at least: what a workgroup costs at its start and
   // end, and the join its sums, is then worth it (16384 rows of 64 floats: 14 us,
   // 17 with eight rows a workgroup; 1024 of 4096 in bf16 20 and 27)
