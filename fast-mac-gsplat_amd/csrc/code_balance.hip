@@ -15,10 +15,11 @@
 //
 // One launch reads the logits once and leaves each workgroup's column sums and
 // counts, a second joins them; the backward is one pass.  On an MI355X: four
-// images of 64K rows x 256 floats 69 us forward (3.9 TB/s: start and end of the
-// persistent workgroups and the join are a fifth of it) and 90 us backward
-// (6 TB/s); 200K rows x 4096 in bf16 358 us (4.6 TB/s, VALU issue beside HBM)
-// and 635 us (5.2 TB/s).
+// images of 64K rows x 256 floats 50 + 9 us forward (4.6 TB/s: start and end of
+// the persistent workgroups and the join are a fifth of it) and 81 us backward
+// (6.7 TB/s); 200K rows x 4096 in bf16 348 + 16 us (4.6 TB/s, VALU issue beside
+// HBM) and 605 us (5.4 TB/s).  Above 16384 codes both directions read the logits
+// twice: 4096 rows x 32768 floats 141 + 103 + 19 us and 349 us.
 #include <algorithm>
 #include <type_traits>
 

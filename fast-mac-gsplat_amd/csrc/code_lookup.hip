@@ -21,13 +21,15 @@
 //
 // What bounds it, on an MI355X: the forward of a million splats x 128 floats
 // over 16384 codes (8 MB of codebook, twice an XCD's L2) takes 120 us, 4.6 TB/s
-// of codes read and rows written, 6 TB/s with the codebook's misses; the
-// output's stores stream past the caches (165 us without).  Its backward: 45 us
-// of sorting (two passes of 16 us and two of 5 to 8, latency), 130 us of runs
-// (rows in sorted order are gathers of 512 bytes: 4.2 TB/s), 10 us of joining.
-// 262144 splats x 48 values: 9 us forward, and in the backward seven launches
-// of 5 to 19 us, each a chain of dependent loads, beside which the host's
-// launches and torch's autograd call take as long.
+// of codes read and rows written, 7.1 TB/s with the codebook's misses; the
+// output's stores stream past the caches (165 us without).  Its backward: 49 us
+// of sorting (two passes of 17 us, keys and histogram of 6 and 9, latency), 134 us
+// of runs (rows in sorted order are gathers of 512 bytes: 5.4 TB/s), 11 us of
+// joining.  262144 splats x 48 bf16 with scales, most on a few codes: 9 us
+// forward, and in the backward six launches of 3 to 19 us, each a chain of
+// dependent loads.  The gradient of the scales alone is bound by the launch of a
+// wavefront a splat, most of whose lanes idle in narrow rows: a million splats x 3
+// floats 180 us for 21 MB, x 128 floats 228 us for 550 MB.
 #include <algorithm>
 
 #include "codes.h"
@@ -722,7 +724,7 @@ int forward_of(const LookupParams& P, const void* codebook, const float* scales,
   // Four vectors a thread, with as many chains of loads on their way, where the
   // codebook does not fit an XCD's 4 MB of L2 (a million splats x 128 floats over
   // 16384 codes: 120 us against 133); one where it does (over 4096 codes 82
-  // against 88, 262144 x 48 6.3 against 7.0, 64K x 11 4.2 against 7.8).  A launch
+  // against 88, 64K x 11 4.2 against 7.8).  A launch
   // has fewer than 2^32 threads: outputs of 32 GiB and more take four too (and those
   // of 256 GiB, which no device holds, are refused by launch_traced).
   const bool missing = (int64_t)P.K * P.D * sizeof(T) > (int64_t(4) << 20) &&

@@ -18,10 +18,11 @@
 // lanes up to 2048 codes (1024 in 32 bits), a workgroup up to 16384, and parts
 // of 2048 to 16384 codes, joined by a second launch, above (or for few long
 // rows).  What bounds it, on an MI355X: HBM where rows are short (a million
-// rows of 512 floats, best code: 382 us, 5.7 TB/s), VALU issue where 16-bit
-// rows are long (64K rows of 16384: 448 us, 4.8 TB/s, with 12 VALU instructions
-// an element, 85% of the launch's issue cycles).  The backward is bound by HBM
-// at all lengths (64K x 16384: 690 us, 6.2 TB/s; 64K x 1024: 48 us, 5.6 TB/s).
+// rows of 512 floats, best code: 393 us, 5.5 TB/s), VALU issue where 16-bit
+// rows are long (64K rows of 16384, 8 best: 473 us, 4.6 TB/s, with 12 VALU
+// instructions an element) or several best codes are wanted of short ones (a
+// million rows of 64 in bf16, 8 best: 96 us, 2.4 TB/s).  The backward is bound by
+// HBM at all lengths (64K x 16384: 664 us, 6.6 TB/s; 64K x 1024: 47 us, 6.0 TB/s).
 #include <algorithm>
 
 #include "codes.h"
@@ -434,9 +435,9 @@ __global__ __launch_bounds__(kThreads) void probs_rows_kernel(
 
 // ---- longer rows: a workgroup per part of a row
 //
-// (64K rows of 16384 in bf16: 64 elements a thread take 448 us, 512 threads of 32
-// elements 629: reductions and the search for the bound are per wavefront.
-// Five wavefronts per SIMD: with four the same launch takes 559 us.)
+// (64K rows of 16384 in bf16, one build against the other: 64 elements a thread
+// take 448 us, 512 threads of 32 elements 629: reductions and the search for the
+// bound are per wavefront.  Five wavefronts per SIMD: with four 559 us.)
 
 // One part of a row per workgroup.  parts = 1: the row's outputs; else its
 // statistics and best keys go to partials, for probs_join_kernel.

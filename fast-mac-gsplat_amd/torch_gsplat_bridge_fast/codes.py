@@ -425,7 +425,7 @@ def lookup_codes(codes: Tensor, codebook: Tensor, scales: Optional[Tensor] = Non
 
     codes [...] (-1: zeros), codebook [K,D], scales float32 of the codes' shape or None.  The result has
     the codebook's type.  Gradients flow to codebook and scales; a row of the codebook's gradient is the
-    sum over the splats that name it, in their order."""
+    sum over the splats that name it, in an order that does not depend on the run."""
     out = _lib.host().lookup_codes(codes, codebook, scales, factor)
     if out is not None:
         return out

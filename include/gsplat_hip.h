@@ -681,8 +681,8 @@ typedef struct gsplat_lookup_meta {
 int gsplat_hip_lookup_forward(const gsplat_lookup_meta* meta, const void* codes,
                               const void* codebook, const float* scales,
                               void* out, void* stream);
-/* g_codebook (num_codes x width, contiguous; may be NULL): sums by code in
- * ascending splat order, the same bits on every call; every row is written.
+/* g_codebook (num_codes x width, contiguous; may be NULL): sums by code, in an
+ * order that does not depend on the run; every row is written.
  * g_scales (rows floats; may be NULL).  grad_out: rows x width, contiguous.
  * codebook is read only for g_scales.  The workspace (0 bytes for few splats)
  * is needed only for g_codebook.  If the sort's look-back gives up (see
