@@ -201,9 +201,11 @@ struct RowEnd {
   float base, log2_s, inv_t;
   __device__ __forceinline__ RowEnd(Part p, float inv_t_)
       : base(base_of(p.m)), log2_s(p.s == 0.0f ? 0.0f : log2_fast(p.s)), inv_t(inv_t_) {}
-  // (not in base 2: a masked logit of the type's lowest value would overflow)
+  // (not in base 2: a masked logit of the type's lowest value would overflow; the
+  // difference by halves: it may be past the range where it is not over T)
   __device__ __forceinline__ float log_prob(float x) const {
-    return __builtin_fmaf(-kLn2, log2_s, (x - base) * inv_t);
+    const float half = __builtin_fmaf(0.5f, x, -0.5f * base) * inv_t;
+    return __builtin_fmaf(-kLn2, log2_s, half + half);
   }
 };
 

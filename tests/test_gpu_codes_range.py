@@ -85,3 +85,30 @@ def test_balance_far_from_zero(gpu, dtype, K):
     y = torch.stack([_logits((40,), K, dtype, seed=K + b) for b in range(2)])
     y[1, 7] = -1e10
     _check_balance(gpu, y, torch.randint(-1, K, (2, 40), generator=_gen(K)), what=f"K={K} {dtype} one row")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("K", PROBS_KS)
+@pytest.mark.parametrize("T", [2.0, 1e6, 1e30])
+def test_probs_of_rows_that_span_the_range(gpu, dtype, K, T):
+    """Logits at both ends of the type: their difference is past the range, over T it is not."""
+    big = float(torch.finfo(dtype).max)
+    x = torch.randn(6, K, generator=_gen(K)).to(dtype)
+    x[0, ::2], x[0, 1::2] = big, -big
+    x[1, 0] = -big
+    x[2] = -big
+    x[2, K - 1] = big
+    x[3] = torch.linspace(-0.9, 0.9, K).mul(big).to(dtype)
+    x[4, : K // 2] = 0.75 * big
+    x[5, K // 2] = big
+    codes = torch.tensor([1, 0, 0, K // 2, K - 1, K // 2])
+    _check(gpu, x, codes, 3, T, f"K={K} {dtype} T={T}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("K", PROBS_KS)
+@pytest.mark.parametrize("T", [1e-30, 1e3, 1e10, 1e30])
+def test_probs_of_extreme_temperatures(gpu, dtype, K, T):
+    x = _logits((5,), K, dtype, seed=K, masked=0.1)
+    x[1] = 1.5
+    _check(gpu, x, torch.randint(-1, K, (5,), generator=_gen(K)), 3, T, f"K={K} {dtype} T={T}")
