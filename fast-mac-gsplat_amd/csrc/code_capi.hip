@@ -53,9 +53,10 @@ int make(const gsplat_probs_meta* m, const void* codes, gs::ProbsParams& P,
     return fail(what, "stride must be at least num_codes");
   if (!dtype_ok(m->dtype)) return fail(what, "dtype must be GSPLAT_F32, _BF16 or _F16");
   if (m->code_bytes != 4 && m->code_bytes != 8) return fail(what, "code_bytes must be 4 or 8");
+  // (1 / T in base 2, 1.44 times that, has to be finite too)
   const float inv_t = 1.0f / m->temperature;
-  if (!(m->temperature > 0.0f) || !(inv_t > 0.0f) || inv_t > 3.0e38f)
-    return fail(what, "temperature must be positive and finite, its reciprocal too");
+  if (!(m->temperature > 0.0f) || !(inv_t > 0.0f) || inv_t > 2.0e38f)
+    return fail(what, "temperature must be positive and finite, twice its reciprocal too");
   P = gs::ProbsParams{m->rows, m->num_codes, m->top, m->stride, m->dtype, inv_t,
                       gs::Codes{codes, m->code_bytes == 8}};
   return GSPLAT_OK;

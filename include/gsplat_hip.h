@@ -711,7 +711,7 @@ typedef struct gsplat_probs_meta {
   int64_t stride;    /* elements between rows of logits, >= num_codes */
   int32_t dtype;
   int32_t code_bytes;
-  float temperature; /* T > 0 */
+  float temperature; /* T > 0, 2 / T finite */
 } gsplat_probs_meta;
 
 size_t gsplat_hip_code_probs_workspace_bytes(const gsplat_probs_meta* meta);
