@@ -130,14 +130,14 @@ def _shape(case):
     return ((case["B"],) if case["B"] else ()) + (case["G"],)
 
 
-def _sorted(codes, K):
+def _sorted(codes, K, S):
     """(order, places, starts): choices by code, those without one last; where each choice went; where codes begin."""
     flat = codes.reshape(-1).long()
     keys = torch.where(flat >= 0, flat, torch.full_like(flat, K))
     order = torch.sort(keys, stable=True).indices
     places = torch.empty_like(order)
     places[order] = torch.arange(order.numel(), device=order.device)
-    places = torch.where(flat >= 0, places, torch.full_like(places, -1)).reshape(codes.shape)
+    places = torch.where(flat >= 0, places, torch.full_like(places, -1)).reshape(*(codes.shape if S > 1 else (*codes.shape, 1)))
     counts = torch.zeros(K + 1, dtype=torch.int64, device=codes.device)
     counts.scatter_add_(0, keys, torch.ones_like(keys))
     starts = torch.cat([counts.new_zeros(1), counts[:K].cumsum(0)])
@@ -177,7 +177,7 @@ def prepare(case, seed):
     c = torch.where(torch.rand(many, device=dev, generator=gen) < 0.02, torch.full_like(c, -1), c)
     c = c if case["long"] else c.to(torch.int32)
     if case["op"] == "back":
-        s["groups"] = _sorted(c, K)  # (as the way there left it)
+        s["groups"] = _sorted(c, K, S)  # (as the way there left it)
         s["rows"] = normal(c.numel(), D).to(dtype).requires_grad_(train)
         s["weights"] = torch.rand(many, device=dev, generator=gen).requires_grad_(train) if case["weights"] else None
         s["grad"] = normal(*shape, D).to(dtype) if train else None
@@ -208,7 +208,7 @@ def _own(s):
         return {"norm": norm, "out": s["whole"] if out is None else s["whole_out"]}
     with torch.set_grad_enabled(s["train"]):
         if s["op"] == "group":
-            groups = gs.group_codes(s["codes"], s["case"]["K"])
+            groups = gs.group_codes(s["codes"], s["case"]["K"], several=s["case"]["S"] > 1)
             out = gs.rows_by_code(s["rows"], groups)
             r = {"out": out.detach(), "order": groups.order, "places": groups.places, "starts": groups.starts}
             inputs = [s["rows"]]
@@ -238,7 +238,7 @@ def _plain(s):
 
 def _plain_group(s):
     codes, x, S = s["codes"], s["rows"].detach(), s["case"]["S"]
-    order, places, starts = _sorted(codes, s["case"]["K"])
+    order, places, starts = _sorted(codes, s["case"]["K"], S)
     flat = x.reshape(-1, x.shape[-1])
     named = (torch.arange(order.numel(), device=x.device) < starts[-1]).unsqueeze(-1)
     out = torch.where(named, flat[order.long() // S], torch.zeros_like(flat[:1]))
@@ -263,7 +263,7 @@ def _plain_back(s):
         of_rows = (g[order.long() // S, 0] * w.reshape(-1)[order.long()].unsqueeze(-1)).to(y.dtype)
         grads = [of_rows]
         if s["weights"] is not None:
-            grads.append(((g * rows).sum(-1) * (at >= 0)).reshape(places.shape))
+            grads.append(((g * rows).sum(-1) * (at >= 0)).reshape(s["weights"].shape))
         r["grads"] = tuple(grads)
     return r
 
@@ -388,7 +388,7 @@ def exact(case, seed):
             if s["weights"] is not None:
                 g_w = torch.zeros(places.numel(), dtype=f64, device=y.device)
                 g_w[choice] = torch.linalg.vecdot(g, y)
-                grads.append(g_w.reshape(places.shape))
+                grads.append(g_w.reshape(s["weights"].shape))
             r["grads"] = tuple(grads)
         return r
     x, codes = s["rows"].detach().reshape(-1, D), s["codes"].reshape(-1)
