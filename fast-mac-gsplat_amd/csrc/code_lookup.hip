@@ -39,31 +39,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float nan_for(int c) {
-  return c == kBadCode ? __builtin_nanf("") : 0.0f;
-}
-
 // ---- forward
 
 // Each thread writes kUnroll vectors of 16 bytes of the output, taken as one
 // array; block b starts at element b * kThreads * V * kUnroll.  div: the
-// quotient of a 32-bit offset by D (below).
-
-// n / d for n < 2^31 by one 32 x 32 multiplication: floor(n m / 2^(32 + s))
-// with m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1 (exact for n < 2^31: the
-// error n (m d - 2^(32 + s)) / (d 2^(32 + s)) is below 1 / d).
-struct Divide {
-  uint32_t d, m, s;
-  explicit Divide(uint32_t d_) : d(d_), m(0), s(0) {
-    if (d == 1) return;
-    while ((uint64_t(1) << (s + 1)) < d) ++s;
-    m = (uint32_t)(((uint64_t(1) << (32 + s)) + d - 1) / d);
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
-    return d == 1 ? n : __umulhi(n, m) >> s;
-  }
-};
-
+// quotient of a 32-bit offset by D.
 template <typename T, bool Rows, int kUnroll>
 __global__ __launch_bounds__(kThreads) void lookup_fwd_kernel(
     LookupParams P, Divide div, const T* __restrict__ codebook,

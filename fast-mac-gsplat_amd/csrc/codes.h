@@ -1,5 +1,6 @@
 // codes.h -- what the kernels of scenes in codes share (code_lookup.hip,
-// code_probs.hip, code_balance.hip): element types, codes, wavefront sums.
+// code_probs.hip, code_balance.hip, code_groups.hip, code_adapters.hip): element
+// types, codes, wavefront sums.
 #pragma once
 
 #include "gs_internal.h"
@@ -32,6 +33,26 @@ struct Codes {
   // Those of rows n on.
   Codes from(int64_t n) const {
     return Codes{p ? static_cast<const char*>(p) + n * (wide ? 8 : 4) : nullptr, wide};
+  }
+};
+
+// What stands for a code that is none: 0, or NaN.
+__device__ __forceinline__ float nan_for(int c) {
+  return c == kBadCode ? __builtin_nanf("") : 0.0f;
+}
+
+// n / d for n < 2^31 by one 32 x 32 multiplication: floor(n m / 2^(32 + s))
+// with m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1 (exact for n < 2^31: the
+// error n (m d - 2^(32 + s)) / (d 2^(32 + s)) is below 1 / d).
+struct Divide {
+  uint32_t d, m, s;
+  explicit Divide(uint32_t d_) : d(d_), m(0), s(0) {
+    if (d == 1) return;
+    while ((uint64_t(1) << (s + 1)) < d) ++s;
+    m = (uint32_t)(((uint64_t(1) << (32 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    return d == 1 ? n : __umulhi(n, m) >> s;
   }
 };
 
@@ -284,6 +305,59 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   for (int w = 1; w < W; ++w) r += red[w];
   return r;
 }
+
+// ---- code_groups.hip
+// Choices (codes of splats, `choices` in all) sorted by code: order[j] the
+// choice at place j, places[i] the place of choice i (kNoCode, kBadCode for
+// those that have none: they stand last), starts[k] the first place of code k.
+struct GroupParams {
+  int64_t choices;
+  int K;
+  Codes codes;
+};
+size_t group_workspace_bytes(const GroupParams& P);
+int launch_group_codes(const GroupParams& P, int32_t* order, int32_t* places,
+                       int32_t* starts, void* workspace, hipStream_t stream);
+
+// Rows of splats and of choices: `choices` per splat.
+struct RowsParams {
+  int64_t splats;
+  int choices, D;
+  int64_t stride;  // elements between the rows that are read
+  int dtype;
+};
+int launch_rows_by_code(const RowsParams& P, const void* rows,
+                        const int32_t* order, const int32_t* places,
+                        const float* weights, void* out, hipStream_t stream);
+int launch_rows_from_codes(const RowsParams& P, const void* rows,
+                           const int32_t* places, const float* weights,
+                           void* out, hipStream_t stream);
+int launch_rows_from_codes_backward(const RowsParams& P, const void* grad,
+                                    const void* rows, const int32_t* order,
+                                    const int32_t* places, const float* weights,
+                                    void* g_rows, float* g_weights,
+                                    hipStream_t stream);
+
+// ---- code_adapters.hip
+struct AdapterParams {
+  int64_t rows;
+  int K, r, D, E;  // codes, rank, values of a row and of a result
+  int64_t stride;  // elements between rows
+  int dtype;
+  bool by_code;    // rows and results stand in the order of the codes
+  float scale;
+  const int32_t *order, *places, *starts;
+};
+size_t adapters_forward_workspace_bytes(const AdapterParams& P);
+int launch_adapters_forward(const AdapterParams& P, const void* rows,
+                            const void* down, const void* up, const void* base,
+                            void* out, float* hidden, void* workspace,
+                            hipStream_t stream);
+size_t adapters_backward_workspace_bytes(const AdapterParams& P);
+int launch_adapters_backward(const AdapterParams& P, const void* grad,
+                             const void* rows, const void* down, const void* up,
+                             const float* hidden, void* g_rows, void* g_down,
+                             void* g_up, void* workspace, hipStream_t stream);
 
 // ---- code_lookup.hip
 struct LookupParams {

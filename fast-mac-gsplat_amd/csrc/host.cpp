@@ -628,6 +628,7 @@ py::object project(py::handle means3d, py::handle scales, py::handle quats,
 PYBIND11_MODULE(_host, m) {
   using namespace gs_host;
   def_codes(m);
+  def_decoders(m);
   m.def("bind", &bind);
   m.def("set_timed", [](bool on) { g_timed.store(on); });
   // Whether saved tensors go through hooks of the caller's (checkpointing,

@@ -46,7 +46,18 @@ using torch::autograd::variable_list;
   F(code_probs_backward)                  \
   F(code_balance_workspace_bytes)         \
   F(code_balance_forward)                 \
-  F(code_balance_backward)
+  F(code_balance_backward)                \
+  F(group_codes_workspace_bytes)          \
+  F(group_codes)                          \
+  F(rows_by_code)                         \
+  F(rows_from_codes)                      \
+  F(rows_from_codes_backward)             \
+  F(code_adapters_workspace_bytes)        \
+  F(code_adapters_forward)                \
+  F(code_adapters_backward_workspace_bytes) \
+  F(code_adapters_backward)               \
+  F(clip_gradients_workspace_bytes)       \
+  F(clip_gradients)
 struct Api {
 #define GS_POINTER(name) decltype(&gsplat_hip_##name) name = nullptr;
   GS_API(GS_POINTER)
@@ -128,5 +139,6 @@ inline Tensor bytes(int64_t n, const Tensor& like) {
 }
 
 void def_codes(py::module_& m);
+void def_decoders(py::module_& m);
 
 }  // namespace gs_host

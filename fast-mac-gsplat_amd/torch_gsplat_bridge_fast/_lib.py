@@ -31,6 +31,9 @@ MAX_CODES, MAX_CODE_WIDTH = 1 << 28, 1 << 20      # GSPLAT_MAX_CODES / _CODE_WID
 MAX_BALANCE_CODES = 1 << 24               # GSPLAT_MAX_BALANCE_CODES
 MAX_BALANCE_IMAGES = 65535                # GSPLAT_MAX_BALANCE_IMAGES
 MAX_CHOICES = 1 << 20                     # GSPLAT_MAX_CHOICES
+MAX_RANK = 128                            # GSPLAT_MAX_RANK
+MAX_ROWS = 1 << 29                        # rows and choices of decoders by code
+MAX_TENSORS, MAX_VALUES = 1 << 20, 1 << 40        # of gradients clipped together
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GSPLAT_F32 / _BF16 / _F16
 
 _vp = ctypes.c_void_p
@@ -94,12 +97,41 @@ class BalanceMeta(ctypes.Structure):
                 ("stride", _i64), ("code_bytes", _i32)]
 
 
+class GroupMeta(ctypes.Structure):
+    """Mirror of ``gsplat_group_meta``."""
+
+    _fields_ = [("choices", _i64), ("num_codes", _i32), ("code_bytes", _i32)]
+
+
+class RowsMeta(ctypes.Structure):
+    """Mirror of ``gsplat_rows_meta``."""
+
+    _fields_ = [("splats", _i64), ("choices", _i32), ("width", _i32), ("stride", _i64), ("dtype", _i32)]
+
+
+class AdaptersMeta(ctypes.Structure):
+    """Mirror of ``gsplat_adapters_meta``."""
+
+    _fields_ = [("rows", _i64), ("num_codes", _i32), ("rank", _i32), ("width_in", _i32), ("width_out", _i32),
+                ("stride", _i64), ("dtype", _i32), ("by_code", _i32), ("scale", ctypes.c_float)]
+
+
+class ClipTensor(ctypes.Structure):
+    """Mirror of ``gsplat_clip_tensor``."""
+
+    _fields_ = [("source", _vp), ("to", _vp), ("size", _i64), ("dtype", _i32)]
+
+
 _PM = ctypes.POINTER(RasterMeta)
 _PP = ctypes.POINTER(ProjectMeta)
 _PS = ctypes.POINTER(Slice)
 _PL = ctypes.POINTER(LookupMeta)
 _PQ = ctypes.POINTER(ProbsMeta)
 _PB = ctypes.POINTER(BalanceMeta)
+_PG = ctypes.POINTER(GroupMeta)
+_PR = ctypes.POINTER(RowsMeta)
+_PA = ctypes.POINTER(AdaptersMeta)
+_PC = ctypes.POINTER(ClipTensor)
 
 # name -> (restype, argtypes); every name here is declared in gsplat_hip.h.
 SIGNATURES = {
@@ -160,6 +192,17 @@ SIGNATURES = {
     "gsplat_hip_code_balance_workspace_bytes": (_sz, [_PB]),
     "gsplat_hip_code_balance_forward": (ctypes.c_int, [_PB] + [_vp] * 8 + [_sz, _vp]),
     "gsplat_hip_code_balance_backward": (ctypes.c_int, [_PB] + [_vp] * 8),
+    "gsplat_hip_group_codes_workspace_bytes": (_sz, [_PG]),
+    "gsplat_hip_group_codes": (ctypes.c_int, [_PG] + [_vp] * 5 + [_sz, _vp]),
+    "gsplat_hip_rows_by_code": (ctypes.c_int, [_PR] + [_vp] * 6),
+    "gsplat_hip_rows_from_codes": (ctypes.c_int, [_PR] + [_vp] * 5),
+    "gsplat_hip_rows_from_codes_backward": (ctypes.c_int, [_PR] + [_vp] * 8),
+    "gsplat_hip_code_adapters_workspace_bytes": (_sz, [_PA]),
+    "gsplat_hip_code_adapters_forward": (ctypes.c_int, [_PA] + [_vp] * 10 + [_sz, _vp]),
+    "gsplat_hip_code_adapters_backward_workspace_bytes": (_sz, [_PA]),
+    "gsplat_hip_code_adapters_backward": (ctypes.c_int, [_PA] + [_vp] * 12 + [_sz, _vp]),
+    "gsplat_hip_clip_gradients_workspace_bytes": (_sz, [_PC, _i64]),
+    "gsplat_hip_clip_gradients": (ctypes.c_int, [_PC, _i64, ctypes.c_double] + [_vp] * 2 + [_sz, _vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -764,6 +764,124 @@ int gsplat_hip_code_balance_backward(const gsplat_balance_meta* meta,
                                      const float* g_mean_probs, void* g_logits,
                                      void* stream);
 
+/* ---- Decoders by code: what belongs to a code applied to the rows of the
+ * splats that name it.  No counterpart in the reference.
+ *
+ * Choices: the codes of all splats, `choices` per splat.  Sorted by code
+ * (stable; those without a code last):
+ *   order[j]   the choice at place j (splat * choices + number)
+ *   places[i]  the place of choice i; -1 without a code, -2 for a code out of
+ *              range
+ *   starts[k]  the first place of code k, k = 0 .. num_codes: starts[num_codes]
+ *              choices have a code
+ * All int32, the same on every call.  If the sort's look-back gives up (see
+ * GSPLAT_STATUS_LOOKBACK_TIMEOUT) every choice counts as one out of range. */
+typedef struct gsplat_group_meta {
+  int64_t choices;   /* of all splats, 0 .. 2^29 */
+  int32_t num_codes; /* 1 .. 2^28 */
+  int32_t code_bytes;
+} gsplat_group_meta;
+
+size_t gsplat_hip_group_codes_workspace_bytes(const gsplat_group_meta* meta);
+int gsplat_hip_group_codes(const gsplat_group_meta* meta, const void* codes,
+                           int32_t* order, int32_t* places, int32_t* starts,
+                           void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Rows by code and back, with order and places as above: what they hold is
+ * checked where it is used (a choice whose place is no row's is one with a code
+ * out of range). */
+typedef struct gsplat_rows_meta {
+  int64_t splats;    /* splats * choices in 0 .. 2^29 */
+  int32_t choices;   /* per splat, 1 .. 2^20 */
+  int32_t width;     /* values per row, 1 .. 2^20 */
+  int64_t stride;    /* elements between the rows that are read, >= width */
+  int32_t dtype;     /* GSPLAT_F32 / _BF16 / _F16 */
+} gsplat_rows_meta;
+
+/* out[j] = rows[order[j] / choices], at a weight of weights[order[j]] where
+ * they are given; zeros without a code, NaN for one out of range.  out:
+ * splats * choices rows, contiguous. */
+int gsplat_hip_rows_by_code(const gsplat_rows_meta* meta, const void* rows,
+                            const int32_t* order, const int32_t* places,
+                            const float* weights, void* out, void* stream);
+/* out[n] = sum over the splat's choices, in order, of weights * rows[place];
+ * weights NULL: ones.  out: splats rows, contiguous. */
+int gsplat_hip_rows_from_codes(const gsplat_rows_meta* meta, const void* rows,
+                               const int32_t* places, const float* weights,
+                               void* out, void* stream);
+/* Its gradient: g_rows[j] = weights * grad[splat] (contiguous; may be NULL)
+ * and g_weights[i] = <grad[splat], rows[places[i]]> (may be NULL).  grad:
+ * contiguous. */
+int gsplat_hip_rows_from_codes_backward(const gsplat_rows_meta* meta,
+                                        const void* grad, const void* rows,
+                                        const int32_t* order,
+                                        const int32_t* places,
+                                        const float* weights, void* g_rows,
+                                        float* g_weights, void* stream);
+
+/* Low-rank maps, one per code, beside a shared one:
+ *   out[n] = base[n] + scale * up[c] (down[c] rows[n])     (c the splat's code)
+ * down [num_codes][rank][width_in], up [num_codes][width_out][rank], one code
+ * per splat.  Without a code out = base (zeros if base is NULL), out of range
+ * NaN.  by_code: rows, base, out and their gradients stand in the order of the
+ * places, otherwise in the order of the splats.  The hidden values down[c]
+ * rows[n] are floats; sums are floats. */
+typedef struct gsplat_adapters_meta {
+  int64_t rows;      /* 0 .. 2^29 */
+  int32_t num_codes; /* 1 .. 2^28 */
+  int32_t rank;      /* 1 .. GSPLAT_MAX_RANK */
+  int32_t width_in;  /* 1 .. 2^20 */
+  int32_t width_out; /* 1 .. 2^20; rank * num_codes * width < 2^40 */
+  int64_t stride;    /* elements between rows, >= width_in */
+  int32_t dtype;
+  int32_t by_code;
+  float scale;
+} gsplat_adapters_meta;
+#define GSPLAT_MAX_RANK 128
+
+/* hidden: float [rows][rank], in the order of the places, for the backward; may
+ * be NULL. */
+size_t gsplat_hip_code_adapters_workspace_bytes(const gsplat_adapters_meta* meta);
+int gsplat_hip_code_adapters_forward(const gsplat_adapters_meta* meta,
+                                     const void* rows, const int32_t* order,
+                                     const int32_t* places,
+                                     const int32_t* starts, const void* down,
+                                     const void* up, const void* base,
+                                     void* out, float* hidden, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+/* grad: contiguous.  g_rows, g_down, g_up: each may be NULL; every value is
+ * written, sums in an order that does not depend on the run. */
+size_t gsplat_hip_code_adapters_backward_workspace_bytes(const gsplat_adapters_meta* meta);
+int gsplat_hip_code_adapters_backward(const gsplat_adapters_meta* meta,
+                                      const void* grad, const void* rows,
+                                      const int32_t* order,
+                                      const int32_t* places,
+                                      const int32_t* starts, const void* down,
+                                      const void* up, const float* hidden,
+                                      void* g_rows, void* g_down, void* g_up,
+                                      void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* ---- Gradients of many tensors: norm = sqrt(sum of all squares), to[i] =
+ * from[i] * min(1, max_norm / norm).  A norm that is not finite as a float leaves
+ * them as they are.  Squares are added in 64 bits, in an order that does not depend on
+ * the run.  No counterpart in the reference. */
+typedef struct gsplat_clip_tensor {
+  const void* from;
+  void* to;          /* may be from; other overlaps are a mistake */
+  int64_t size;      /* elements, 0 .. 2^40, contiguous */
+  int32_t dtype;     /* GSPLAT_F32 / _BF16 / _F16 */
+} gsplat_clip_tensor;
+
+/* tensors: host memory, read before the call returns.  count: 0 .. 2^20.
+ * max_norm >= 0 (infinity: the norm only).  norm: a float in device memory. */
+size_t gsplat_hip_clip_gradients_workspace_bytes(const gsplat_clip_tensor* tensors,
+                                                 int64_t count);
+int gsplat_hip_clip_gradients(const gsplat_clip_tensor* tensors, int64_t count,
+                              double max_norm, float* norm, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
