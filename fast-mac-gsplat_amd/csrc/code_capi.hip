@@ -295,13 +295,14 @@ int gsplat_hip_group_codes(const gsplat_group_meta* meta, const void* codes,
 
 int gsplat_hip_rows_by_code(const gsplat_rows_meta* meta, const void* rows,
                             const int32_t* order, const int32_t* places,
-                            const float* weights, void* out, void* stream) {
+                            const int32_t* named, const float* weights, void* out,
+                            void* stream) {
   const char* what = "gsplat_hip_rows_by_code";
   gs::RowsParams P;
   int rc = make(meta, P, what);
   if (rc || P.splats == 0) return rc;
-  if ((rc = needs({rows, order, places, out}, what))) return rc;
-  return gs::launch_rows_by_code(P, rows, order, places, weights, out,
+  if ((rc = needs({rows, order, places, named, out}, what))) return rc;
+  return gs::launch_rows_by_code(P, rows, order, places, named, weights, out,
                                  static_cast<hipStream_t>(stream));
 }
 
@@ -320,15 +321,15 @@ int gsplat_hip_rows_from_codes(const gsplat_rows_meta* meta, const void* rows,
 int gsplat_hip_rows_from_codes_backward(const gsplat_rows_meta* meta,
                                         const void* grad, const void* rows,
                                         const int32_t* order, const int32_t* places,
-                                        const float* weights, void* g_rows,
-                                        float* g_weights, void* stream) {
+                                        const int32_t* named, const float* weights,
+                                        void* g_rows, float* g_weights, void* stream) {
   const char* what = "gsplat_hip_rows_from_codes_backward";
   gs::RowsParams P;
   int rc = make(meta, P, what);
   if (rc || P.splats == 0 || (g_rows == nullptr && g_weights == nullptr)) return rc;
-  if ((rc = needs({grad, order, places}, what))) return rc;
-  if (g_weights != nullptr && (rc = needs({rows}, what))) return rc;
-  return gs::launch_rows_from_codes_backward(P, grad, rows, order, places, weights,
+  if ((rc = needs({grad, order, places, named}, what))) return rc;
+  if (g_weights != nullptr && (rc = needs({rows, weights}, what))) return rc;
+  return gs::launch_rows_from_codes_backward(P, grad, rows, order, places, named, weights,
                                              g_rows, g_weights,
                                              static_cast<hipStream_t>(stream));
 }

@@ -319,7 +319,8 @@ size_t group_workspace_bytes(const GroupParams& P);
 int launch_group_codes(const GroupParams& P, int32_t* order, int32_t* places,
                        int32_t* starts, void* workspace, hipStream_t stream);
 
-// Rows of splats and of choices: `choices` per splat.
+// Rows of splats and of choices: `choices` per splat.  named: starts[K], the
+// choices that have a code.
 struct RowsParams {
   int64_t splats;
   int choices, D;
@@ -328,14 +329,15 @@ struct RowsParams {
 };
 int launch_rows_by_code(const RowsParams& P, const void* rows,
                         const int32_t* order, const int32_t* places,
-                        const float* weights, void* out, hipStream_t stream);
+                        const int32_t* named, const float* weights, void* out,
+                        hipStream_t stream);
 int launch_rows_from_codes(const RowsParams& P, const void* rows,
                            const int32_t* places, const float* weights,
                            void* out, hipStream_t stream);
 int launch_rows_from_codes_backward(const RowsParams& P, const void* grad,
                                     const void* rows, const int32_t* order,
-                                    const int32_t* places, const float* weights,
-                                    void* g_rows, float* g_weights,
+                                    const int32_t* places, const int32_t* named,
+                                    const float* weights, void* g_rows, float* g_weights,
                                     hipStream_t stream);
 
 // ---- code_adapters.hip

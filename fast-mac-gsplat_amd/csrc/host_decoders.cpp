@@ -79,14 +79,17 @@ gsplat_rows_meta rows_meta(const Tensor& rows, int64_t stride, const Tensor& pla
                           dtype_of(rows)};
 }
 
-Tensor by_code_values(const Tensor& rows, const Tensor& order, const Tensor& places) {
+// Where the number of choices with a code stands.
+const int32_t* named(const Tensor& starts) { return ids(starts) + starts.numel() - 1; }
+
+Tensor by_code_values(const Tensor& rows, const Groups& g) {
   int64_t stride;
   const Tensor x = rows_of(rows, stride);
-  const Tensor out = at::empty({order.numel(), x.size(x.dim() - 1)}, plain_options(x));
-  const auto meta = rows_meta(x, stride, places);
+  const Tensor out = at::empty({g.order.numel(), x.size(x.dim() - 1)}, plain_options(x));
+  const auto meta = rows_meta(x, stride, g.places);
   const Timed timed("rows_by_code");
-  check(api.rows_by_code(&meta, x.data_ptr(), ids(order), ids(places), nullptr, out.data_ptr(),
-                         stream_of(x)),
+  check(api.rows_by_code(&meta, x.data_ptr(), ids(g.order), ids(g.places), named(g.starts), nullptr,
+                         out.data_ptr(), stream_of(x)),
         "gsplat_hip_rows_by_code");
   return out;
 }
@@ -109,13 +112,13 @@ Tensor from_codes_values(const Tensor& rows, const Tensor& places, const Tensor&
 
 struct ByCode : torch::autograd::Function<ByCode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& order,
-                        const Tensor& places) {
+                        const Tensor& places, const Tensor& starts) {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({places});
-    return by_code_values(rows, order, places);
+    return by_code_values(rows, Groups{order, places, starts});
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(3);
+    variable_list out(4);
     if (!grads[0].defined() || !ctx->needs_input_grad(0)) return out;
     const c10::DeviceGuard device(grads[0].device());
     out[0] = from_codes_values(grads[0], ctx->get_saved_variables()[0].contiguous(), Tensor(),
@@ -136,46 +139,48 @@ py::object by_code(py::handle rows, py::handle order, py::handle places, py::han
   const c10::DeviceGuard device(x.device());
   Tensor out;
   if (at::GradMode::is_enabled() && x.requires_grad()) {
-    out = ByCode::apply(x, g.order, g.places);
+    out = ByCode::apply(x, g.order, g.places, g.starts);
   } else {
     at::AutoDispatchBelowADInplaceOrView below;
-    out = by_code_values(x, g.order, g.places);
+    out = by_code_values(x, g);
   }
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
 }
 
 struct FromCodes : torch::autograd::Function<FromCodes> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& order,
-                        const Tensor& places, const std::optional<Tensor>& given_weights) {
+                        const Tensor& places, const Tensor& starts,
+                        const std::optional<Tensor>& given_weights) {
     const Tensor weights = given_weights.value_or(Tensor());
     ctx->set_materialize_grads(false);
     // (the rows are for the weights' gradient only)
     const bool keep = weights.defined() && weights.requires_grad();
-    ctx->save_for_backward({keep ? rows : Tensor(), order, places, weights});
-    ctx->saved_data["dtype"] = (int64_t)dtype_of(rows);
+    ctx->save_for_backward({keep ? rows : Tensor(), order, places, starts, weights});
     return from_codes_values(rows, places, weights, "rows_from_codes");
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(4);
+    variable_list out(5);
     const auto saved = ctx->get_saved_variables();
-    const Tensor& weights = saved[3];
+    const Tensor& weights = saved[4];
     const bool need_rows = ctx->needs_input_grad(0);
-    const bool need_weights = weights.defined() && ctx->needs_input_grad(3);
+    const bool need_weights = weights.defined() && ctx->needs_input_grad(4);
     if (!grads[0].defined() || !(need_rows || need_weights)) return out;
     const c10::DeviceGuard device(grads[0].device());
     const Tensor g = grads[0].contiguous();
     const Tensor order = saved[1].contiguous(), places = saved[2].contiguous();
+    const Tensor starts = saved[3].contiguous();
     const Tensor w = weights.defined() ? weights.contiguous() : weights;
     const int64_t D = g.size(g.dim() - 1);
     int64_t stride = D;
     const Tensor rows = need_weights ? rows_of(saved[0], stride) : Tensor();
     auto meta = rows_meta(g, stride, places);
     if (need_rows) out[0] = at::empty({order.numel(), D}, plain_options(g));
-    if (need_weights) out[3] = at::empty(weights.sizes(), plain_options(g).dtype(at::kFloat));
+    if (need_weights) out[4] = at::empty(weights.sizes(), plain_options(g).dtype(at::kFloat));
     {
       const Timed timed("rows_from_codes_backward");
       check(api.rows_from_codes_backward(&meta, g.data_ptr(), pointer(rows), ids(order), ids(places),
-                                         f32_or_null(w), pointer(out[0]), f32_or_null(out[3]),
+                                         named(starts), f32_or_null(w), pointer(out[0]),
+                                         f32_or_null(out[4]),
                                          stream_of(g)),
             "gsplat_hip_rows_from_codes_backward");
     }
@@ -200,7 +205,8 @@ py::object from_codes(py::handle rows, py::handle order, py::handle places, py::
   const c10::DeviceGuard device(y.device());
   Tensor out;
   if (at::GradMode::is_enabled() && (y.requires_grad() || (w.defined() && w.requires_grad()))) {
-    out = FromCodes::apply(y, g.order, g.places, w.defined() ? std::optional<Tensor>(w) : std::nullopt);
+    out = FromCodes::apply(y, g.order, g.places, g.starts,
+                           w.defined() ? std::optional<Tensor>(w) : std::nullopt);
   } else {
     at::AutoDispatchBelowADInplaceOrView below;
     out = from_codes_values(y, g.places, w, "rows_from_codes");

@@ -194,9 +194,9 @@ SIGNATURES = {
     "gsplat_hip_code_balance_backward": (ctypes.c_int, [_PB] + [_vp] * 8),
     "gsplat_hip_group_codes_workspace_bytes": (_sz, [_PG]),
     "gsplat_hip_group_codes": (ctypes.c_int, [_PG] + [_vp] * 5 + [_sz, _vp]),
-    "gsplat_hip_rows_by_code": (ctypes.c_int, [_PR] + [_vp] * 6),
+    "gsplat_hip_rows_by_code": (ctypes.c_int, [_PR] + [_vp] * 7),
     "gsplat_hip_rows_from_codes": (ctypes.c_int, [_PR] + [_vp] * 5),
-    "gsplat_hip_rows_from_codes_backward": (ctypes.c_int, [_PR] + [_vp] * 8),
+    "gsplat_hip_rows_from_codes_backward": (ctypes.c_int, [_PR] + [_vp] * 9),
     "gsplat_hip_code_adapters_workspace_bytes": (_sz, [_PA]),
     "gsplat_hip_code_adapters_forward": (ctypes.c_int, [_PA] + [_vp] * 10 + [_sz, _vp]),
     "gsplat_hip_code_adapters_backward_workspace_bytes": (_sz, [_PA]),

@@ -82,38 +82,41 @@ def _rows_meta(flat: Tensor, places: Tensor) -> _lib.RowsMeta:
     return _lib.RowsMeta(places.numel() // S, S, flat.shape[-1], _stride(flat), _lib.DTYPES[flat.dtype])
 
 
+def _named(starts: Tensor) -> int:
+    """Where the number of choices with a code stands."""
+    return ptr(starts) + 4 * (starts.numel() - 1)
+
+
 @torch.library.custom_op(f"{_NS}::rows_by_code", mutates_args=())
-def _by_code(rows: Tensor, order: Tensor, places: Tensor) -> Tensor:
-    _check_by_code(rows, order, places)
-    flat, o, p = _rows_of(rows), order.contiguous(), places.contiguous()
+def _by_code(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor) -> Tensor:
+    _check_by_code(rows, order, places, starts)
+    flat, o, p, s = _rows_of(rows), order.contiguous(), places.contiguous(), starts.contiguous()
     out = torch.empty((o.numel(), rows.shape[-1]), dtype=rows.dtype, device=rows.device)
     with torch.cuda.device(rows.device), _timed("rows_by_code"):
-        check(_lib.lib().gsplat_hip_rows_by_code(_rows_meta(flat, p), ptr(flat), ptr(o), ptr(p), None, ptr(out),
-                                                 stream_of(flat)), "gsplat_hip_rows_by_code")
+        check(_lib.lib().gsplat_hip_rows_by_code(_rows_meta(flat, p), ptr(flat), ptr(o), ptr(p), _named(s), None,
+                                                 ptr(out), stream_of(flat)), "gsplat_hip_rows_by_code")
     return out
 
 
 @_by_code.register_fake
-def _(rows, order, places):
+def _(rows, order, places, starts):
     return rows.new_empty((order.numel(), rows.shape[-1]))
 
 
 def _by_code_setup(ctx, inputs, output):
-    _, order, places = inputs
-    ctx.save_for_backward(order, places)
+    ctx.save_for_backward(*inputs[1:])
 
 
 def _by_code_grad(ctx, grad):
-    order, places = ctx.saved_tensors
-    return (_from_codes(grad, order, places, None) if ctx.needs_input_grad[0] else None), None, None
+    return (_from_codes(grad, *ctx.saved_tensors, None) if ctx.needs_input_grad[0] else None), None, None, None
 
 
 _by_code.register_autograd(_by_code_grad, setup_context=_by_code_setup)
 
 
 @torch.library.custom_op(f"{_NS}::rows_from_codes", mutates_args=())
-def _from_codes(rows: Tensor, order: Tensor, places: Tensor, weights: Optional[Tensor]) -> Tensor:
-    _check_from_codes(rows, order, places, weights)
+def _from_codes(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor, weights: Optional[Tensor]) -> Tensor:
+    _check_from_codes(rows, order, places, starts, weights)
     flat, p = _rows_of(rows), places.contiguous()
     w = None if weights is None else weights.contiguous()
     out = torch.empty((*places.shape[:-1], rows.shape[1]), dtype=rows.dtype, device=rows.device)
@@ -124,30 +127,30 @@ def _from_codes(rows: Tensor, order: Tensor, places: Tensor, weights: Optional[T
 
 
 @_from_codes.register_fake
-def _(rows, order, places, weights):
+def _(rows, order, places, starts, weights):
     return rows.new_empty((*places.shape[:-1], rows.shape[1]))
 
 
 @torch.library.custom_op(f"{_NS}::rows_from_codes_backward", mutates_args=())
-def _from_codes_backward(grad: Tensor, rows: Tensor, order: Tensor, places: Tensor, weights: Optional[Tensor],
-                         need_rows: bool, need_weights: bool) -> Tuple[Tensor, Tensor]:
-    _check_from_codes(rows, order, places, weights)
+def _from_codes_backward(grad: Tensor, rows: Tensor, order: Tensor, places: Tensor, starts: Tensor,
+                         weights: Optional[Tensor], need_rows: bool, need_weights: bool) -> Tuple[Tensor, Tensor]:
+    _check_from_codes(rows, order, places, starts, weights)
     _check_given("grad", grad, (*places.shape[:-1], rows.shape[1]), rows.dtype, rows)
     if need_weights and weights is None:
         raise ValueError("weights are required for their gradient")
-    flat, g, o, p = _rows_of(rows), grad.contiguous(), order.contiguous(), places.contiguous()
+    flat, g, o, p, s = _rows_of(rows), *(t.contiguous() for t in (grad, order, places, starts))
     w = None if weights is None else weights.contiguous()
     g_rows = torch.empty(rows.shape if need_rows else (0,), dtype=rows.dtype, device=rows.device)
     g_weights = torch.empty(weights.shape if need_weights else (0,), dtype=torch.float32, device=rows.device)
     with torch.cuda.device(rows.device), _timed("rows_from_codes_backward"):
         check(_lib.lib().gsplat_hip_rows_from_codes_backward(
-            _rows_meta(flat, p), ptr(g), ptr(flat), ptr(o), ptr(p), ptr(w), ptr(g_rows) if need_rows else None,
+            _rows_meta(flat, p), ptr(g), ptr(flat), ptr(o), ptr(p), _named(s), ptr(w), ptr(g_rows) if need_rows else None,
             ptr(g_weights) if need_weights else None, stream_of(g)), "gsplat_hip_rows_from_codes_backward")
     return g_rows, g_weights
 
 
 @_from_codes_backward.register_fake
-def _(grad, rows, order, places, weights, need_rows, need_weights):
+def _(grad, rows, order, places, starts, weights, need_rows, need_weights):
     return (rows.new_empty(rows.shape if need_rows else (0,)),
             rows.new_empty(weights.shape if need_weights else (0,), dtype=torch.float32))
 
@@ -157,10 +160,9 @@ def _from_codes_setup(ctx, inputs, output):
 
 
 def _from_codes_grad(ctx, grad):
-    rows, order, places, weights = ctx.saved_tensors
     need = ctx.needs_input_grad
-    g_rows, g_weights = _from_codes_backward(grad, rows, order, places, weights, need[0], need[3])
-    return g_rows if need[0] else None, None, None, g_weights if need[3] else None
+    g_rows, g_weights = _from_codes_backward(grad, *ctx.saved_tensors, need[0], need[4])
+    return g_rows if need[0] else None, None, None, None, g_weights if need[4] else None
 
 
 _from_codes.register_autograd(_from_codes_grad, setup_context=_from_codes_setup)
@@ -273,13 +275,13 @@ def _check_group(codes: Tensor, num_codes: int, several: bool) -> None:
     _check_device(codes=codes)
 
 
-def _check_groups(order: Tensor, places: Tensor, starts: Optional[Tensor] = None) -> None:
+def _check_groups(order: Tensor, places: Tensor, starts: Tensor) -> None:
     for name, t in (("order", order), ("places", places), ("starts", starts)):
-        if t is not None and t.dtype != torch.int32:
+        if t.dtype != torch.int32:
             raise ValueError(f"groups' {name} must be int32")
     if places.ndim < 1 or places.shape[-1] == 0 or tuple(order.shape) != (places.numel(),):
         raise ValueError("groups must be what group_codes returns: order [N*S], places [...,S]")
-    if starts is not None and (starts.ndim != 1 or starts.numel() < 2):
+    if starts.ndim != 1 or starts.numel() < 2:
         raise ValueError("groups must be what group_codes returns: starts [K+1]")
     _check_size("choices", order.numel(), _lib.MAX_ROWS)
     _check_size("choices per splat", places.shape[-1], _lib.MAX_CHOICES)
@@ -292,17 +294,17 @@ def _check_rows(rows: Tensor) -> None:
     _check_size("values per row", rows.shape[-1], _lib.MAX_CODE_WIDTH)
 
 
-def _check_by_code(rows: Tensor, order: Tensor, places: Tensor) -> None:
+def _check_by_code(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor) -> None:
     _check_rows(rows)
-    _check_groups(order, places)
+    _check_groups(order, places, starts)
     if rows.shape[:-1] != places.shape[:-1]:
         raise ValueError("rows must have a row per splat: the shape of the splats, and the values")
-    _check_device(rows=rows, order=order, places=places)
+    _check_device(rows=rows, order=order, places=places, starts=starts)
 
 
-def _check_from_codes(rows: Tensor, order: Tensor, places: Tensor, weights: Optional[Tensor]) -> None:
+def _check_from_codes(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor, weights: Optional[Tensor]) -> None:
     _check_rows(rows)
-    _check_groups(order, places)
+    _check_groups(order, places, starts)
     if rows.ndim != 2 or rows.shape[0] != order.numel():
         raise ValueError("rows must have a row per choice, in the order of the codes")
     if weights is not None:
@@ -310,7 +312,7 @@ def _check_from_codes(rows: Tensor, order: Tensor, places: Tensor, weights: Opti
             raise ValueError("weights must be float32")
         if weights.shape != places.shape and (places.shape[-1] != 1 or weights.shape != places.shape[:-1]):
             raise ValueError("weights must match codes shape")
-    _check_device(rows=rows, order=order, places=places, weights=weights)
+    _check_device(rows=rows, order=order, places=places, starts=starts, weights=weights)
 
 
 def _check_adapters(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor, down: Tensor, up: Tensor,
@@ -366,8 +368,8 @@ def rows_by_code(rows: Tensor, groups: CodeGroups) -> Tensor:
     if out is not None:
         return out
     _check_reverse(rows)
-    _check_by_code(rows, groups.order, groups.places)
-    return _by_code(rows, groups.order, groups.places)
+    _check_by_code(rows, *groups)
+    return _by_code(rows, *groups)
 
 
 def rows_from_codes(rows: Tensor, groups: CodeGroups, weights: Optional[Tensor] = None) -> Tensor:
@@ -379,8 +381,8 @@ def rows_from_codes(rows: Tensor, groups: CodeGroups, weights: Optional[Tensor] 
     if out is not None:
         return out
     _check_reverse(rows, weights)
-    _check_from_codes(rows, groups.order, groups.places, weights)
-    return _from_codes(rows, groups.order, groups.places, weights)
+    _check_from_codes(rows, *groups, weights)
+    return _from_codes(rows, *groups, weights)
 
 
 def code_adapters(rows: Tensor, groups: CodeGroups, down: Tensor, up: Tensor, base: Optional[Tensor] = None,

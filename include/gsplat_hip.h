@@ -800,23 +800,26 @@ typedef struct gsplat_rows_meta {
 } gsplat_rows_meta;
 
 /* out[j] = rows[order[j] / choices], at a weight of weights[order[j]] where
- * they are given; zeros without a code, NaN for one out of range.  out:
- * splats * choices rows, contiguous. */
+ * they are given; zeros without a code, NaN for one out of range.  named:
+ * starts + num_codes, the number of choices that have a code, in device memory.
+ * out: splats * choices rows, contiguous. */
 int gsplat_hip_rows_by_code(const gsplat_rows_meta* meta, const void* rows,
                             const int32_t* order, const int32_t* places,
-                            const float* weights, void* out, void* stream);
+                            const int32_t* named, const float* weights,
+                            void* out, void* stream);
 /* out[n] = sum over the splat's choices, in order, of weights * rows[place];
  * weights NULL: ones.  out: splats rows, contiguous. */
 int gsplat_hip_rows_from_codes(const gsplat_rows_meta* meta, const void* rows,
                                const int32_t* places, const float* weights,
                                void* out, void* stream);
 /* Its gradient: g_rows[j] = weights * grad[splat] (contiguous; may be NULL)
- * and g_weights[i] = <grad[splat], rows[places[i]]> (may be NULL).  grad:
- * contiguous. */
+ * and g_weights[i] = <grad[splat], rows[places[i]]> (may be NULL; needs
+ * weights).  grad: contiguous. */
 int gsplat_hip_rows_from_codes_backward(const gsplat_rows_meta* meta,
                                         const void* grad, const void* rows,
                                         const int32_t* order,
                                         const int32_t* places,
+                                        const int32_t* named,
                                         const float* weights, void* g_rows,
                                         float* g_weights, void* stream);
 

@@ -127,9 +127,9 @@ def test_fake_implementations():
         order, places, starts = ops.group_codes(c, 7, True)
         assert places.shape == (2, 5)
         x = torch.zeros(2, 4, dtype=BF16)
-        y = ops.rows_by_code(x, order, places)
+        y = ops.rows_by_code(x, order, places, starts)
         assert y.shape == (10, 4) and y.dtype == BF16
-        assert ops.rows_from_codes(y, order, places, None).shape == (2, 4)
+        assert ops.rows_from_codes(y, order, places, starts, None).shape == (2, 4)
         out, hidden = ops.code_adapters(y, order, places, starts, torch.zeros(7, 3, 4, dtype=BF16),
                                         torch.zeros(7, 6, 3, dtype=BF16), None, 1.0, True)
         assert out.shape == (10, 6) and out.dtype == BF16 and hidden.shape == (10, 3) and hidden.dtype == torch.float32
@@ -153,11 +153,11 @@ def test_c_abi_refusals():
     for m, text in ((_lib.RowsMeta(5, 0, 3, 3, 0), "choices must lie"), (_lib.RowsMeta(1 << 28, 4, 3, 3, 0), "splats * choices"),
                     (_lib.RowsMeta(5, 1, 0, 3, 0), "width must lie"), (_lib.RowsMeta(5, 1, 3, 2, 0), "stride"),
                     (_lib.RowsMeta(5, 1, 3, 3, 3), "dtype")):
-        _refused(L.gsplat_hip_rows_by_code(m, d, d, d, None, d, None), text)
+        _refused(L.gsplat_hip_rows_by_code(m, d, d, d, d, None, d, None), text)
         _refused(L.gsplat_hip_rows_from_codes(m, d, d, None, d, None), text)
-        _refused(L.gsplat_hip_rows_from_codes_backward(m, d, d, d, d, None, d, None, None), text)
-    _refused(L.gsplat_hip_rows_by_code(_lib.RowsMeta(5, 1, 3, 3, 0), d, None, d, None, d, None), "NULL")
-    _refused(L.gsplat_hip_rows_from_codes_backward(_lib.RowsMeta(5, 1, 3, 3, 0), d, None, d, d, d, d, d, None), "NULL")
+        _refused(L.gsplat_hip_rows_from_codes_backward(m, d, d, d, d, d, None, d, None, None), text)
+    _refused(L.gsplat_hip_rows_by_code(_lib.RowsMeta(5, 1, 3, 3, 0), d, None, d, d, None, d, None), "NULL")
+    _refused(L.gsplat_hip_rows_from_codes_backward(_lib.RowsMeta(5, 1, 3, 3, 0), d, None, d, d, d, d, d, d, None), "NULL")
     ok = (5, 3, 2, 4, 6, 4, 0, 0, 1.0)
     for at, v, text in ((0, -1, "rows must lie"), (1, 0, "num_codes"), (2, 129, "rank must lie"), (2, 0, "rank must lie"),
                         (3, 0, "width_in"), (4, (1 << 20) + 1, "width_out"), (5, 3, "stride"), (6, 7, "dtype")):
