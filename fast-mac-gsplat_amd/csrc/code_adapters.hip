@@ -12,7 +12,7 @@
 // A workgroup takes a tile: up to M places of one code, whose rows it reads
 // once.  Its four wavefronts share out the rows' values, D, for the hidden
 // values (which meet in LDS) and then the results' values, E.  The gradient of
-// the rows is the same with up^T and down^T, laid out by a launch before it.
+// the rows is the same with up^T and down^T, turned on their way through LDS.
 // Gradients of the maps: a workgroup takes up to L places of a code and a block
 // of columns; longer codes' sums are joined by another launch, in order.
 //
@@ -21,6 +21,7 @@
 // that the result's rounding is the only one that counts), and float16 factors
 // beside them as two bfloat16 too, exactly: hidden values have no range to leave.
 #include <algorithm>
+#include <type_traits>
 
 #include "codes.h"
 
@@ -155,6 +156,140 @@ __device__ __forceinline__ void parts(vec_t<T> x, bf16x8& hi, bf16x8& lo) {
   }
 }
 
+// Values i .. i + kVec - 1 of a row of n, zeros past its end.  Whole: n is a multiple
+// of kVec, so that a vector is in the row or past it.  (Nothing branches then:
+// with a branch around each load the compiler waits for one before the next.)
+template <typename T, bool Whole>
+__device__ __forceinline__ vec_t<T> load_whole(const T* row, int i, int n) {
+  if constexpr (Whole) {
+    vec_t<T> v = load_vec(row + min(i, n - kVec<T>));
+    if (i >= n)
+#pragma unroll
+      for (int q = 0; q < kVec<T>; ++q) v[q] = static_cast<T>(0.0f);
+    return v;
+  } else {
+    return load_part(row, i, n, static_cast<T>(0.0f));
+  }
+}
+
+// N adjacent values of a row of n from i on, zeros past its end.  Whole: n is a
+// multiple of N.
+template <int N, typename T, bool Whole>
+__device__ __forceinline__ void load_n(T (&v)[N], const T* row, int i, int n) {
+  if (Whole || i + N <= n) {
+    __builtin_memcpy(v, row + (Whole ? min(i, n - N) : i), sizeof(v));
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < N; ++q) v[q] = i + q < n ? row[i + q] : static_cast<T>(0.0f);
+}
+template <int N, typename T, bool Whole>
+__device__ __forceinline__ void store_n(T* row, int i, int n, const T (&v)[N]) {
+  if (Whole ? i < n : i + N <= n) {
+    __builtin_memcpy(row + i, v, sizeof(v));
+    return;
+  }
+  if (Whole) return;
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+    if (i + q < n) row[i + q] = v[q];
+}
+
+// Eight rows of eight 16-bit values (four of four in 32 bits) turned.
+template <typename T>
+__device__ __forceinline__ void turn(vec_t<T> (&x)[kVec<T>]) {
+  constexpr int V = kVec<T>;
+  vec_t<T> y[V];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[i][j] = x[j][i];
+  } else {
+    u32x4 w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __builtin_bit_cast(u32x4, x[j]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u32x4 z;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        z[p] = __builtin_amdgcn_perm(w[2 * p + 1][i / 2], w[2 * p][i / 2],
+                                     i % 2 ? 0x07060302u : 0x05040100u);
+      y[i] = __builtin_bit_cast(vec_t<T>, z);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = y[i];
+}
+
+// A factor on its way to the tiles.  The matrix instructions take a lane's 16
+// bytes from row lane % 16: loaded so, every lane would be a request of its own
+// (64 a load, where 8 lanes of a row make one).  So a wavefront
+// loads rows of adjacent chunks of 16 bytes, and turns them over in its own part
+// of LDS, no barrier needed.  Chunk c of row i lies at c ^ (a few bits of i): both
+// ways touch every bank once.
+template <int Chunks>
+__device__ __forceinline__ int swizzled(int row, int chunk) {
+  constexpr int kMask = Chunks < 8 ? Chunks - 1 : 7, kRows = Chunks < 8 ? 8 / Chunks : 1;
+  return row * Chunks + (chunk ^ (row / kRows & kMask));
+}
+__device__ __forceinline__ void wavefront_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// kRows x kChunks chunks of a map of `rows` x `depth` values, ld apart: rows of
+// adjacent values, or (Turned) the values of adjacent rows side by side.  Values
+// past the depth are zeros, rows past the last repeat it.
+template <typename T, bool Turned, bool Whole, int kRows, int kChunks>
+struct MapChunks {
+  static constexpr int V = kVec<T>, kEach = Turned ? V : 1;
+  static constexpr int kTasks = kRows / kEach * kChunks, kTurns = (kTasks + 63) / 64;
+  vec_t<T> v[kTurns][kEach];
+  __device__ __forceinline__ void load(const T* map, int ld, int rows, int depth, int row0, int k0) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int task = u * 64 + lane;
+      if constexpr (Turned) {
+        const int row = row0 + task % (kRows / V) * V, k = k0 + task / (kRows / V) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const T* at = map + (int64_t)min(k + j, depth - 1) * ld;
+          v[u][j] = Whole ? load_vec(at + min(row, rows - V))
+                          : load_part(at, row, rows, static_cast<T>(0.0f));
+          if (k + j >= depth)
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[u][j][q] = static_cast<T>(0.0f);
+        }
+      } else {
+        const int row = row0 + task / kChunks, k = k0 + task % kChunks * V;
+        v[u][0] = load_whole<T, Whole>(map + (int64_t)min(row, rows - 1) * ld, k, depth);
+      }
+    }
+  }
+  // place(row, chunk): where it lies
+  template <typename Place>
+  __device__ __forceinline__ void store(u32x4* lds, Place place) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int task = u * 64 + lane;
+      if (kTasks % 64 != 0 && task >= kTasks) continue;
+      if constexpr (Turned) {
+        turn<T>(v[u]);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          lds[place(task % (kRows / V) * V + i, task / (kRows / V))] = __builtin_bit_cast(u32x4, v[u][i]);
+      } else {
+        lds[place(task / kChunks, task % kChunks)] = __builtin_bit_cast(u32x4, v[u][0]);
+      }
+    }
+  }
+};
+
 // Hidden values of a tile as the second product's factor.  Rank blocks of 16 in
 // 32 bits, of 32 in 16 bits; a single block of 16 ranks holds hi and lo side by
 // side instead.
@@ -164,22 +299,27 @@ struct Hidden {
   static constexpr bool kBoth = !kWide && RT == 1;
   static constexpr int kBlocks = kWide || RT == 1 ? RT : RT / 2;
   static constexpr int kRow = kWide ? 16 * RT + 4 : 16 * RT + 8;  // of LDS, elements
+  static constexpr int kChunks = 16 * RT / kVec<T>;               // of a map's row
   using Factor = std::conditional_t<kWide, vec_t<float>, bf16x8>;
+  using Element = std::conditional_t<kWide, float, uint16_t>;
+  // the map's chunk that a lane's quarter multiplies in rank block k
+  static __device__ __forceinline__ int chunk(int k, int quarter) {
+    return kBoth ? quarter & 1 : 4 * k + quarter;
+  }
 };
 
-// acc += up * h for one rank block.
+// acc += h * up for one rank block.
 template <typename T, int RT>
-__device__ __forceinline__ void mma_hidden(f32x4& acc, vec_t<T> up,
-                                           typename Hidden<T, RT>::Factor hi,
-                                           typename Hidden<T, RT>::Factor lo) {
+__device__ __forceinline__ void mma_hidden(f32x4& acc, typename Hidden<T, RT>::Factor hi,
+                                           typename Hidden<T, RT>::Factor lo, vec_t<T> up) {
   if constexpr (sizeof(T) == 4) {
-    mma<float>(acc, up, hi);
+    mma<float>(acc, hi, up);
   } else {
     bf16x8 u, v;
     parts<T>(up, u, v);
-    mma<__bf16>(acc, u, hi);
-    if constexpr (RT > 1) mma<__bf16>(acc, u, lo);
-    if constexpr (!__is_same(T, __bf16)) mma<__bf16>(acc, v, hi);
+    mma<__bf16>(acc, hi, u);
+    if constexpr (RT > 1) mma<__bf16>(acc, lo, u);
+    if constexpr (!__is_same(T, __bf16)) mma<__bf16>(acc, hi, v);
   }
 }
 
@@ -189,8 +329,8 @@ struct RowsArgs {
   const void* rows;
   int64_t stride;
   int D, E;
-  const void* down;  // [K][r][D]
-  const void* up;    // [K][E][r]
+  const void* down;  // [K][r][D], or turned: [K][D][r]
+  const void* up;    // [K][E][r], or turned: [K][r][E]
   const void* base;  // [rows][E], or null
   float f_hidden, f_out;
   void* out;         // or null: the hidden values only
@@ -199,101 +339,257 @@ struct RowsArgs {
   int splits;
 };
 
-// Phase 1: hidden values, over part blockIdx.y of D, left in `parts`; 2: results
-// from them, over part blockIdx.y of E; 3: both.
-template <typename T, int MT, int RT, int Phase>
-__global__ __launch_bounds__(kThreads) void adapters_rows_kernel(AdapterParams P, RowsArgs A,
-                                                                 Slots S) {
+// The LDS of a workgroup.
+template <typename T, int MT, int RT>
+struct RowsLds {
   using H = Hidden<T, RT>;
-  constexpr int V = kVec<T>, M = 16 * MT, R = 16 * RT, kStep = 4 * V, kPad = R + 4;
-  __shared__ __attribute__((aligned(16))) float red[2][M][kPad];
-  __shared__ __attribute__((aligned(16))) uint16_t parts16[H::kWide ? 1 : 2][H::kWide ? 1 : M][H::kWide ? 8 : H::kRow];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int col = lane & 15, quarter = lane >> 4;
-  const Tile t = tile_at(P, S, S.begin + xcd_remap(blockIdx.x, gridDim.x));
-  if (t.count == 0) return;
-  const T* rows = static_cast<const T*>(A.rows);
-  if (t.code >= P.K) {  // without a code
-    if (Phase == 1 || A.out == nullptr) return;
-    const T* base = static_cast<const T*>(A.base);
-    T* out = static_cast<T*>(A.out);
-    const int step = kThreads * (Phase == 2 ? gridDim.y : 1);
-    for (int m = 0; m < t.count; ++m) {
-      const int64_t j = t.first + m;
-      const int i = P.order[j], n = row_at(P, j);
-      if (n < 0) continue;
-      const float rest =
-          i >= 0 && i < P.rows && P.places[i] == kNoCode ? 0.0f : __builtin_nanf("");
-      for (int e = (Phase == 2 ? blockIdx.y * kThreads : 0) + threadIdx.x; e < A.E; e += step)
-        out[(int64_t)n * A.E + e] =
-            base && rest == 0.0f ? base[(int64_t)n * A.E + e] : static_cast<T>(rest);
-    }
-    return;
-  }
-  int n[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) n[m] = row_at(P, t.first + min(16 * m + col, t.count - 1));
+  static constexpr int V = kVec<T>, M = 16 * MT, R = 16 * RT;
+  // columns of a lane in the second product
+  static constexpr int kCols = RT >= (sizeof(T) == 4 ? 8 : 4) ? V / 2 : V;
+  static constexpr int kFirst = (M + R) * 8, kSecond = 16 * kCols * H::kChunks;  // chunks of a wavefront
+  union {
+    u32x4 stage[4][kFirst > kSecond ? kFirst : kSecond];
+    float red[2][M][R + 4];
+  };
+  __attribute__((aligned(16))) typename H::Element hidden[H::kWide ? 1 : 2][M][H::kRow];
+  int rows[M];
+};
 
-  if constexpr (Phase & 1) {
-    f32x4 acc[MT][RT];
+// Sums of a wavefront's rows m0 .. m0 + 16 MW over chunks first, first + step, ... of
+// D: 128 bytes of each row.
+template <typename T, int MW, int RT, bool Turned, bool Whole>
+__device__ __forceinline__ void first_product(f32x4 (&acc)[MW][RT], const RowsArgs& A, int r,
+                                              const T* down, u32x4* stage, const int* ids, int first,
+                                              int step) {
+  constexpr int V = kVec<T>, kChunk = 8 * V;
+  const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const int row = lane >> 3, c = lane & 7;
+  const T* x[2 * MW];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < 2 * MW; ++i)
+    x[i] = static_cast<const T*>(A.rows) + (int64_t)max(ids[8 * i + row], 0) * A.stride;
+  u32x4 *rows_at = stage, *map_at = stage + 16 * MW * 8;
+  vec_t<T> v[2 * MW];
+  MapChunks<T, Turned, Whole, 16 * RT, 8> map;
+  const int ld = Turned ? r : A.D;
+  auto load = [&](int at) {
 #pragma unroll
-      for (int k = 0; k < RT; ++k) acc[m][k] = f32x4{0, 0, 0, 0};
-    const T *x[MT], *d[RT];
+    for (int i = 0; i < 2 * MW; ++i) v[i] = load_whole<T, Whole>(x[i], at * kChunk + c * V, A.D);
+    map.load(down, ld, r, A.D, 0, at * kChunk);
+  };
+  int at = first;
+  if (at * kChunk < A.D) load(at);
+  for (; at * kChunk < A.D; at += step) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) x[m] = rows + (int64_t)max(n[m], 0) * A.stride;
-    const T* down = static_cast<const T*>(A.down) + t.code * P.r * A.D;
+    for (int i = 0; i < 2 * MW; ++i)
+      rows_at[swizzled<8>(8 * i + row, c)] = __builtin_bit_cast(u32x4, v[i]);
+    map.store(map_at, swizzled<8>);
+    wavefront_sync();
+    if ((at + step) * kChunk < A.D) load(at + step);  // (on its way during the products)
 #pragma unroll
-    for (int k = 0; k < RT; ++k) d[k] = down + (int64_t)min(16 * k + col, P.r - 1) * A.D;
-    constexpr int U = MT * RT > 8 ? 1 : MT + RT > 4 ? 2 : 4;
-    const int full = A.D / kStep, turn = 4 * (Phase == 1 ? gridDim.y : 1);
-    int s = w + 4 * (Phase == 1 ? blockIdx.y : 0);
-    for (; s + (U - 1) * turn < full; s += U * turn) {
-      vec_t<T> a[U][RT], b[U][MT];
+    for (int u = 0; u < 2; ++u) {
+      vec_t<T> a[RT];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = (s + u * turn) * kStep + quarter * V;
+      for (int k = 0; k < RT; ++k)
+        a[k] = __builtin_bit_cast(vec_t<T>, map_at[swizzled<8>(16 * k + col, 4 * u + quarter)]);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) b[u][m] = load_vec(x[m] + at);
+      for (int m = 0; m < MW; ++m) {
+        const auto b = __builtin_bit_cast(vec_t<T>, rows_at[swizzled<8>(16 * m + col, 4 * u + quarter)]);
 #pragma unroll
-        for (int k = 0; k < RT; ++k) a[u][k] = load_vec(d[k] + at);
+        for (int k = 0; k < RT; ++k) mma<T>(acc[m][k], a[k], b);
+      }
+    }
+    wavefront_sync();
+  }
+}
+
+// Results of rows m0 .. m0 + 16 MW in column blocks first, first + step, ...: lane l
+// has kCols adjacent columns of rows 4 (l / 16) + 0..3, so that 16 lanes write
+// 16 kCols adjacent ones.
+template <typename T, int MT, int RT, int MW, bool Turned, bool Whole>
+__device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T* up,
+                                               RowsLds<T, MT, RT>& lds, u32x4* stage, int m0,
+                                               int count, int first, int step) {
+  using L = RowsLds<T, MT, RT>;
+  using H = Hidden<T, RT>;
+  constexpr int N = L::kCols, kBlock = 16 * N;
+  const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const T* base = static_cast<const T*>(A.base);
+  T* out = static_cast<T*>(A.out);
+  const int ld = Turned ? A.E : r;
+  auto place = [](int row, int chunk) {
+    const int n = row / N, t = row % N;
+    return t * 16 * H::kChunks + swizzled<H::kChunks>(n, chunk);
+  };
+  MapChunks<T, Turned, Whole, kBlock, H::kChunks> map;
+  if (first * kBlock < A.E) map.load(up, ld, A.E, r, first * kBlock, 0);
+  for (int at = first; at * kBlock < A.E; at += step) {
+    const int e = at * kBlock + N * col;
+    T y[2][4][N];
+    auto load_base = [&](int m, T (&to)[4][N]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_n<N, T, Whole>(to[i], base + (int64_t)max(lds.rows[m0 + 16 * m + 4 * quarter + i], 0) * A.E,
+                            e, A.E);
+    };
+    if (base) load_base(0, y[0]);
+    map.store(stage, place);
+    wavefront_sync();
+    if ((at + step) * kBlock < A.E) map.load(up, ld, A.E, r, (at + step) * kBlock, 0);
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
+      if (base && m + 1 < MW) load_base(m + 1, y[(m + 1) & 1]);
+      typename H::Factor hi[H::kBlocks], lo[H::kBlocks];
+      const int row = m0 + 16 * m + col;
+#pragma unroll
+      for (int k = 0; k < H::kBlocks; ++k) {
+        auto read = [&](int part, int i) {
+          return __builtin_bit_cast(typename H::Factor,
+                                    *reinterpret_cast<const u32x4*>(&lds.hidden[part][row][i]));
+        };
+        if constexpr (H::kWide) {
+          hi[k] = read(0, 16 * k + 4 * quarter);
+        } else if constexpr (H::kBoth) {
+          hi[k] = read(quarter >> 1, 8 * (quarter & 1));
+        } else {
+          hi[k] = read(0, 32 * k + 8 * quarter);
+          lo[k] = read(1, 32 * k + 8 * quarter);
+        }
+      }
+      f32x4 acc[N];
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        acc[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < H::kBlocks; ++k)
+          mma_hidden<T, RT>(acc[t], hi[k], lo[k],
+                            __builtin_bit_cast(vec_t<T>, stage[place(N * col + t, H::chunk(k, quarter))]));
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < 4; ++i) {
+        const int n = lds.rows[m0 + 16 * m + 4 * quarter + i];
+        if (m0 + 16 * m + 4 * quarter + i >= count || n < 0) continue;
+        T z[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+          const float f = acc[t][i] * A.f_out;
+          z[t] = static_cast<T>(base ? to_float(y[m & 1][i][t]) + f : f);
+        }
+        store_n<N, T, Whole>(out + (int64_t)n * A.E, e, A.E, z);
+      }
+    }
+    wavefront_sync();
+  }
+}
+
+// A tile of rows without a code: base, or zeros; NaN for codes out of range.  ids:
+// the rows in LDS, those with codes out of range at -2 - row.
+template <typename T, bool Whole>
+__device__ __forceinline__ void rows_without_code(const RowsArgs& A, const int* ids, int count,
+                                                  int part, int parts) {
+  constexpr int V = kVec<T>, kAhead = 4;
+  const T* base = static_cast<const T*>(A.base);
+  T* out = static_cast<T*>(A.out);
+  const int vecs = (A.E + V - 1) / V, all = count * vecs, step = kThreads * parts;
+  for (int i0 = kThreads * part + threadIdx.x; i0 < all; i0 += step * kAhead) {
+    vec_t<T> y[kAhead];
+    int n[kAhead], e[kAhead];
+    bool bad[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u * step, all - 1), m = i / vecs;
+      e[u] = (i - m * vecs) * V;
+      n[u] = ids[m];
+      bad[u] = n[u] < -1;
+      if (bad[u]) n[u] = -2 - n[u];
+      if (base) y[u] = load_whole<T, Whole>(base + (int64_t)max(n[u], 0) * A.E, e[u], A.E);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (!base || bad[u])
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[u][v] = static_cast<T>(bad[u] ? __builtin_nanf("") : 0.0f);
+      if (n[u] >= 0) store_part<T, Whole>(out + (int64_t)n[u] * A.E, e[u], A.E, y[u]);
+    }
+  }
+}
+
+// Phase 1: hidden values, over part blockIdx.y of D, left in `parts`; 2: results
+// from them, over part blockIdx.y of E; 3: both.  Whole: D, E and r are whole
+// vectors.
+template <typename T, int MT, int RT, int Phase, bool Turned, bool Whole>
+__global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParams P, RowsArgs A,
+                                                                    Slots S) {
+  using L = RowsLds<T, MT, RT>;
+  using H = Hidden<T, RT>;
+  constexpr int V = kVec<T>, M = L::M, R = L::R;
+  __shared__ L lds;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int col = lane & 15, quarter = lane >> 4;
+  // (the last first: those without a code have the most to wait for)
+  const Tile t = tile_at(P, S, S.begin + gridDim.x - 1 - xcd_remap(blockIdx.x, gridDim.x));
+  if (t.count == 0) return;
+  const bool none = t.code >= P.K;
+  if (none && (Phase == 1 || A.out == nullptr)) return;
+  if (threadIdx.x < M) {
+    const int64_t j = t.first + min((int)threadIdx.x, t.count - 1);
+    int n = row_at(P, j);
+    if (none && n >= 0) {
+      const int i = P.order[j];
+      if (i < 0 || i >= P.rows || P.places[i] != kNoCode) n = -2 - n;
+    }
+    lds.rows[threadIdx.x] = n;
+  }
+  __syncthreads();
+  const int parts = Phase == 3 ? 1 : gridDim.y, part = Phase == 3 ? 0 : blockIdx.y;
+  if (none) {
+    rows_without_code<T, Whole>(A, lds.rows, t.count, part, parts);
+    return;
+  }
+
+  // Rows of four chunks and more go over the wavefronts by chunks, whose sums meet;
+  // shorter ones by tiles.
+  const bool by_rows = MT > 1 && A.D <= 3 * 8 * V;
+  if constexpr (Phase & 1) {
+    const T* down = static_cast<const T*>(A.down) + t.code * P.r * A.D;
+    if (by_rows) {
+      f32x4 acc[1][RT];
+#pragma unroll
+      for (int k = 0; k < RT; ++k) acc[0][k] = f32x4{0, 0, 0, 0};
+      if (w < MT)
+        first_product<T, 1, RT, Turned, Whole>(acc, A, P.r, down, lds.stage[w], lds.rows + 16 * w, 0, 1);
+      __syncthreads();
+      if (w < MT)
+#pragma unroll
+        for (int k = 0; k < RT; ++k)
+          *reinterpret_cast<f32x4*>(&lds.red[0][16 * w + col][16 * k + 4 * quarter]) = acc[0][k];
+      __syncthreads();
+    } else {
+      f32x4 acc[MT][RT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) acc[m][k] = f32x4{0, 0, 0, 0};
+      first_product<T, MT, RT, Turned, Whole>(acc, A, P.r, down, lds.stage[w], lds.rows, w + 4 * part,
+                                              4 * parts);
+      __syncthreads();
+      // Wavefronts 2 and 3's sums to 0 and 1's, whose two are added where they are read.
+      auto at = [&](int which, int m, int k) {
+        return reinterpret_cast<f32x4*>(&lds.red[which][16 * m + col][16 * k + 4 * quarter]);
+      };
+      if (w >= 2)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int k = 0; k < RT; ++k) mma<T>(acc[m][k], a[u][k], b[u][m]);
+          for (int k = 0; k < RT; ++k) *at(w - 2, m, k) = acc[m][k];
+      __syncthreads();
+      if (w < 2)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int k = 0; k < RT; ++k) *at(w, m, k) += acc[m][k];
+      __syncthreads();
     }
-    for (; s * kStep < A.D; s += turn) {
-      const int at = s * kStep + quarter * V;
-      vec_t<T> a[RT], b[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) b[m] = load_part(x[m], at, A.D, static_cast<T>(0.0f));
-#pragma unroll
-      for (int k = 0; k < RT; ++k) a[k] = load_part(d[k], at, A.D, static_cast<T>(0.0f));
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int k = 0; k < RT; ++k) mma<T>(acc[m][k], a[k], b[m]);
-    }
-    // The wavefronts' sums: 2 and 3 to 0 and 1, whose two are added where they are read.
-    auto at = [&](int which, int m, int k) {
-      return reinterpret_cast<f32x4*>(&red[which][16 * m + col][16 * k + 4 * quarter]);
-    };
-    if (w >= 2)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int k = 0; k < RT; ++k) *at(w - 2, m, k) = acc[m][k];
-    __syncthreads();
-    if (w < 2)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int k = 0; k < RT; ++k) *at(w, m, k) += acc[m][k];
-    __syncthreads();
   }
   // Hidden values: summed, kept, and as the next product's factor.
   for (int i = threadIdx.x; i < M * R; i += kThreads) {
@@ -304,11 +600,12 @@ __global__ __launch_bounds__(kThreads) void adapters_rows_kernel(AdapterParams P
       if constexpr (Phase == 2) {
         for (int p = 0; p < A.splits; ++p) h += A.parts[p * P.rows * P.r + at];
         h *= A.f_hidden;
-        if (A.hidden && blockIdx.y == 0) A.hidden[at] = h;
+        if (A.hidden && part == 0) A.hidden[at] = h;
       } else {
-        h = red[0][m][k] + red[1][m][k];
+        h = lds.red[0][m][k];
+        if (!by_rows) h += lds.red[1][m][k];
         if constexpr (Phase == 1) {
-          A.parts[blockIdx.y * P.rows * P.r + at] = h;
+          A.parts[part * P.rows * P.r + at] = h;
         } else {
           h *= A.f_hidden;
           if (A.hidden) A.hidden[at] = h;
@@ -317,102 +614,28 @@ __global__ __launch_bounds__(kThreads) void adapters_rows_kernel(AdapterParams P
     }
     if constexpr (Phase != 1) {
       if constexpr (H::kWide) {
-        red[0][m][k] = h;
+        lds.hidden[0][m][k] = h;
       } else {
         uint32_t hi;
         float lo;
         split(h, hi, lo);
-        parts16[0][m][k] = (uint16_t)hi;
-        parts16[1][m][k] = (uint16_t)bf16_bits(lo);
+        lds.hidden[0][m][k] = (uint16_t)hi;
+        lds.hidden[1][m][k] = (uint16_t)bf16_bits(lo);
       }
     }
   }
   if constexpr (Phase != 1) {
     if (A.out == nullptr) return;
     __syncthreads();
-    typename H::Factor hi[MT][H::kBlocks], lo[MT][H::kBlocks];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int k = 0; k < H::kBlocks; ++k) {
-        const int row = 16 * m + col;
-        if constexpr (H::kWide) {
-          hi[m][k] = load_vec(&red[0][row][16 * k + 4 * quarter]);
-        } else if constexpr (H::kBoth) {
-          hi[m][k] = __builtin_bit_cast(
-              bf16x8, *reinterpret_cast<const u32x4*>(&parts16[quarter >> 1][row][8 * (quarter & 1)]));
-        } else {
-          hi[m][k] = __builtin_bit_cast(
-              bf16x8, *reinterpret_cast<const u32x4*>(&parts16[0][row][32 * k + 8 * quarter]));
-          lo[m][k] = __builtin_bit_cast(
-              bf16x8, *reinterpret_cast<const u32x4*>(&parts16[1][row][32 * k + 8 * quarter]));
-        }
-      }
-    // 32 columns at a time: lane l's results are columns 8 (l / 16) + 0..7 of row
-    // l % 16, four of either of two tiles.
     const T* up = static_cast<const T*>(A.up) + t.code * P.r * A.E;
-    const T* base = static_cast<const T*>(A.base);
-    T* out = static_cast<T*>(A.out);
-    const int turn = 128 * (Phase == 2 ? gridDim.y : 1);
-    for (int c0 = 32 * (w + 4 * (Phase == 2 ? blockIdx.y : 0)); c0 < A.E; c0 += turn) {
-      f32x4 acc[MT][2];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int e = min(c0 + 8 * (col >> 2) + 4 * v + (col & 3), A.E - 1);
-        const T* row = up + (int64_t)e * P.r;
-#pragma unroll
-        for (int k = 0; k < H::kBlocks; ++k) {
-          const int rank = H::kWide ? 16 * k + 4 * quarter
-                                    : H::kBoth ? 8 * (quarter & 1) : 32 * k + 8 * quarter;
-          const vec_t<T> u = load_part(row, rank, P.r, static_cast<T>(0.0f));
-#pragma unroll
-          for (int m = 0; m < MT; ++m) mma_hidden<T, RT>(acc[m][v], u, hi[m][k], lo[m][k]);
-        }
-      }
-      const int e = c0 + 8 * quarter;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (16 * m + col >= t.count || n[m] < 0) continue;
-        T* to = out + (int64_t)n[m] * A.E;
-        const T* from = base + (int64_t)n[m] * A.E;
-#pragma unroll
-        for (int v = 0; v < 8 / V; ++v) {
-          const int first = e + v * V;
-          vec_t<T> y;
-          if (base) y = load_part(from, first, A.E, static_cast<T>(0.0f));
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int q = v * V + i;
-            const float z = acc[m][q / 4][q % 4] * A.f_out;
-            y[i] = static_cast<T>(base ? to_float(y[i]) + z : z);
-          }
-          store_part(to, first, A.E, y);
-        }
-      }
+    if (MT > 1 && A.E <= 3 * 16 * L::kCols) {
+      if (w < MT)
+        second_product<T, MT, RT, 1, Turned, Whole>(A, P.r, up, lds, lds.stage[w], 16 * w, t.count, 0, 1);
+    } else {
+      second_product<T, MT, RT, MT, Turned, Whole>(A, P.r, up, lds, lds.stage[w], 0, t.count,
+                                                   w + 4 * part, 4 * parts);
     }
   }
-}
-
-// Maps transposed, [K][a][b] -> [K][b][a], of the codes that have places.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void adapters_transpose_kernel(
-    AdapterParams P, const T* __restrict__ from, T* __restrict__ to, int a, int b,
-    int64_t first_code) {
-  __shared__ T tile[32][34];
-  const int64_t across = (b + 31) / 32, down = (a + 31) / 32, tiles = across * down;
-  const int64_t i = blockIdx.x % tiles, k = first_code + blockIdx.x / tiles;
-  if (start_of(P, k) >= start_of(P, k + 1)) return;
-  const int a0 = (int)(i / across) * 32, b0 = (int)(i % across) * 32;
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  from += k * a * b;
-  to += k * a * b;
-  for (int v = y; v < 32; v += 8)
-    if (a0 + v < a && b0 + x < b) tile[v][x] = from[(int64_t)(a0 + v) * b + b0 + x];
-  __syncthreads();
-  for (int v = y; v < 32; v += 8)
-    if (b0 + v < b && a0 + x < a) to[(int64_t)(b0 + v) * a + a0 + x] = tile[x][v];
 }
 
 // ---- gradients of the maps
@@ -435,7 +658,7 @@ __device__ __forceinline__ int64_t sums_at(int64_t start, int64_t index, int L) 
   return 2 * start / L + index;
 }
 
-template <typename T, int RT>
+template <typename T, int RT, bool Whole>
 __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P, MapsArgs A,
                                                                  Slots S) {
   constexpr int V = kVec<T>, W = 16 * V, R = 16 * RT;
@@ -472,7 +695,7 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
         const int64_t j = j0 + 4 * u + quarter, safe = min(j, end - 1);
         const int n = row_at(P, safe);
         const bool in = j < end && n >= 0;
-        x[u] = load_part(rows + (int64_t)max(n, 0) * stride, d, width, 0.0f);
+        x[u] = load_whole<T, Whole>(rows + (int64_t)max(n, 0) * stride, d, width);
         if (!in) x[u] = vec_t<T>{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
@@ -493,7 +716,7 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
     // A step is 32 places: a lane's eight rows, places 8 quarter + 0..7, turned
     // into eight columns' values.
     for (int64_t j0 = t.first + 32 * w; j0 < end; j0 += 128) {
-      u32x4 x[8];
+      vec_t<T> x[8];
       bool in[8];
       int64_t safe[8];
 #pragma unroll
@@ -502,9 +725,8 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
         safe[q] = min(j, end - 1);
         const int n = row_at(P, safe[q]);
         in[q] = j < end && n >= 0;
-        x[q] = __builtin_bit_cast(
-            u32x4, load_part(rows + (int64_t)max(n, 0) * stride, d, width, static_cast<T>(0.0f)));
-        if (!in[q]) x[q] = u32x4{0, 0, 0, 0};
+        x[q] = load_whole<T, Whole>(rows + (int64_t)max(n, 0) * stride, d, width);
+        if (!in[q]) x[q] = vec_t<T>{};
       }
       bf16x8 hi[RT], lo[RT];
 #pragma unroll
@@ -516,15 +738,11 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
           h[q] = in[q] && rank < P.r ? hidden[safe[q] * P.r + rank] : 0.0f;
         split8(h, hi[k], lo[k]);
       }
+      turn<T>(x);
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
-        u32x4 y;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-          y[p] = __builtin_amdgcn_perm(x[2 * p + 1][v / 2], x[2 * p][v / 2],
-                                       v % 2 ? 0x07060302u : 0x05040100u);
         bf16x8 big, small;
-        parts<T>(__builtin_bit_cast(vec_t<T>, y), big, small);
+        parts<T>(x[v], big, small);
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
           mma<__bf16>(acc[k][v], hi[k], big);
@@ -613,51 +831,51 @@ RowsPlan rows_plan(const AdapterParams& P, int D, int E) {
 }
 bool is_split(const RowsPlan& L) { return L.splits_down > 1 || L.splits_up > 1; }
 
-template <typename T, int MT, int RT, int Phase>
+template <typename T, int MT, int RT, int Phase, bool Turned, bool Whole>
 int launch_rows(const AdapterParams& P, const RowsArgs& A, int parts, hipStream_t stream) {
   Slots S{16 * MT, by_place(P, 16 * MT), 0};
   return in_launches(slots_of(P, S.M, S.by_place), kMostBlocks, [&](int64_t first, int64_t n) {
     S.begin = first;
-    launch_traced("adapters_rows_kernel", (adapters_rows_kernel<T, MT, RT, Phase>),
+    launch_traced("adapters_rows_kernel", (adapters_rows_kernel<T, MT, RT, Phase, Turned, Whole>),
                   dim3((unsigned)n, parts), dim3(kThreads), 0, stream, P, A, S);
     return check_launch("adapters_rows_kernel");
   });
 }
 
-template <typename T>
+template <typename T, int RT, bool Turned, bool Whole>
+int rows_of_rank(const AdapterParams& P, RowsArgs A, const RowsPlan& L, hipStream_t stream) {
+  if (is_split(L)) {
+    const int rc = launch_rows<T, 1, RT, 1, Turned, Whole>(P, A, L.splits_down, stream);
+    return rc ? rc : launch_rows<T, 1, RT, 2, Turned, Whole>(P, A, A.out ? L.splits_up : 1, stream);
+  }
+  if (L.row_tiles == 1) return launch_rows<T, 1, RT, 3, Turned, Whole>(P, A, 1, stream);
+  return launch_rows<T, RT == 8 ? 2 : 4, RT, 3, Turned, Whole>(P, A, 1, stream);
+}
+
+template <typename T, bool Turned>
 int rows_of(const AdapterParams& P, RowsArgs A, float* parts, hipStream_t stream) {
   const RowsPlan L = rows_plan(P, A.D, A.E);
-  const int rt = rank_tiles(P.r);
-  if (is_split(L)) {
-    A.parts = parts;
-    A.splits = L.splits_down;
-#define GS_SPLIT(RT)                                                                   \
-  if (rt == RT) {                                                                      \
-    const int rc = launch_rows<T, 1, RT, 1>(P, A, L.splits_down, stream);              \
-    return rc ? rc : launch_rows<T, 1, RT, 2>(P, A, A.out ? L.splits_up : 1, stream);  \
+  A.parts = parts;
+  A.splits = L.splits_down;
+  const bool whole = A.D % kVec<T> == 0 && A.E % kVec<T> == 0 && P.r % kVec<T> == 0;
+  switch (rank_tiles(P.r)) {
+#define GS_RANK(RT)                                                           \
+  case RT:                                                                    \
+    return whole ? rows_of_rank<T, RT, Turned, true>(P, A, L, stream)         \
+                 : rows_of_rank<T, RT, Turned, false>(P, A, L, stream);
+    GS_RANK(1) GS_RANK(2) GS_RANK(4)
+    default: GS_RANK(8)
+#undef GS_RANK
   }
-    GS_SPLIT(1) GS_SPLIT(2) GS_SPLIT(4) GS_SPLIT(8)
-#undef GS_SPLIT
-  }
-  if (L.row_tiles == 1) {
-    if (rt == 1) return launch_rows<T, 1, 1, 3>(P, A, 1, stream);
-    if (rt == 2) return launch_rows<T, 1, 2, 3>(P, A, 1, stream);
-    if (rt == 4) return launch_rows<T, 1, 4, 3>(P, A, 1, stream);
-    return launch_rows<T, 1, 8, 3>(P, A, 1, stream);
-  }
-  if (rt == 1) return launch_rows<T, 4, 1, 3>(P, A, 1, stream);
-  if (rt == 2) return launch_rows<T, 4, 2, 3>(P, A, 1, stream);
-  if (rt == 4) return launch_rows<T, 4, 4, 3>(P, A, 1, stream);
-  return launch_rows<T, 2, 8, 3>(P, A, 1, stream);
 }
 
 template <typename T>
 int forward_of(const AdapterParams& P, const void* rows, const void* down,
                const void* up, const void* base, void* out, float* hidden,
                void* workspace, hipStream_t stream) {
-  return rows_of<T>(P, RowsArgs{rows, P.stride, P.D, P.E, down, up, base, 1.0f, P.scale, out,
-                                hidden, nullptr, 0},
-                    static_cast<float*>(workspace), stream);
+  return rows_of<T, false>(P, RowsArgs{rows, P.stride, P.D, P.E, down, up, base, 1.0f, P.scale, out,
+                                       hidden, nullptr, 0},
+                           static_cast<float*>(workspace), stream);
 }
 
 // Places of a chunk: enough workgroups for the card, and sums that are few beside
@@ -670,7 +888,7 @@ int chunk_of(const AdapterParams& P, int dtype_bytes) {
 }
 
 struct BackwardLayout {
-  size_t dh, parts, down_t, up_t, sums[2], total;
+  size_t dh, parts, sums[2], total;
   int chunk;
 };
 BackwardLayout backward_layout(const AdapterParams& P) {
@@ -686,8 +904,6 @@ BackwardLayout backward_layout(const AdapterParams& P) {
   L.dh = take((size_t)P.rows * P.r * 4);
   const RowsPlan R = rows_plan(P, P.E, P.D);
   L.parts = take(is_split(R) ? (size_t)R.splits_down * P.rows * P.r * 4 : 0);
-  L.down_t = take((size_t)P.K * P.r * P.D * bytes);
-  L.up_t = take((size_t)P.K * P.r * P.E * bytes);
   if (P.rows > L.chunk) {
     const size_t n = (size_t)(2 * P.rows / L.chunk + 2) * P.r * 4;
     L.sums[0] = take(n * P.D);
@@ -695,18 +911,6 @@ BackwardLayout backward_layout(const AdapterParams& P) {
   }
   L.total = off;
   return L;
-}
-
-template <typename T>
-int transpose(const AdapterParams& P, const void* from, void* to, int a, int b,
-              hipStream_t stream) {
-  const int64_t tiles = (int64_t)((a + 31) / 32) * ((b + 31) / 32);
-  return in_launches(P.K, kMostBlocks / tiles, [&](int64_t first, int64_t codes) {
-    launch_traced("adapters_transpose_kernel", (adapters_transpose_kernel<T>),
-                  dim3((unsigned)(tiles * codes)), dim3(kThreads), 0, stream, P,
-                  static_cast<const T*>(from), static_cast<T*>(to), a, b, first);
-    return check_launch("adapters_transpose_kernel");
-  });
 }
 
 template <typename T>
@@ -719,11 +923,9 @@ int backward_of(const AdapterParams& P, const void* grad, const void* rows,
   auto* dh = reinterpret_cast<float*>(ws + L.dh);
   int rc = GSPLAT_OK;
   if ((g_rows || g_down) && P.rows > 0) {
-    if ((rc = transpose<T>(P, up, ws + L.up_t, P.E, P.r, stream))) return rc;
-    if (g_rows && (rc = transpose<T>(P, down, ws + L.down_t, P.r, P.D, stream))) return rc;
-    rc = rows_of<T>(P, RowsArgs{grad, P.E, P.E, P.D, ws + L.up_t, ws + L.down_t, nullptr, P.scale,
-                                1.0f, g_rows, dh, nullptr, 0},
-                    reinterpret_cast<float*>(ws + L.parts), stream);
+    rc = rows_of<T, true>(P, RowsArgs{grad, P.E, P.E, P.D, up, down, nullptr, P.scale, 1.0f, g_rows,
+                                      dh, nullptr, 0},
+                          reinterpret_cast<float*>(ws + L.parts), stream);
     if (rc) return rc;
   }
   if (!g_down && !g_up) return rc;
@@ -734,6 +936,7 @@ int backward_of(const AdapterParams& P, const void* grad, const void* rows,
                    {reinterpret_cast<float*>(ws + L.sums[0]), reinterpret_cast<float*>(ws + L.sums[1])},
                    {g_down ? (P.D + W - 1) / W : 0, g_up ? (P.E + W - 1) / W : 0},
                    rank_tiles(P.r) == 8 ? 2 : 1};
+  const bool whole = P.D % kVec<T> == 0 && P.E % kVec<T> == 0;
   Slots S{L.chunk, false, 0};
   const int64_t slots = P.rows / L.chunk + P.K;
   const int per_slot = (A.blocks[0] + A.blocks[1]) * A.rank_blocks;
@@ -742,8 +945,9 @@ int backward_of(const AdapterParams& P, const void* grad, const void* rows,
     const dim3 grid((unsigned)(n * per_slot));
 #define GS_MAPS(RT)                                                                     \
   if (rt == RT)                                                                         \
-    launch_traced("adapters_maps_kernel", (adapters_maps_kernel<T, RT>), grid,          \
-                  dim3(kThreads), 0, stream, P, A, S);
+    launch_traced("adapters_maps_kernel",                                               \
+                  whole ? adapters_maps_kernel<T, RT, true> : adapters_maps_kernel<T, RT, false>, \
+                  grid, dim3(kThreads), 0, stream, P, A, S);
     GS_MAPS(1) GS_MAPS(2) GS_MAPS(4)
 #undef GS_MAPS
     return check_launch("adapters_maps_kernel");
