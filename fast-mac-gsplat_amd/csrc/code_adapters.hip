@@ -156,33 +156,23 @@ __device__ __forceinline__ void parts(vec_t<T> x, bf16x8& hi, bf16x8& lo) {
   }
 }
 
-// Values i .. i + kVec - 1 of a row of n, zeros past its end.  Whole: n is a multiple
-// of kVec, so that a vector is in the row or past it.  (Nothing branches then:
-// with a branch around each load the compiler waits for one before the next.)
+// Values i .. i + kVec - 1 of a row of n as one load, and later brought to their
+// place, zeros past the row's end (Whole: n is a multiple of kVec).  Apart, since a
+// value that is looked at as it is loaded, or loaded behind a branch, is waited
+// for: the loads after it would start only then.
 template <typename T, bool Whole>
-__device__ __forceinline__ vec_t<T> load_whole(const T* row, int i, int n) {
-  if constexpr (Whole) {
-    vec_t<T> v = load_vec(row + min(i, n - kVec<T>));
-    if (i >= n)
-#pragma unroll
-      for (int q = 0; q < kVec<T>; ++q) v[q] = static_cast<T>(0.0f);
-    return v;
-  } else {
-    return load_part(row, i, n, static_cast<T>(0.0f));
-  }
+__device__ __forceinline__ vec_t<T> load_raw(const T* row, int i, int n) {
+  if (Whole || n >= kVec<T>) return load_vec(row + min(i, n - kVec<T>));
+  return load_part(row, i, n, static_cast<T>(0.0f));
+}
+template <typename T, bool Whole>
+__device__ __forceinline__ void bring(vec_t<T>& v, int i, int n) {
+  vec_t<T> x[1] = {v};
+  fix_row<T, 1, Whole>(x, i, 0, n, static_cast<T>(0.0f));
+  v = i < n ? x[0] : vec_t<T>{};
 }
 
-// N adjacent values of a row of n from i on, zeros past its end.  Whole: n is a
-// multiple of N.
-template <int N, typename T, bool Whole>
-__device__ __forceinline__ void load_n(T (&v)[N], const T* row, int i, int n) {
-  if (Whole || i + N <= n) {
-    __builtin_memcpy(v, row + (Whole ? min(i, n - N) : i), sizeof(v));
-    return;
-  }
-#pragma unroll
-  for (int q = 0; q < N; ++q) v[q] = i + q < n ? row[i + q] : static_cast<T>(0.0f);
-}
+// N adjacent values of a row of n from i on.  (Whole: n is a multiple of N.)
 template <int N, typename T, bool Whole>
 __device__ __forceinline__ void store_n(T* row, int i, int n, const T (&v)[N]) {
   if (Whole ? i < n : i + N <= n) {
@@ -258,21 +248,37 @@ struct MapChunks {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const T* at = map + (int64_t)min(k + j, depth - 1) * ld;
-          v[u][j] = Whole ? load_vec(at + min(row, rows - V))
-                          : load_part(at, row, rows, static_cast<T>(0.0f));
-          if (k + j >= depth)
-#pragma unroll
-            for (int q = 0; q < V; ++q) v[u][j][q] = static_cast<T>(0.0f);
+          v[u][j] = load_raw<T, Whole>(at, row, rows);
         }
       } else {
         const int row = row0 + task / kChunks, k = k0 + task % kChunks * V;
-        v[u][0] = load_whole<T, Whole>(map + (int64_t)min(row, rows - 1) * ld, k, depth);
+        v[u][0] = load_raw<T, Whole>(map + (int64_t)min(row, rows - 1) * ld, k, depth);
+      }
+    }
+  }
+  // What lies past the ends, zeros past the depth.
+  __device__ __forceinline__ void finish(int rows, int depth, int row0, int k0) {
+    if (k0 + kChunks * V <= depth && (!Turned || Whole || row0 + kRows <= rows)) return;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int task = u * 64 + lane;
+      if constexpr (Turned) {
+        const int row = row0 + task % (kRows / V) * V, k = k0 + task / (kRows / V) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (!Whole) bring<T, false>(v[u][j], row, rows);
+          if (k + j >= depth) v[u][j] = vec_t<T>{};
+        }
+      } else {
+        bring<T, Whole>(v[u][0], k0 + task % kChunks * V, depth);
       }
     }
   }
   // place(row, chunk): where it lies
   template <typename Place>
-  __device__ __forceinline__ void store(u32x4* lds, Place place) {
+  __device__ __forceinline__ void store(u32x4* lds, Place place, int rows, int depth, int row0, int k0) {
+    finish(rows, depth, row0, k0);
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
@@ -374,16 +380,19 @@ __device__ __forceinline__ void first_product(f32x4 (&acc)[MW][RT], const RowsAr
   const int ld = Turned ? r : A.D;
   auto load = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < 2 * MW; ++i) v[i] = load_whole<T, Whole>(x[i], at * kChunk + c * V, A.D);
+    for (int i = 0; i < 2 * MW; ++i) v[i] = load_raw<T, Whole>(x[i], at * kChunk + c * V, A.D);
     map.load(down, ld, r, A.D, 0, at * kChunk);
   };
   int at = first;
   if (at * kChunk < A.D) load(at);
   for (; at * kChunk < A.D; at += step) {
+    if ((at + 1) * kChunk > A.D)
+#pragma unroll
+      for (int i = 0; i < 2 * MW; ++i) bring<T, Whole>(v[i], at * kChunk + c * V, A.D);
 #pragma unroll
     for (int i = 0; i < 2 * MW; ++i)
       rows_at[swizzled<8>(8 * i + row, c)] = __builtin_bit_cast(u32x4, v[i]);
-    map.store(map_at, swizzled<8>);
+    map.store(map_at, swizzled<8>, r, A.D, 0, at * kChunk);
     wavefront_sync();
     if ((at + step) * kChunk < A.D) load(at + step);  // (on its way during the products)
 #pragma unroll
@@ -414,8 +423,11 @@ __device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T
   using H = Hidden<T, RT>;
   constexpr int N = L::kCols, kBlock = 16 * N;
   const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-  const T* base = static_cast<const T*>(A.base);
+  const T* base = Turned ? nullptr : static_cast<const T*>(A.base);  // (no gradient has one)
   T* out = static_cast<T*>(A.out);
+  // (what is read without a base is a row of `out`, unused: no branch)
+  const T* from = base ? base : out;
+  const int64_t from_row = base ? A.E : 0;
   const int ld = Turned ? A.E : r;
   auto place = [](int row, int chunk) {
     const int n = row / N, t = row % N;
@@ -426,19 +438,25 @@ __device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T
   for (int at = first; at * kBlock < A.E; at += step) {
     const int e = at * kBlock + N * col;
     T y[2][4][N];
-    auto load_base = [&](int m, T (&to)[4][N]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        load_n<N, T, Whole>(to[i], base + (int64_t)max(lds.rows[m0 + 16 * m + 4 * quarter + i], 0) * A.E,
-                            e, A.E);
+    // (a last block that is not whole takes its values one by one, where they are used)
+    const bool cut = !Whole && (at + 1) * kBlock > A.E;
+    auto base_row = [&](int m, int i) {
+      return from + max(lds.rows[m0 + 16 * m + 4 * quarter + i], 0) * from_row;
     };
-    if (base) load_base(0, y[0]);
-    map.store(stage, place);
+    auto load_base = [&](int m, T (&to)[4][N]) {
+      if constexpr (Turned) return;
+      if (Whole || (base && !cut))
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_memcpy(to[i], base_row(m, i) + min(e, A.E - N), sizeof(to[i]));
+    };
+    load_base(0, y[0]);
+    map.store(stage, place, A.E, r, at * kBlock, 0);
     wavefront_sync();
     if ((at + step) * kBlock < A.E) map.load(up, ld, A.E, r, (at + step) * kBlock, 0);
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
-      if (base && m + 1 < MW) load_base(m + 1, y[(m + 1) & 1]);
+      if (m + 1 < MW) load_base(m + 1, y[(m + 1) & 1]);
       typename H::Factor hi[H::kBlocks], lo[H::kBlocks];
       const int row = m0 + 16 * m + col;
 #pragma unroll
@@ -470,6 +488,9 @@ __device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T
         const int n = lds.rows[m0 + 16 * m + 4 * quarter + i];
         if (m0 + 16 * m + 4 * quarter + i >= count || n < 0) continue;
         T z[N];
+        if (cut && base)
+#pragma unroll
+          for (int t = 0; t < N; ++t) y[m & 1][i][t] = base_row(m, i)[min(e + t, A.E - 1)];
 #pragma unroll
         for (int t = 0; t < N; ++t) {
           const float f = acc[t][i] * A.f_out;
@@ -502,10 +523,11 @@ __device__ __forceinline__ void rows_without_code(const RowsArgs& A, const int* 
       n[u] = ids[m];
       bad[u] = n[u] < -1;
       if (bad[u]) n[u] = -2 - n[u];
-      if (base) y[u] = load_whole<T, Whole>(base + (int64_t)max(n[u], 0) * A.E, e[u], A.E);
+      if (base) y[u] = load_raw<T, Whole>(base + (int64_t)max(n[u], 0) * A.E, e[u], A.E);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
+      if (base && !Whole) bring<T, false>(y[u], e[u], A.E);
       if (!base || bad[u])
 #pragma unroll
         for (int v = 0; v < V; ++v) y[u][v] = static_cast<T>(bad[u] ? __builtin_nanf("") : 0.0f);
@@ -658,16 +680,18 @@ __device__ __forceinline__ int64_t sums_at(int64_t start, int64_t index, int L) 
   return 2 * start / L + index;
 }
 
-template <typename T, int RT, bool Whole>
-__global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P, MapsArgs A,
+template <typename T, int RT, bool Whole, int Waves>
+__global__ __launch_bounds__(64 * Waves) void adapters_maps_kernel(AdapterParams P, MapsArgs A,
                                                                  Slots S) {
   constexpr int V = kVec<T>, W = 16 * V, R = 16 * RT;
-  __shared__ __attribute__((aligned(16))) float red[R][W + 4];
+  __shared__ __attribute__((aligned(16))) float red[Waves == 1 ? 1 : 2][R][W + 4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int col = lane & 15, quarter = lane >> 4;
   const int per_slot = (A.blocks[0] + A.blocks[1]) * A.rank_blocks;
-  const int64_t slot = S.begin + blockIdx.x / per_slot;
-  int at = (int)(blockIdx.x % per_slot);
+  // (a slot's blocks on one XCD: all of them read its hidden values)
+  const int block = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t slot = S.begin + block / per_slot;
+  int at = block % per_slot;
   const int r0 = at % A.rank_blocks * R;
   at /= A.rank_blocks;
   const int which = at < A.blocks[0] ? 0 : 1;
@@ -683,66 +707,88 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
   for (int k = 0; k < RT; ++k)
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[k][v] = f32x4{0, 0, 0, 0};
-  const int d = c0 + V * col;
-  const int64_t end = t.first + t.count;
-  if constexpr (sizeof(T) == 4) {
-    // A step is 16 places, four a product: place 4 u + quarter.
-    for (int64_t j0 = t.first + 16 * w; j0 < end; j0 += 64) {
-      vec_t<T> x[4];
-      float h[4][RT];
+  const int d = c0 + V * col, end = t.count;  // (places from the tile's first on)
+  // A step has kRows places; a lane has kVec of them, each 16 bytes of a row and the
+  // hidden values of a rank.  The next step's rows and the places after that are
+  // loaded during this step's products.
+  constexpr int kRows = 4 * V;
+  auto place = [&](int j0, int q) { return sizeof(T) == 4 ? j0 + 4 * q + quarter : j0 + 8 * quarter + q; };
+  int n[V];
+  vec_t<T> x[V];
+  float h[RT][V];
+  auto ids = [&](int j0) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t j = j0 + 4 * u + quarter, safe = min(j, end - 1);
-        const int n = row_at(P, safe);
-        const bool in = j < end && n >= 0;
-        x[u] = load_whole<T, Whole>(rows + (int64_t)max(n, 0) * stride, d, width);
-        if (!in) x[u] = vec_t<T>{0, 0, 0, 0};
+    for (int q = 0; q < V; ++q) n[q] = P.order[t.first + min(place(j0, q), end - 1)];
+  };
+  // (ranks past the last make sums that nobody writes)
+  auto load = [&](int j0) {
 #pragma unroll
-        for (int k = 0; k < RT; ++k) {
-          const int rank = r0 + 16 * k + col;
-          h[u][k] = in && rank < P.r ? hidden[safe * P.r + rank] : 0.0f;
-        }
+    for (int q = 0; q < V; ++q) {
+      const int64_t at = t.first + min(place(j0, q), end - 1);
+      const int64_t row = P.by_code ? at : (uint32_t)n[q] < (uint32_t)P.rows ? n[q] : 0;
+      x[q] = load_raw<T, Whole>(rows + row * stride, d, width);
+      const float* from = hidden + at * P.r + r0;
+#pragma unroll
+      for (int k = 0; k < RT; ++k) h[k][q] = from[min(16 * k + col, P.r - 1 - r0)];
+    }
+  };
+  // What stands in for places past the tile's end.  (Only there and only now: a
+  // value that is looked at as it is loaded is waited for.)
+  auto cut = [&](int j0) {
+    if (!Whole && c0 + W > width)
+#pragma unroll
+      for (int q = 0; q < V; ++q) bring<T, false>(x[q], d, width);
+    if (j0 + kRows <= end) return;
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      if (place(j0, q) < end) continue;
+      x[q] = vec_t<T>{};
+#pragma unroll
+      for (int k = 0; k < RT; ++k) h[k][q] = 0.0f;
+    }
+  };
+  int j0 = kRows * w;
+  if (j0 < end) {
+    ids(j0);
+    load(j0);
+    ids(j0 + Waves * kRows);
+  }
+  for (; j0 < end; j0 += Waves * kRows) {
+    cut(j0);
+    if constexpr (sizeof(T) == 4) {
+      float g[RT][V];
+      vec_t<T> y[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        y[q] = x[q];
+#pragma unroll
+        for (int k = 0; k < RT; ++k) g[k][q] = h[k][q];
       }
+      load(j0 + Waves * kRows);  // (the last row again, past the end)
+      ids(j0 + 2 * Waves * kRows);
+      // (four places a product: 4 q + quarter)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int q = 0; q < V; ++q)
 #pragma unroll
         for (int k = 0; k < RT; ++k)
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            acc[k][v] =
-                __builtin_amdgcn_mfma_f32_16x16x4f32(h[u][k], x[u][v], acc[k][v], 0, 0, 0);
-    }
-  } else {
-    // A step is 32 places: a lane's eight rows, places 8 quarter + 0..7, turned
-    // into eight columns' values.
-    for (int64_t j0 = t.first + 32 * w; j0 < end; j0 += 128) {
-      vec_t<T> x[8];
-      bool in[8];
-      int64_t safe[8];
+            acc[k][v] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[k][q], y[q][v], acc[k][v], 0, 0, 0);
+    } else {
+      // (a lane's eight rows turned into eight columns' values)
+      vec_t<T> y[V];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int64_t j = j0 + 8 * quarter + q;
-        safe[q] = min(j, end - 1);
-        const int n = row_at(P, safe[q]);
-        in[q] = j < end && n >= 0;
-        x[q] = load_whole<T, Whole>(rows + (int64_t)max(n, 0) * stride, d, width);
-        if (!in[q]) x[q] = vec_t<T>{};
-      }
+      for (int q = 0; q < V; ++q) y[q] = x[q];
+      turn<T>(y);
       bf16x8 hi[RT], lo[RT];
 #pragma unroll
-      for (int k = 0; k < RT; ++k) {
-        const int rank = r0 + 16 * k + col;
-        float h[8];
+      for (int k = 0; k < RT; ++k) split8(h[k], hi[k], lo[k]);
+      load(j0 + Waves * kRows);  // (the last row again, past the end)
+      ids(j0 + 2 * Waves * kRows);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          h[q] = in[q] && rank < P.r ? hidden[safe[q] * P.r + rank] : 0.0f;
-        split8(h, hi[k], lo[k]);
-      }
-      turn<T>(x);
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
+      for (int v = 0; v < V; ++v) {
         bf16x8 big, small;
-        parts<T>(x[v], big, small);
+        parts<T>(y[v], big, small);
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
           mma<__bf16>(acc[k][v], hi[k], big);
@@ -752,34 +798,58 @@ __global__ __launch_bounds__(kThreads) void adapters_maps_kernel(AdapterParams P
       }
     }
   }
-  // The wavefronts' sums, one after another.
+  // Of four, wavefronts 2 and 3's sums to 0 and 1's, whose two are added where they
+  // are read.
+  auto red_at = [&](int half, int k, int i) { return &red[half][16 * k + 4 * quarter + i][V * col]; };
+  if (Waves == 1 || w >= 2)
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if (w == u)
+    for (int k = 0; k < RT; ++k)
 #pragma unroll
-      for (int k = 0; k < RT; ++k)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int v = 0; v < V; v += 4)
+          *reinterpret_cast<f32x4*>(red_at(Waves == 1 ? 0 : w - 2, k, i) + v) =
+              f32x4{acc[k][v][i], acc[k][v + 1][i], acc[k][v + 2][i], acc[k][v + 3][i]};
+  __syncthreads();
+  if (Waves > 1 && w < 2)
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            float& s = red[16 * k + 4 * quarter + i][V * col + v];
-            s = u == 0 ? acc[k][v][i] : s + acc[k][v][i];
-          }
-    __syncthreads();
-  }
+    for (int k = 0; k < RT; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < V; v += 4)
+          *reinterpret_cast<f32x4*>(red_at(w, k, i) + v) +=
+              f32x4{acc[k][v][i], acc[k][v + 1][i], acc[k][v + 2][i], acc[k][v + 3][i]};
+  if (Waves > 1) __syncthreads();
   const int64_t from = start_of(P, t.code), to = start_of(P, t.code + 1);
-  const int ranks = min(R, P.r - r0), cols = min(W, width - c0);
   const bool alone = to - from <= S.M;
   const int64_t values = (int64_t)P.r * width;
   T* out = static_cast<T*>(A.out[which]) + t.code * values;
   float* sums = alone ? nullptr : A.sums[which] + sums_at(from, t.index, S.M) * values;
-  for (int i = threadIdx.x; i < ranks * cols; i += kThreads) {
-    // down's gradient has the columns adjacent, up's the ranks
-    const int k = which ? i % ranks : i / cols, c = which ? i / ranks : i % cols;
-    const int64_t to_at = which ? (int64_t)(c0 + c) * P.r + r0 + k : (int64_t)(r0 + k) * width + c0 + c;
-    const float v = red[k][c] * A.factor[which];
-    if (alone) out[to_at] = static_cast<T>(v);
-    else sums[to_at] = v;
+  const float factor = A.factor[which];
+  // Down's gradient has the columns adjacent, up's the ranks: kVec of them a thread.
+  constexpr int kAcross = R / V;
+  for (int i = threadIdx.x; i < R * 16; i += 64 * Waves) {
+    const int k = which ? i % kAcross * V : i / 16, c = which ? i / kAcross : i % 16 * V;
+    if (r0 + k >= P.r || c0 + c >= width) continue;
+    float f[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int y = which ? k + v : k, x = which ? c : c + v;
+      f[v] = (Waves == 1 ? red[0][y][x] : red[0][y][x] + red[Waves > 1][y][x]) * factor;
+    }
+    const int first = which ? r0 + k : c0 + c, n = which ? P.r : width;
+    const int64_t row = (int64_t)(which ? c0 + c : r0 + k) * n;
+    if (alone) {
+      vec_t<T> z;
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = static_cast<T>(f[v]);
+      store_part(out + row, first, n, z);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (first + v < n) sums[row + first + v] = f[v];
+    }
   }
 }
 
@@ -937,19 +1007,28 @@ int backward_of(const AdapterParams& P, const void* grad, const void* rows,
                    {g_down ? (P.D + W - 1) / W : 0, g_up ? (P.E + W - 1) / W : 0},
                    rank_tiles(P.r) == 8 ? 2 : 1};
   const bool whole = P.D % kVec<T> == 0 && P.E % kVec<T> == 0;
+  // One wavefront a workgroup where that makes enough of them.
+  const bool single = std::min<int64_t>(P.rows / 64, P.K + P.rows / L.chunk) *
+                          (A.blocks[0] + A.blocks[1]) * A.rank_blocks >= 4096;
   Slots S{L.chunk, false, 0};
   const int64_t slots = P.rows / L.chunk + P.K;
   const int per_slot = (A.blocks[0] + A.blocks[1]) * A.rank_blocks;
   rc = in_launches(slots, kMostBlocks / per_slot, [&](int64_t first, int64_t n) {
     S.begin = first;
     const dim3 grid((unsigned)(n * per_slot));
-#define GS_MAPS(RT)                                                                     \
-  if (rt == RT)                                                                         \
-    launch_traced("adapters_maps_kernel",                                               \
-                  whole ? adapters_maps_kernel<T, RT, true> : adapters_maps_kernel<T, RT, false>, \
-                  grid, dim3(kThreads), 0, stream, P, A, S);
+#define GS_MAPS_OF(RT, WHOLE, WAVES)                                                      \
+  launch_traced("adapters_maps_kernel", (adapters_maps_kernel<T, RT, WHOLE, WAVES>), grid, \
+                dim3(64 * WAVES), 0, stream, P, A, S)
+#define GS_MAPS(RT)                                                    \
+  if (rt == RT) {                                                      \
+    if (whole && single) GS_MAPS_OF(RT, true, 1);                      \
+    else if (whole) GS_MAPS_OF(RT, true, 4);                           \
+    else if (single) GS_MAPS_OF(RT, false, 1);                         \
+    else GS_MAPS_OF(RT, false, 4);                                     \
+  }
     GS_MAPS(1) GS_MAPS(2) GS_MAPS(4)
 #undef GS_MAPS
+#undef GS_MAPS_OF
     return check_launch("adapters_maps_kernel");
   });
   if (rc || P.rows <= L.chunk) return rc;
