@@ -620,6 +620,7 @@ __global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParam
     if (m < t.count && k < P.r) {
       const int64_t at = (t.first + m) * P.r + k;
       if constexpr (Phase == 2) {
+#pragma unroll 8
         for (int p = 0; p < A.splits; ++p) h += A.parts[p * P.rows * P.r + at];
         h *= A.f_hidden;
         if (A.hidden && part == 0) A.hidden[at] = h;
@@ -894,8 +895,10 @@ RowsPlan rows_plan(const AdapterParams& P, int D, int E) {
   const int64_t tiles = std::min<int64_t>(P.rows, P.rows / 16 + P.K);
   if (tiles < 512 && std::max(D, E) >= 1024) {
     const int64_t most = 512 / std::max<int64_t>(tiles, 1) + 1;
-    L.splits_down = (int)std::clamp<int64_t>(D / 256, 1, most);
-    L.splits_up = (int)std::clamp<int64_t>(E / 256, 1, most);
+    // (a chunk of a row, a block of columns for each of the four wavefronts)
+    const int wide = P.dtype == GSPLAT_F32 ? 1 : 2;
+    L.splits_down = (int)std::clamp<int64_t>(D / (128 * wide), 1, most);
+    L.splits_up = (int)std::clamp<int64_t>(E / (256 * wide), 1, most);
   }
   return L;
 }

@@ -254,7 +254,7 @@ Way way_of(const GroupParams& P) {
   return Way::kRadix;
 }
 // Choices of a chunk over kThreads.
-int rounds_of(const GroupParams& P) { return P.choices <= 1 << 17 ? 4 : 16; }
+int rounds_of(const GroupParams& P) { return P.choices <= 1 << 18 ? 4 : P.choices <= 1 << 20 ? 8 : 16; }
 
 struct SortLayout {
   RadixPlan sort;
@@ -297,12 +297,17 @@ __device__ __forceinline__ int state_of(int place, int64_t rows) {
   return place == kNoCode ? kNoCode : kBadCode;
 }
 
-// The choice at place j (-1, -2: none).  The first `named` places have codes.
-__device__ __forceinline__ int64_t choice_at(int64_t j, int64_t all, int64_t named,
-                                             const int32_t* order, const int32_t* places) {
-  const int64_t i = order[j];
-  if (i < 0 || i >= all) return kBadCode;
-  return j < named ? i : places[i] == kNoCode ? kNoCode : kBadCode;
+// The choice at place j as order[j] has it: 0 a row, else kNoCode or kBadCode.  The
+// first `named` places have codes, the others are few.
+__device__ __forceinline__ int state_at(int choice, int64_t j, int64_t all, int64_t named,
+                                        const int32_t* places) {
+  if ((uint32_t)choice >= (uint32_t)all) return kBadCode;
+  if (j < named) return 0;
+  return places[choice] == kNoCode ? kNoCode : kBadCode;
+}
+// (a row, whatever the choice is)
+__device__ __forceinline__ uint32_t safe_choice(int choice, int64_t all) {
+  return (uint32_t)choice < (uint32_t)all ? choice : 0;
 }
 
 // Rows as vectors: thread t of a launch's block b has vectors b * kThreads * U +
@@ -354,25 +359,28 @@ __global__ __launch_bounds__(kThreads) void rows_by_code_kernel(
   const int64_t all = P.splats * P.choices, codes = *named;
   At at[U];
   at_of<U>(X, P.D, V, at);
-  int64_t i[U];
+  int i[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    i[u] = at[u].in ? choice_at(at[u].row, all, codes, order, places) : kNoCode;
+  for (int u = 0; u < U; ++u) i[u] = order[min(at[u].row, all - 1)];
   vec_t<T> y[U];
   float w[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t n = choices((uint32_t)max(i[u], (int64_t)0));
-    y[u] = load_at(rows + n * P.stride, at[u].d, P.D);
-    w[u] = weights ? weights[max(i[u], (int64_t)0)] : 1.0f;
+    const uint32_t choice = safe_choice(i[u], all);
+    y[u] = load_at(rows + choices(choice) * P.stride, at[u].d, P.D);
+    w[u] = 1.0f;
+    if (weights) w[u] = weights[choice];
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (!at[u].in) continue;
-    if (i[u] < 0 || weights)
+    const int state = state_at(i[u], at[u].row, all, codes, places);
+    if (weights)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        y[u][v] = static_cast<T>(i[u] < 0 ? nan_for((int)i[u]) : w[u] * to_float(y[u][v]));
+      for (int v = 0; v < V; ++v) y[u][v] = static_cast<T>(w[u] * to_float(y[u][v]));
+    if (state != 0)
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[u][v] = static_cast<T>(nan_for(state));
     store_at(out + at[u].row * P.D, at[u].d, P.D, y[u]);
   }
 }
@@ -401,14 +409,16 @@ __global__ __launch_bounds__(kThreads) void rows_from_codes_kernel(
       for (int s = 0; s < C; ++s) {
         const bool in = at[u].in && (C == 1 || s0 + s < P.choices);
         const int64_t i = in ? at[u].row * P.choices + s0 + s : 0;
-        place[u][s] = in ? places[i] : kNoCode;
-        w[u][s] = weights ? weights[i] : 1.0f;
+        place[u][s] = places[i];
+        w[u][s] = 1.0f;
+        if (weights) w[u][s] = weights[i];
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int s = 0; s < C; ++s) {
-        const int state = state_of(place[u][s], all);
+        const bool in = at[u].in && (C == 1 || s0 + s < P.choices);
+        const int state = in ? state_of(place[u][s], all) : kNoCode;
         y[u][s] = load_at(rows + (state == 0 ? place[u][s] : 0) * P.stride, at[u].d, P.D);
         place[u][s] = state;
       }
@@ -432,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void rows_from_codes_kernel(
 }
 
 // Both gradients: a team of TL lanes has a place's row, kAhead of them at a time.
-template <typename T, int TL>
+template <typename T, int TL, bool Whole>
 __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
     RowsParams P, Divide choices, int64_t begin, const T* __restrict__ grad,
     const T* __restrict__ rows, const int32_t* __restrict__ order,
@@ -442,23 +452,27 @@ __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
   const int team = threadIdx.x / TL, lane = threadIdx.x % TL;
   const int64_t all = P.splats * P.choices, codes = *named;
   const int64_t j0 = (begin + blockIdx.x) * (kTeams * kAhead) + team;
-  int64_t i[kAhead], n[kAhead];
+  int i[kAhead], state[kAhead];
+  int64_t n[kAhead];
   float w[kAhead], dot[kAhead];
 #pragma unroll
+  for (int u = 0; u < kAhead; ++u) i[u] = order[min(j0 + u * kTeams, all - 1)];
+#pragma unroll
   for (int u = 0; u < kAhead; ++u) {
-    const int64_t j = j0 + u * kTeams;
-    i[u] = j < all ? choice_at(j, all, codes, order, places) : kNoCode;
-    n[u] = choices((uint32_t)max(i[u], (int64_t)0));
-    w[u] = weights[max(i[u], (int64_t)0)];
+    const uint32_t choice = safe_choice(i[u], all);
+    n[u] = choices(choice);
+    w[u] = weights[choice];
     dot[u] = 0.0f;
   }
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) state[u] = state_at(i[u], j0 + u * kTeams, all, codes, places);
   for (int d = lane * V; d < P.D; d += TL * V) {
     vec_t<T> g[kAhead], y[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int64_t j = min(j0 + u * kTeams, all - 1);
-      g[u] = load_part(grad + n[u] * P.D, d, P.D, static_cast<T>(0.0f));
-      y[u] = load_part(rows + j * P.stride, d, P.D, static_cast<T>(0.0f));
+      g[u] = load_part<T, Whole>(grad + n[u] * P.D, d, P.D, static_cast<T>(0.0f));
+      y[u] = load_part<T, Whole>(rows + j * P.stride, d, P.D, static_cast<T>(0.0f));
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -466,10 +480,10 @@ __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
       for (int v = 0; v < V; ++v) {
         const float x = to_float(g[u][v]);
         dot[u] = __builtin_fmaf(x, to_float(y[u][v]), dot[u]);
-        g[u][v] = static_cast<T>(i[u] < 0 ? nan_for((int)i[u]) : w[u] * x);
+        g[u][v] = static_cast<T>(state[u] != 0 ? nan_for(state[u]) : w[u] * x);
       }
       if (g_rows && j0 + u * kTeams < all)
-        store_part(g_rows + (j0 + u * kTeams) * P.D, d, P.D, g[u]);
+        store_part<T, Whole>(g_rows + (j0 + u * kTeams) * P.D, d, P.D, g[u]);
     }
   }
 #pragma unroll
@@ -477,8 +491,7 @@ __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
     const float sum = team_sum<TL>(dot[u]);
     const int64_t j = j0 + u * kTeams;
     if (lane != 0 || j >= all) continue;
-    const int64_t at = order[j];
-    if (at >= 0 && at < all) g_weights[at] = i[u] < 0 ? nan_for((int)i[u]) : sum;
+    if ((uint32_t)i[u] < (uint32_t)all) g_weights[i[u]] = state[u] != 0 ? nan_for(state[u]) : sum;
   }
 }
 
@@ -543,13 +556,12 @@ int from_codes_bwd_of(const RowsParams& P, const void* grad, const void* rows,
       return check_launch("rows_from_bwd_kernel");
     });
   };
-  if (vecs <= 1) return run(rows_from_bwd_kernel<T, 1>, 1);
-  if (vecs <= 2) return run(rows_from_bwd_kernel<T, 2>, 2);
-  if (vecs <= 4) return run(rows_from_bwd_kernel<T, 4>, 4);
-  if (vecs <= 8) return run(rows_from_bwd_kernel<T, 8>, 8);
-  if (vecs <= 16) return run(rows_from_bwd_kernel<T, 16>, 16);
-  if (vecs <= 32) return run(rows_from_bwd_kernel<T, 32>, 32);
-  return run(rows_from_bwd_kernel<T, 64>, 64);
+  const bool whole = P.D % kVec<T> == 0;
+#define GS_LANES(TL) \
+  if (vecs <= TL || TL == 64) \
+    return whole ? run(rows_from_bwd_kernel<T, TL, true>, TL) : run(rows_from_bwd_kernel<T, TL, false>, TL);
+  GS_LANES(1) GS_LANES(2) GS_LANES(4) GS_LANES(8) GS_LANES(16) GS_LANES(32) GS_LANES(64)
+#undef GS_LANES
 }
 
 }  // namespace
@@ -580,7 +592,7 @@ int launch_group_codes(const GroupParams& P, int32_t* order, int32_t* places,
     if ((rc = check_launch("group_scan_kernel"))) return rc;
     int bits = 1;
     while ((1 << bits) <= P.K) ++bits;
-    auto place = rounds == 4 ? group_place_kernel<4> : group_place_kernel<16>;
+    auto place = rounds == 4 ? group_place_kernel<4> : rounds == 8 ? group_place_kernel<8> : group_place_kernel<16>;
     launch_traced("group_place_kernel", place, dim3(L.chunks), dim3(kThreads), 0, stream, P, bits,
                   counts, totals, order, places, starts);
     return check_launch("group_place_kernel");
