@@ -871,6 +871,7 @@ __global__ __launch_bounds__(kThreads) void adapters_join_kernel(AdapterParams P
     T* out = static_cast<T*>(A.out[which]) + t.code * values;
     for (int64_t i = blockIdx.y * kThreads + threadIdx.x; i < values; i += gridDim.y * kThreads) {
       float a = 0.0f;
+#pragma unroll 8
       for (int64_t c = 0; c < chunks; ++c) a += sums[c * values + i];
       out[i] = static_cast<T>(a);
     }
@@ -956,7 +957,7 @@ int forward_of(const AdapterParams& P, const void* rows, const void* down,
 int chunk_of(const AdapterParams& P, int dtype_bytes) {
   const int64_t blocks = (P.D + P.E) * dtype_bytes / 256 + 1;
   int L = 512;
-  while (L < 8192 && P.rows * blocks > (int64_t)L * 2048) L *= 2;
+  while (L < 65536 && P.rows * blocks > (int64_t)L * 2048) L *= 2;
   return L;
 }
 

@@ -91,30 +91,31 @@ __global__ __launch_bounds__(kThreads) void group_count_kernel(GroupParams P, in
 }
 
 // Each bin's counts to the sums of the chunks before, and its total.  A workgroup
-// has 16 bins; 16 threads a bin take a part of the chunks each.
-__global__ __launch_bounds__(kThreads) void group_scan_kernel(GroupParams P, int chunks,
-                                                              uint32_t* __restrict__ counts,
-                                                              uint32_t* __restrict__ totals) {
-  __shared__ uint32_t sums[16][17];
+// has 16 bins; 64 threads a bin take a part of the chunks each.
+constexpr int kScanParts = 64;
+__global__ __launch_bounds__(16 * kScanParts) void group_scan_kernel(GroupParams P, int chunks,
+                                                                     uint32_t* __restrict__ counts,
+                                                                     uint32_t* __restrict__ totals) {
+  __shared__ uint32_t sums[kScanParts][17];
   const int lane = threadIdx.x & 15, part = threadIdx.x >> 4;
-  const int bin = blockIdx.x * 16 + lane, bins = P.K + 1;
-  const int span = (chunks + 15) / 16, from = min(part * span, chunks), to = min(from + span, chunks);
-  const bool in = bin < bins;
+  const int bin = blockIdx.x * 16 + lane, bins = P.K + 1, safe = min(bin, bins - 1);
+  const int span = (chunks + kScanParts - 1) / kScanParts;
+  const int from = min(part * span, chunks), to = min(from + span, chunks);
   uint32_t a = 0;
-#pragma unroll 8
-  for (int c = from; c < to; ++c)
-    if (in) a += counts[(int64_t)c * bins + bin];
+#pragma unroll 4
+  for (int c = from; c < to; ++c) a += counts[(int64_t)c * bins + safe];
   sums[part][lane] = a;
   __syncthreads();
   uint32_t before = 0, total = 0;
-#pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    if (q < part) before += sums[q][lane];
-    total += sums[q][lane];
+#pragma unroll 16
+  for (int q = 0; q < kScanParts; ++q) {
+    const uint32_t n = sums[q][lane];
+    if (q < part) before += n;
+    total += n;
   }
-  if (!in) return;
+  if (bin >= bins) return;
   if (part == 0) totals[bin] = total;
-#pragma unroll 8
+#pragma unroll 4
   for (int c = from; c < to; ++c) {
     const uint32_t n = counts[(int64_t)c * bins + bin];
     counts[(int64_t)c * bins + bin] = before;
@@ -587,7 +588,7 @@ int launch_group_codes(const GroupParams& P, int32_t* order, int32_t* places,
                   stream, P, rounds, counts);
     int rc = check_launch("group_count_kernel");
     if (rc) return rc;
-    launch_traced("group_scan_kernel", group_scan_kernel, dim3((P.K + 16) / 16), dim3(kThreads), 0,
+    launch_traced("group_scan_kernel", group_scan_kernel, dim3((P.K + 16) / 16), dim3(16 * kScanParts), 0,
                   stream, P, L.chunks, counts, totals);
     if ((rc = check_launch("group_scan_kernel"))) return rc;
     int bits = 1;

@@ -50,14 +50,22 @@ __device__ __forceinline__ double squares(const T* x, int64_t n) {
 #pragma unroll
   for (int v = 0; v < V; ++v) a[v] = 0.0;
   int64_t i = (int64_t)threadIdx.x * V;
-  for (; i + V <= n; i += kThreads * V) {
-    const vec_t<T> y = load_vec(x + i);
+  auto add = [&](vec_t<T> y) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const double z = (double)to_float(y[v]);
       a[v] = __builtin_fma(z, z, a[v]);
     }
+  };
+  // (four loads on their way at a time)
+  for (; i + 3 * kThreads * V + V <= n; i += 4 * kThreads * V) {
+    vec_t<T> y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) y[u] = load_vec(x + i + u * kThreads * V);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(y[u]);
   }
+  for (; i + V <= n; i += kThreads * V) add(load_vec(x + i));
   for (; i < n; ++i) {
     const double z = (double)to_float(x[i]);
     a[0] = __builtin_fma(z, z, a[0]);
@@ -108,13 +116,20 @@ template <typename T>
 __device__ __forceinline__ void scale(const T* x, T* y, int64_t n, float f) {
   constexpr int V = kVec<T>;
   int64_t i = (int64_t)threadIdx.x * V;
-  for (; i + V <= n; i += kThreads * V) {
-    vec_t<T> z = load_vec(x + i);
+  auto put = [&](int64_t at, vec_t<T> z) {
     if (f != 1.0f)
 #pragma unroll
       for (int v = 0; v < V; ++v) z[v] = static_cast<T>(to_float(z[v]) * f);
-    store_vec(y + i, z);
+    store_vec(y + at, z);
+  };
+  for (; i + 3 * kThreads * V + V <= n; i += 4 * kThreads * V) {
+    vec_t<T> z[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] = load_vec(x + i + u * kThreads * V);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) put(i + u * kThreads * V, z[u]);
   }
+  for (; i + V <= n; i += kThreads * V) put(i, load_vec(x + i));
   for (; i < n; ++i) y[i] = f != 1.0f ? static_cast<T>(to_float(x[i]) * f) : x[i];
 }
 
@@ -141,12 +156,12 @@ __global__ __launch_bounds__(kThreads) void clip_scale_kernel(
     scale(static_cast<const _Float16*>(A.from[t]) + from, static_cast<_Float16*>(A.to[t]) + from, n, f);
 }
 
-// Elements of a chunk: as many as make about 2048 workgroups of all, 4096 to 2^24.
+// Elements of a chunk: as many as make about 4096 workgroups of all, 4096 to 2^24.
 int64_t chunk_of(const ClipTensor* x, int64_t count) {
   int64_t all = 0;
   for (int64_t i = 0; i < count; ++i) all += x[i].size;
   int64_t c = 4096;
-  while (c < int64_t(1) << 24 && c * 2048 < all) c *= 2;
+  while (c < int64_t(1) << 24 && c * 4096 < all) c *= 2;
   return c;
 }
 int64_t blocks_of(const ClipTensor* x, int64_t count, int64_t chunk) {
@@ -154,7 +169,7 @@ int64_t blocks_of(const ClipTensor* x, int64_t count, int64_t chunk) {
   for (int64_t i = 0; i < count; ++i) n += (x[i].size + chunk - 1) / chunk;
   return n;
 }
-constexpr int64_t kMostSums = 4096;  // that every workgroup adds up itself
+constexpr int64_t kMostSums = 8192;  // that every workgroup adds up itself
 
 }  // namespace
 

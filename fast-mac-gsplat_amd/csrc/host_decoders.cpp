@@ -340,7 +340,8 @@ py::object adapters(py::handle rows, py::handle order, py::handle places, py::ha
 
 // ---- clipping
 
-// gradients and out: lists or tuples of tensors (out None: in place).
+// gradients and out: lists or tuples of tensors (out None: in place; a gradient that
+// is None is left out).
 py::object clip(py::handle gradients, double max_norm, py::handle out) {
   if (!plain_context() || !(max_norm >= 0.0)) return py::none();
   const bool into = !out.is_none();
@@ -352,7 +353,8 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
   struct Range {
     uintptr_t from, to;
   };
-  std::vector<gsplat_clip_tensor> table(count);
+  std::vector<gsplat_clip_tensor> table;
+  table.reserve(count);
   std::vector<Range> written, read;
   written.reserve(count);
   if (into) read.reserve(count);
@@ -360,6 +362,7 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
   int64_t all = 0;
   for (Py_ssize_t k = 0; k < count; ++k) {
     PyObject* p = PySequence_Fast_GET_ITEM(gradients.ptr(), k);
+    if (p == Py_None) continue;
     if (!ordinary(p)) return py::none();
     const Tensor& g = THPVariable_Unpack(p);
     if (first == nullptr) first = &g;
@@ -368,7 +371,7 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
     if (dtype < 0 || g.device() != first->device() || g.requires_grad() ||
         !g.is_non_overlapping_and_dense() || (all += n) > (int64_t(1) << 40))
       return py::none();
-    table[k] = gsplat_clip_tensor{g.data_ptr(), g.data_ptr(), n, dtype};
+    table.push_back(gsplat_clip_tensor{g.data_ptr(), g.data_ptr(), n, dtype});
     const size_t bytes = (size_t)n * g.element_size();
     const auto at = reinterpret_cast<uintptr_t>(g.data_ptr());
     if (into) {
@@ -378,7 +381,7 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
       if (o.scalar_type() != g.scalar_type() || o.device() != g.device() || o.requires_grad() ||
           o.sizes() != g.sizes() || o.strides() != g.strides() || o.is_inference())
         return py::none();
-      table[k].to = o.data_ptr();
+      table.back().to = o.data_ptr();
       const auto to = reinterpret_cast<uintptr_t>(o.data_ptr());
       if (bytes == 0) continue;
       written.push_back({to, to + bytes});
@@ -388,6 +391,7 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
       if (bytes > 0) written.push_back({at, at + bytes});
     }
   }
+  if (first == nullptr) return py::none();
   // What is written must be nobody else's, read or written.
   const auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
   std::sort(written.begin(), written.end(), before);
@@ -402,18 +406,19 @@ py::object clip(py::handle gradients, double max_norm, py::handle out) {
   const c10::DeviceGuard device(first->device());
   at::AutoDispatchBelowADInplaceOrView below;
   const Tensor norm = at::empty({}, first->options().dtype(at::kFloat));
-  const size_t n = api.clip_gradients_workspace_bytes(table.data(), count);
+  const size_t n = api.clip_gradients_workspace_bytes(table.data(), table.size());
   const Tensor ws = bytes((int64_t)n, *first);
   {
     const Timed timed("clip_gradients");
-    check(api.clip_gradients(table.data(), count, max_norm, norm.data_ptr<float>(), pointer(ws), n,
+    check(api.clip_gradients(table.data(), table.size(), max_norm, norm.data_ptr<float>(), pointer(ws), n,
                              stream_of(*first)),
           "gsplat_hip_clip_gradients");
   }
   for (Py_ssize_t k = 0; k < count; ++k)
-    THPVariable_Unpack(PySequence_Fast_GET_ITEM((into ? out : gradients).ptr(), k))
-        .unsafeGetTensorImpl()
-        ->bump_version();
+    if (PySequence_Fast_GET_ITEM(gradients.ptr(), k) != Py_None)
+      THPVariable_Unpack(PySequence_Fast_GET_ITEM((into ? out : gradients).ptr(), k))
+          .unsafeGetTensorImpl()
+          ->bump_version();
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
 }
 

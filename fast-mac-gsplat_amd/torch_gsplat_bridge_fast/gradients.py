@@ -112,13 +112,10 @@ def clip_gradients(gradients: Iterable[Tensor], max_norm: float, out: Optional[I
     out = out if out is None or isinstance(out, (list, tuple)) else list(out)
     if out is not None and len(out) != len(gradients):
         raise ValueError("out must have a tensor for each gradient")
-    if any(g is None for g in gradients):
-        if out is not None:
-            out = [o for g, o in zip(gradients, out) if g is not None]
-        gradients = [g for g in gradients if g is not None]
     norm = _lib.host().clip_gradients(gradients, max_norm, out)
     if norm is not None:
         return norm
-    gradients, out = list(gradients), None if out is None else list(out)
+    out = None if out is None else [o for g, o in zip(gradients, out) if g is not None]
+    gradients = [g for g in gradients if g is not None]
     _check_clip(gradients, gradients if out is None else out, max_norm)
     return _clip_in_place(gradients, float(max_norm)) if out is None else _clip_into(gradients, out, float(max_norm))
