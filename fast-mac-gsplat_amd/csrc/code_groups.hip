@@ -19,7 +19,16 @@
 //
 // Rows: a thread has 16 bytes of a row, taken as one array of whole vectors per
 // row (the last one of a row that is not whole vectors overlaps the one before:
-// both hold the same values there).
+// both hold the same values there); the rows' and weights' gradients together, a
+// team of lanes a row.  All loads of a thread are issued before the first is
+// looked at; places past the last code are looked up by those few threads alone.
+//
+// What bounds it, on an MI355X: rows are HBM's, gathers of whole rows.  A million
+// rows of 128 floats by code 208 us (5.2 TB/s), 262144 splats x 4 rows of 128
+// bfloat16 back 72 us and 144 for both gradients (4.7 and 4.4 TB/s).  Sorting is
+// latency: 512 choices 5 us, 524288 of 256 codes 20 (three launches; by radix 45),
+// a million of 16384 codes 63 (five launches, 16 of them the places' scattered
+// stores).
 #include <algorithm>
 
 #include "codes.h"
@@ -41,7 +50,7 @@ __device__ __forceinline__ uint32_t key_of(const GroupParams& P, int64_t i) {
 // in the order, or a code, whose start is the number of choices of lower codes.
 // Four lanes an item compare it with a quarter of the choices each, held in LDS
 // as (key, index) in one word.
-constexpr int kFew = 4096, kFewBits = 12;
+constexpr int kFew = 2048, kFewBits = 11;
 
 __global__ __launch_bounds__(kThreads) void group_few_kernel(GroupParams P,
                                                              int32_t* __restrict__ order,
@@ -246,15 +255,19 @@ __global__ __launch_bounds__(kThreads) void group_finish_kernel(
   }
 }
 
-// How choices are sorted.  (Kernels in a row, 524288 choices of 256 codes: counted 26 us,
-// by radix 45.)
+// How choices are sorted, us of a call.  Few: one launch, 512 choices 5, 2048 12; 4096
+// would take 23, counted 13.  Counted: 65536 of 64 codes 14, 524288 of 256 codes 20
+// (by radix 45) and of 2047 codes 26 (of 2048 by radix 48), 4 million of 256 codes 54
+// (by radix 127); as long as a workgroup's LDS holds a bin a wavefront and code, and
+// the chunks' counts are less than the choices.
 enum class Way { kFew, kCounted, kRadix };
 Way way_of(const GroupParams& P) {
   if (P.choices <= kFew && P.K <= 16384) return Way::kFew;
-  if (P.choices <= 1 << 22 && P.K < kMostBins) return Way::kCounted;
+  if (P.choices <= 1 << 25 && P.K < kMostBins) return Way::kCounted;
   return Way::kRadix;
 }
-// Choices of a chunk over kThreads.
+// Choices of a chunk over kThreads: small ones while there are less of them than
+// compute units (524288 choices: 31 us in chunks of 4096, 25 of 2048).
 int rounds_of(const GroupParams& P) { return P.choices <= 1 << 18 ? 4 : P.choices <= 1 << 20 ? 8 : 16; }
 
 struct SortLayout {

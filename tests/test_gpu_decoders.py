@@ -39,7 +39,7 @@ def _check_group(gpu, codes, K, several=False, what=""):
 
 # ---- sorting
 
-SIZES = [1, 2, 63, 64, 65, 255, 256, 257, 1000, 1023, 1024, 1025, 2048, 4095, 4096, 4097, 8191, 8193, 16385, 40000, 65536,
+SIZES = [1, 2, 63, 64, 65, 255, 256, 257, 1000, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8193, 16385, 40000, 65536,
          70001, 300007]
 
 

@@ -23,7 +23,7 @@ def _give_back(gpu):
     torch.cuda.empty_cache()
 
 
-@pytest.mark.parametrize("N,K", [((1 << 22) + 77, 100), ((1 << 22) - 5, 2047), (3000001, 5000)])
+@pytest.mark.parametrize("N,K", [((1 << 22) + 77, 100), ((1 << 22) - 5, 2047), (3000001, 5000), (1 << 25, 60), ((1 << 25) + 9, 60)])
 def test_sort(gpu, N, K):
     codes = torch.randint(-1, K, (N,), device=gpu, dtype=torch.int32)
     got = gs.group_codes(codes, K)
