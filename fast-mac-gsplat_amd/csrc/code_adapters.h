@@ -204,7 +204,13 @@ __device__ __forceinline__ void bring(vec_t<T>& v, int i, int n) {
 template <int N, typename T, bool Whole>
 __device__ __forceinline__ void store_n(T* row, int i, int n, const T (&v)[N]) {
   if (Whole ? i < n : i + N <= n) {
-    __builtin_memcpy(row + i, v, sizeof(v));
+    if constexpr (sizeof(v) == 16) {
+      vec_t<T> x;
+      __builtin_memcpy(&x, v, 16);
+      store_vec_stream(row + i, x);
+    } else {
+      __builtin_memcpy(row + i, v, sizeof(v));
+    }
     return;
   }
   if (Whole) return;

@@ -359,7 +359,7 @@ __device__ __forceinline__ vec_t<T> load_at(const T* row, int d, int D) {
 }
 template <typename T>
 __device__ __forceinline__ void store_at(T* row, int d, int D, vec_t<T> v) {
-  if (D >= kVec<T>) store_vec(row + d, v);
+  if (D >= kVec<T>) store_vec_stream(row + d, v);
   else store_part(row, d, D, v);
 }
 
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
     for (int u = 0; u < kAhead; ++u) {
       const int64_t j = min(j0 + u * kTeams, all - 1);
       g[u] = load_part<T, Whole>(grad + n[u] * P.D, d, P.D, static_cast<T>(0.0f));
-      y[u] = load_part<T, Whole>(rows + j * P.stride, d, P.D, static_cast<T>(0.0f));
+      y[u] = load_part<T, Whole, true>(rows + j * P.stride, d, P.D, static_cast<T>(0.0f));
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -497,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void rows_from_bwd_kernel(
         g[u][v] = static_cast<T>(state[u] != 0 ? nan_for(state[u]) : w[u] * x);
       }
       if (g_rows && j0 + u * kTeams < all)
-        store_part<T, Whole>(g_rows + (j0 + u * kTeams) * P.D, d, P.D, g[u]);
+        store_part<T, Whole, true>(g_rows + (j0 + u * kTeams) * P.D, d, P.D, g[u]);
     }
   }
 #pragma unroll
