@@ -23,15 +23,16 @@
 // (An infinite value of a row or a map makes what depends on it infinite or NaN.)
 //
 // What bounds it, on an MI355X: 131072 rows of 1024 -> 1024 values of bfloat16,
-// rank 32, 256 codes: the forward 171 us for 805 MB (4.7 TB/s; a large copy
-// reaches 4.9), the rows' gradient 135 us for 537 MB, the maps' gradients 155 us
-// for 537 MB and the hidden values.  Both wait on loads: two wavefronts a SIMD,
-// 6 to 12 KB on their way each.  65536 rows of 128 -> 59 floats, rank 8: 20, 21 and
-// 19 us for 49 MB each: one and a half rounds of workgroups, each a chain of
-// dependent loads (starts, order, rows, maps).  Loads without a mask, a branch or
-// a use behind them took 785 us of the first case's step to 485; coalesced rows of
-// the factors (turned in LDS) and rows without a code in all threads were the
-// other half.
+// rank 32, 256 codes: the forward 179 us for 805 MB (4.5 TB/s; a large copy
+// reaches 4.9), the rows' gradient 134 us for 537 MB, the maps' gradients 114 us
+// for 537 MB and the hidden values (4.7 TB/s).  They wait on loads: two wavefronts
+// a SIMD, 6 to 12 KB on their way each.  65536 rows of 128 -> 59 floats, rank 8:
+// 22, 21 and 20 us for 49 MB each: one and a half rounds of workgroups, each a
+// chain of dependent loads (starts, order, rows, maps).  What took the first case's
+// step from 785 us to 448: coalesced rows of the factors (turned in LDS), rows
+// without a code in all threads, loads without a mask, a branch or a use behind
+// them, and stores and last reads past the caches (the maps' gradients 155 us
+// without, as what they read was no longer there).
 //
 // Tiles: 64 places (32 above rank 64, for their registers) once codes have 32 on
 // average and tiles fill the card; 16 below.  Measured and not kept: 32 places for
@@ -188,9 +189,13 @@ inline int fit_of(std::initializer_list<int> widths, int vec) {
 // place, zeros past the row's end.  Apart, since a value that is looked at as it is
 // loaded, or loaded behind a branch, is waited for: the loads after it would start
 // only then.
-template <typename T, int Fit>
+// Stream: past the caches, for what nothing reads again.
+template <typename T, int Fit, bool Stream = false>
 __device__ __forceinline__ vec_t<T> load_raw(const T* row, int i, int n) {
-  if (Fit != kShort || n >= kVec<T>) return load_vec(row + min(i, n - kVec<T>));
+  if (Fit != kShort || n >= kVec<T>) {
+    const T* at = row + min(i, n - kVec<T>);
+    return Stream ? load_vec_stream(at) : load_vec(at);
+  }
   return load_part(row, i, n, static_cast<T>(0.0f));
 }
 template <typename T, int Fit>
@@ -760,7 +765,7 @@ __global__ __launch_bounds__(64 * Waves) void adapters_maps_kernel(AdapterParams
     for (int q = 0; q < V; ++q) {
       const int64_t at = t.first + min(place(j0, q), end - 1);
       const int64_t row = P.by_code ? at : (uint32_t)n[q] < (uint32_t)P.rows ? n[q] : 0;
-      x[q] = load_raw<T, Fit>(rows + row * stride, d, width);
+      x[q] = load_raw<T, Fit, true>(rows + row * stride, d, width);
       const float* from = hidden + at * P.r + r0;
 #pragma unroll
       for (int k = 0; k < RT; ++k) h[k][q] = from[min(16 * k + col, P.r - 1 - r0)];
