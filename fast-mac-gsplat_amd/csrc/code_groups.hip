@@ -23,12 +23,13 @@
 // team of lanes a row.  All loads of a thread are issued before the first is
 // looked at; places past the last code are looked up by those few threads alone.
 //
-// What bounds it, on an MI355X: rows are HBM's, gathers of whole rows.  A million
-// rows of 128 floats by code 208 us (5.2 TB/s), 262144 splats x 4 rows of 128
-// bfloat16 back 72 us and 144 for both gradients (4.7 and 4.4 TB/s).  Sorting is
-// latency: 512 choices 5 us, 524288 of 256 codes 20 (three launches; by radix 45),
-// a million of 16384 codes 63 (five launches, 16 of them the places' scattered
-// stores).
+// What bounds it, on an MI355X: rows are HBM's, gathers of whole rows; stores go
+// past the caches.  A million rows of 128 floats by code 195 us (5.5 TB/s; 208
+// through the caches), 262144 splats x 4 rows of 128 bfloat16 back 62 us and 139 for
+// both gradients (5.4 and 4.3 TB/s, 6.8 with a splat's row read for each of its
+// codes).  Sorting is latency: 512 choices 5 us, 524288 of 256 codes 20 (three
+// launches; by radix 45), a million of 16384 codes 62 (five launches, 16 us of them
+// the places' scattered stores).
 #include <algorithm>
 
 #include "codes.h"
