@@ -54,6 +54,27 @@ def test_adapters_of_more_tiles_than_a_launch_has_workgroups(gpu):
         R.check(out[a:a + 500], want["out"], f"rows from {a}")
 
 
+@pytest.mark.parametrize("N", [0, 5, 3000])
+def test_adapters_of_more_codes_than_a_launch_has_workgroups(gpu, N):
+    """Every map's gradient is written, however few rows there are."""
+    _room(4)
+    K = (1 << 24) + 3
+    codes = torch.randint(0, K - 2, (N,), generator=torch.Generator().manual_seed(N)).to(gpu)
+    if N:
+        codes[0], codes[N // 2] = K - 2, K - 2
+    dn, up = torch.full((K, 1, 2), 2.0, device=gpu, requires_grad=True), torch.full((K, 3, 1), 3.0, device=gpu, requires_grad=True)
+    junk = torch.full((K, 3), 7.0, device=gpu)  # (what the gradients' memory may hold)
+    del junk
+    x = torch.ones(N, 2, device=gpu)
+    out = gs.code_adapters(x, gs.group_codes(codes, K), dn, up)
+    assert out.shape == (N, 3) and bool((out == 12.0).all())
+    g_down, g_up = torch.autograd.grad(out, [dn, up], torch.ones_like(out))
+    where, counts = codes.unique(return_counts=True)
+    assert torch.equal(g_down[where], (9.0 * counts)[:, None, None].expand(-1, 1, 2))
+    assert torch.equal(g_up[where], (4.0 * counts)[:, None, None].expand(-1, 3, 1))
+    assert int(g_down.count_nonzero()) == 2 * where.numel() and int(g_up.count_nonzero()) == 3 * where.numel()
+
+
 def test_adapters_gradient_past_32_bits(gpu):
     """More than 2^32 values of rows and results, one code of most rows: chunks by the thousand."""
     _room(120)
