@@ -23,13 +23,13 @@
 // (An infinite value of a row or a map makes what depends on it infinite or NaN.)
 //
 // What bounds it, on an MI355X: 131072 rows of 1024 -> 1024 values of bfloat16,
-// rank 32, 256 codes: the forward 179 us for 805 MB (4.5 TB/s; a large copy
-// reaches 4.9), the rows' gradient 134 us for 537 MB, the maps' gradients 114 us
-// for 537 MB and the hidden values (4.7 TB/s).  They wait on loads: two wavefronts
-// a SIMD, 6 to 12 KB on their way each.  65536 rows of 128 -> 59 floats, rank 8:
+// rank 32, 256 codes: the forward 176 us for 805 MB (4.6 TB/s; a large copy
+// reaches 4.9), the rows' gradient 130 us for 537 MB, the maps' gradients 115 us
+// for 537 MB and the hidden values (4.7 TB/s).  They wait on loads: two to three
+// wavefronts a SIMD, 6 to 12 KB on their way each.  65536 rows of 128 -> 59 floats, rank 8:
 // 22, 21 and 20 us for 49 MB each: one and a half rounds of workgroups, each a
 // chain of dependent loads (starts, order, rows, maps).  What took the first case's
-// step from 785 us to 448: coalesced rows of the factors (turned in LDS), rows
+// step from 785 us to 442: coalesced rows of the factors (turned in LDS), rows
 // without a code in all threads, loads without a mask, a branch or a use behind
 // them, and stores and last reads past the caches (the maps' gradients 155 us
 // without, as what they read was no longer there).
@@ -123,9 +123,9 @@ __device__ __forceinline__ int row_at(const AdapterParams& P, int64_t j) {
 
 // ---- 16 x 16 tiles
 
-// A lane's 16 bytes of a factor: row lane % 16, values 4 v + ... of the quarter
-// lane / 16.  A product of two takes 4 * kVec values of the rows; lane l has its
-// elements 4 (l / 16) + 0..3 of column l % 16.
+// A lane has 16 bytes of a factor: of its row lane % 16, the quarter lane / 16 of 4 *
+// kVec values.  Of the product of two, lane l has elements 4 (l / 16) + 0..3 of
+// column l % 16.
 template <typename T>
 __device__ __forceinline__ void mma(f32x4& acc, vec_t<T> a, vec_t<T> b) {
   if constexpr (sizeof(T) == 4) {
@@ -253,11 +253,10 @@ __device__ __forceinline__ void turn(vec_t<T> (&x)[kVec<T>]) {
 }
 
 // A factor on its way to the tiles.  The matrix instructions take a lane's 16
-// bytes from row lane % 16: loaded so, every lane would be a request of its own
-// (64 a load, where 8 lanes of a row make one).  So a wavefront
-// loads rows of adjacent chunks of 16 bytes, and turns them over in its own part
-// of LDS, no barrier needed.  Chunk c of row i lies at c ^ (a few bits of i): both
-// ways touch every bank once.
+// bytes from row lane % 16: loaded so, every lane would be a request of its own (64 a
+// load, where 8 lanes of a row make one).  So a wavefront loads rows of adjacent
+// chunks of 16 bytes, and turns them over in its own part of LDS, no barrier needed.
+// Chunk c of row i lies at c ^ (a few bits of i): both ways touch every bank once.
 template <int Chunks>
 __device__ __forceinline__ int swizzled(int row, int chunk) {
   constexpr int kMask = Chunks < 8 ? Chunks - 1 : 7, kRows = Chunks < 8 ? 8 / Chunks : 1;
@@ -392,11 +391,18 @@ struct RowsLds {
   // columns of a lane in the second product
   static constexpr int kCols = RT >= (sizeof(T) == 4 ? 8 : 4) ? V / 2 : V;
   static constexpr int kFirst = (M + R) * 8, kSecond = 16 * kCols * H::kChunks;  // chunks of a wavefront
+  // (the hidden values lie where the first product's factors were: at rank 32 three
+  // workgroups of 49 KB a compute unit instead of two of 60)
   union {
-    u32x4 stage[4][kFirst > kSecond ? kFirst : kSecond];
-    float red[2][M][R + 4];
+    u32x4 first[4][kFirst];
+    struct {
+      union {
+        u32x4 second[4][kSecond];
+        float red[2][M][R + 4];
+      };
+      __attribute__((aligned(16))) typename H::Element hidden[H::kWide ? 1 : 2][M][H::kRow];
+    };
   };
-  __attribute__((aligned(16))) typename H::Element hidden[H::kWide ? 1 : 2][M][H::kRow];
   int rows[M];
 };
 
@@ -617,7 +623,7 @@ __global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParam
 #pragma unroll
       for (int k = 0; k < RT; ++k) acc[0][k] = f32x4{0, 0, 0, 0};
       if (w < MT)
-        first_product<T, 1, RT, Turned, Fit>(acc, A, P.r, down, lds.stage[w], lds.rows + 16 * w, 0, 1);
+        first_product<T, 1, RT, Turned, Fit>(acc, A, P.r, down, lds.first[w], lds.rows + 16 * w, 0, 1);
       __syncthreads();
       if (w < MT)
 #pragma unroll
@@ -630,7 +636,7 @@ __global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParam
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int k = 0; k < RT; ++k) acc[m][k] = f32x4{0, 0, 0, 0};
-      first_product<T, MT, RT, Turned, Fit>(acc, A, P.r, down, lds.stage[w], lds.rows, w + 4 * part,
+      first_product<T, MT, RT, Turned, Fit>(acc, A, P.r, down, lds.first[w], lds.rows, w + 4 * part,
                                               4 * parts);
       __syncthreads();
       // Wavefronts 2 and 3's sums to 0 and 1's, whose two are added where they are read.
@@ -691,9 +697,9 @@ __global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParam
     const T* up = static_cast<const T*>(A.up) + t.code * P.r * A.E;
     if (MT > 1 && A.E <= 3 * 16 * L::kCols) {
       if (w < MT)
-        second_product<T, MT, RT, 1, Turned, Fit>(A, P.r, up, lds, lds.stage[w], 16 * w, t.count, 0, 1);
+        second_product<T, MT, RT, 1, Turned, Fit>(A, P.r, up, lds, lds.second[w], 16 * w, t.count, 0, 1);
     } else {
-      second_product<T, MT, RT, MT, Turned, Fit>(A, P.r, up, lds, lds.stage[w], 0, t.count,
+      second_product<T, MT, RT, MT, Turned, Fit>(A, P.r, up, lds, lds.second[w], 0, t.count,
                                                    w + 4 * part, 4 * parts);
     }
   }
@@ -924,7 +930,7 @@ int rank_tiles(int r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 // How rows go: tiles of 16 * row_tiles places; splits > 1: hidden values and
 // results in launches of their own, each over parts of a row, for few rows of 2048
 // values and more (one row of 1024 -> 1024: 4.0 and 3.8 us so, 5.6 in one launch
-// that saves the host 3; 61 of 4096 -> 4096: 4.5 and 8.2).
+// that saves the host 3; 61 of 4096 -> 4096: 4.6 and 7.9).
 struct RowsPlan {
   int row_tiles, splits_down, splits_up;
 };
