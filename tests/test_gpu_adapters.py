@@ -197,6 +197,31 @@ def test_empty(gpu):
         assert not g[0].any() and not g[1].any() and g[0].shape == dn.shape and g[1].shape == up.shape
 
 
+def test_one_row_without_leading_axes(gpu):
+    for code in (2, -1):
+        codes, x, dn, up, b, go = _inputs(1, 4, 20, 11, 3, F32, codes=torch.tensor([code]))
+        want = R.adapters(x, R.group(codes, 4), dn, up, b, 0.5, False, go)
+        groups = gs.group_codes(codes[0].to(gpu), 4)
+        xg = x[0].to(gpu).requires_grad_(True)
+        out = gs.code_adapters(xg, groups, dn.to(gpu), up.to(gpu), b[0].to(gpu), 0.5)
+        R.check(out[None], want["out"], "out")
+        R.check(torch.autograd.grad(out, xg, go[0].to(gpu))[0][None], want["g_rows"], "g_rows")
+
+
+def test_rows_that_are_their_own_base(gpu):
+    """One tensor in two places: its gradients add up."""
+    codes, x, dn, up, _, go = _inputs(300, 5, 32, 32, 8, F32)
+    want = R.adapters(x, R.group(codes, 5), dn, up, x, 0.5, False, go)
+    xg = x.to(gpu).requires_grad_(True)
+    groups = gs.group_codes(codes.to(gpu), 5)
+    out = gs.code_adapters(xg, groups, dn.to(gpu), up.to(gpu), xg, 0.5)
+    R.check(out, want["out"], "out")
+    g, = torch.autograd.grad(out, xg, go.to(gpu))
+    value, bound = want["g_rows"]
+    total = value + go.double()
+    R.check(g, (total, bound + R.E * total.abs() * 2), "g_rows")
+
+
 def test_same_bits(gpu):
     codes, x, dn, up, b, go = (t.to(gpu) for t in _inputs(20000, 12, 130, 70, 16, BF16, skew=True))
     leaves = [t.requires_grad_(True) for t in (x, dn, up)]

@@ -165,3 +165,28 @@ def test_of_parameters(gpu):
     R.check(norm, (n, bound), "norm")
     for t, w in zip(p, out):
         R.check(t.grad, w, "grad")
+
+
+def test_graph_capture_of_many_tensors(gpu):
+    """Several tables of tensors in a captured graph: nothing of the host's is needed when it is replayed."""
+    sizes = [1 + (k * 37) % 300 for k in range(400)]
+    flat = torch.zeros(sum(sizes), device=gpu)
+    out = torch.zeros_like(flat)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gs.clip_gradients(list(flat.split(sizes)), 2.0, out=list(out.split(sizes)))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = gs.clip_gradients(list(flat.split(sizes)), 2.0, out=list(out.split(sizes)))
+    for k in range(3):
+        new = torch.randn(flat.numel(), generator=_gen(k))
+        flat.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        (want, bound), outs = R.clip([new], 2.0)
+        R.check(norm, (want, bound), "norm")
+        R.check(out, outs[0], "out")
+        eager = flat.clone()
+        assert torch.equal(gs.clip_gradients(list(eager.split(sizes)), 2.0), norm) and torch.equal(eager, out)
