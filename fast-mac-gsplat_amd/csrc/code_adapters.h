@@ -17,9 +17,9 @@
 // of columns; longer codes' sums are joined by another launch, in order.
 //
 // Everything is a matrix product of 16 x 16 tiles.  In 16 bits the hidden values
-// go into the second product as two bfloat16, h = hi + lo (16 bits of them, so
-// that the result's rounding is the only one that counts), and float16 factors
-// beside them as two bfloat16 too, exactly: hidden values have no range to leave.
+// go into the second product as the sum of three bfloat16, and float16 factors beside
+// them as that of two: exactly, and without a range to leave.  Each part of one is
+// multiplied with each of the other.
 // (An infinite value of a row or a map makes what depends on it infinite or NaN.)
 //
 // What bounds it, on an MI355X: 131072 rows of 1024 -> 1024 values of bfloat16,
@@ -139,41 +139,46 @@ __device__ __forceinline__ void mma(f32x4& acc, vec_t<T> a, vec_t<T> b) {
   }
 }
 
-// x = hi + lo, the larger part cut off after 8 bits (it stays in range), the
-// smaller one rounded to 8; an infinity has no smaller part.
-__device__ __forceinline__ void split(float x, uint32_t& hi, float& lo) {
-  const uint32_t u = __float_as_uint(x);
-  hi = u >> 16;
-  lo = x - __uint_as_float(u & 0xffff0000u);
-  if ((u & 0x7f800000u) == 0x7f800000u) lo = 0.0f;
+// x as the sum of N bfloat16, each what the ones before leave, cut off after 8 bits (so
+// that it stays in range): three hold a float, two a float16, exactly.  An infinity and
+// a NaN have no smaller parts.
+constexpr int kParts = 3;
+template <int N>
+__device__ __forceinline__ void split(float x, uint32_t (&part)[N]) {
+  const bool whole = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t u = __float_as_uint(x);
+    part[i] = u >> 16;
+    x = whole ? x - __uint_as_float(u & 0xffff0000u) : 0.0f;
+  }
 }
-__device__ __forceinline__ uint32_t bf16_bits(float x) {
-  return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
-}
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8& hi, bf16x8& lo) {
-  u32x4 h, l;
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&part)[N]) {
+  u32x4 w[N];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    uint32_t h0, h1;
-    float l0, l1;
-    split(x[2 * p], h0, l0);
-    split(x[2 * p + 1], h1, l1);
-    h[p] = h0 | h1 << 16;
-    l[p] = bf16_bits(l0) | bf16_bits(l1) << 16;
+    uint32_t a[N], b[N];
+    split(x[2 * p], a);
+    split(x[2 * p + 1], b);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i][p] = a[i] | b[i] << 16;
   }
-  hi = __builtin_bit_cast(bf16x8, h);
-  lo = __builtin_bit_cast(bf16x8, l);
+#pragma unroll
+  for (int i = 0; i < N; ++i) part[i] = __builtin_bit_cast(bf16x8, w[i]);
 }
 // Eight values of a map or a row as bfloat16: themselves, or a float16's two parts.
 template <typename T>
-__device__ __forceinline__ void parts(vec_t<T> x, bf16x8& hi, bf16x8& lo) {
+constexpr int kOfMap = __is_same(T, __bf16) ? 1 : 2;
+template <typename T>
+__device__ __forceinline__ void parts(vec_t<T> x, bf16x8 (&part)[kOfMap<T>]) {
   if constexpr (__is_same(T, __bf16)) {
-    hi = x;
+    part[0] = x;
   } else {
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = to_float(x[i]);
-    split8(f, hi, lo);
+    split8(f, part);
   }
 }
 
@@ -334,9 +339,9 @@ struct MapChunks {
   }
 };
 
-// Hidden values of a tile as the second product's factor.  Rank blocks of 16 in
-// 32 bits, of 32 in 16 bits; a single block of 16 ranks holds hi and lo side by
-// side instead.
+// Hidden values of a tile as the second product's factors.  Rank blocks of 16 in
+// 32 bits, of 32 in 16 bits, a factor for each part; a single block of 16 ranks is there
+// twice instead, for the first two parts side by side and for the halves of the third.
 template <typename T, int RT>
 struct Hidden {
   static constexpr bool kWide = sizeof(T) == 4;
@@ -344,26 +349,34 @@ struct Hidden {
   static constexpr int kBlocks = kWide || RT == 1 ? RT : RT / 2;
   static constexpr int kRow = kWide ? 16 * RT + 4 : 16 * RT + 8;  // of LDS, elements
   static constexpr int kChunks = 16 * RT / kVec<T>;               // of a map's row
+  static constexpr int kHeld = kWide ? 1 : kParts;                // in LDS
+  static constexpr int kFactors = kWide ? 1 : kBoth ? 2 : kParts;
   using Factor = std::conditional_t<kWide, vec_t<float>, bf16x8>;
   using Element = std::conditional_t<kWide, float, uint16_t>;
   // the map's chunk that a lane's quarter multiplies in rank block k
   static __device__ __forceinline__ int chunk(int k, int quarter) {
     return kBoth ? quarter & 1 : 4 * k + quarter;
   }
+  // the part that a lane's quarter has of factor i
+  static __device__ __forceinline__ int part(int i, int quarter) {
+    return !kBoth ? i : i == 0 ? quarter >> 1 : 2;
+  }
 };
 
 // acc += h * up for one rank block.
 template <typename T, int RT>
-__device__ __forceinline__ void mma_hidden(f32x4& acc, typename Hidden<T, RT>::Factor hi,
-                                           typename Hidden<T, RT>::Factor lo, vec_t<T> up) {
+__device__ __forceinline__ void mma_hidden(f32x4& acc,
+                                           const typename Hidden<T, RT>::Factor (&h)[Hidden<T, RT>::kFactors],
+                                           vec_t<T> up) {
   if constexpr (sizeof(T) == 4) {
-    mma<float>(acc, hi, up);
+    mma<float>(acc, h[0], up);
   } else {
-    bf16x8 u, v;
-    parts<T>(up, u, v);
-    mma<__bf16>(acc, hi, u);
-    if constexpr (RT > 1) mma<__bf16>(acc, lo, u);
-    if constexpr (!__is_same(T, __bf16)) mma<__bf16>(acc, hi, v);
+    bf16x8 u[kOfMap<T>];
+    parts<T>(up, u);
+#pragma unroll
+    for (int p = 0; p < kOfMap<T>; ++p)
+#pragma unroll
+      for (int i = 0; i < Hidden<T, RT>::kFactors; ++i) mma<__bf16>(acc, h[i], u[p]);
   }
 }
 
@@ -400,7 +413,7 @@ struct RowsLds {
         u32x4 second[4][kSecond];
         float red[2][M][R + 4];
       };
-      __attribute__((aligned(16))) typename H::Element hidden[H::kWide ? 1 : 2][M][H::kRow];
+      __attribute__((aligned(16))) typename H::Element hidden[H::kHeld][M][H::kRow];
     };
   };
   int rows[M];
@@ -502,30 +515,22 @@ __device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
       if (m + 1 < MW) load_base(m + 1, y[(m + 1) & 1]);
-      typename H::Factor hi[H::kBlocks], lo[H::kBlocks];
+      typename H::Factor h[H::kBlocks][H::kFactors];
       const int row = m0 + 16 * m + col;
 #pragma unroll
-      for (int k = 0; k < H::kBlocks; ++k) {
-        auto read = [&](int part, int i) {
-          return __builtin_bit_cast(typename H::Factor,
-                                    *reinterpret_cast<const u32x4*>(&lds.hidden[part][row][i]));
-        };
-        if constexpr (H::kWide) {
-          hi[k] = read(0, 16 * k + 4 * quarter);
-        } else if constexpr (H::kBoth) {
-          hi[k] = read(quarter >> 1, 8 * (quarter & 1));
-        } else {
-          hi[k] = read(0, 32 * k + 8 * quarter);
-          lo[k] = read(1, 32 * k + 8 * quarter);
-        }
-      }
+      for (int k = 0; k < H::kBlocks; ++k)
+#pragma unroll
+        for (int i = 0; i < H::kFactors; ++i)
+          h[k][i] = __builtin_bit_cast(
+              typename H::Factor,
+              *reinterpret_cast<const u32x4*>(&lds.hidden[H::part(i, quarter)][row][kVec<T> * H::chunk(k, quarter)]));
       f32x4 acc[N];
 #pragma unroll
       for (int t = 0; t < N; ++t) {
         acc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < H::kBlocks; ++k)
-          mma_hidden<T, RT>(acc[t], hi[k], lo[k],
+          mma_hidden<T, RT>(acc[t], h[k],
                             __builtin_bit_cast(vec_t<T>, stage[place(N * col + t, H::chunk(k, quarter))]));
       }
 #pragma unroll
@@ -581,10 +586,15 @@ __device__ __forceinline__ void rows_without_code(const RowsArgs& A, const int* 
   }
 }
 
+// Wavefronts a SIMD that the compiler keeps room for: three where it takes them without
+// spills and would have two registers too many.
+template <typename T, int MT, int RT, int Fit>
+constexpr int kRowsWaves = MT == 4 && RT == 2 && Fit == kWhole && __is_same(T, __bf16) ? 3 : 2;
+
 // Phase 1: hidden values, over part blockIdx.y of D, left in `parts`; 2: results
 // from them, over part blockIdx.y of E; 3: both.  Fit: that of D, E and r.
 template <typename T, int MT, int RT, int Phase, bool Turned, int Fit>
-__global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParams P, RowsArgs A,
+__global__ __launch_bounds__(kThreads, (kRowsWaves<T, MT, RT, Fit>)) void adapters_rows_kernel(AdapterParams P, RowsArgs A,
                                                                     Slots S) {
   using L = RowsLds<T, MT, RT>;
   using H = Hidden<T, RT>;
@@ -683,11 +693,11 @@ __global__ __launch_bounds__(kThreads, 2) void adapters_rows_kernel(AdapterParam
       if constexpr (H::kWide) {
         lds.hidden[0][m][k] = h;
       } else {
-        uint32_t hi;
-        float lo;
-        split(h, hi, lo);
-        lds.hidden[0][m][k] = (uint16_t)hi;
-        lds.hidden[1][m][k] = (uint16_t)bf16_bits(lo);
+        uint32_t part[kParts];
+        split(h, part);
+        if (H::kBoth) part[2] = __float_as_uint(0.5f * __uint_as_float(part[2] << 16)) >> 16;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) lds.hidden[i][m][k] = (uint16_t)part[i];
       }
     }
   }
@@ -825,21 +835,21 @@ __global__ __launch_bounds__(64 * Waves) void adapters_maps_kernel(AdapterParams
 #pragma unroll
       for (int q = 0; q < V; ++q) y[q] = x[q];
       turn<T>(y);
-      bf16x8 hi[RT], lo[RT];
+      bf16x8 g[RT][kParts];
 #pragma unroll
-      for (int k = 0; k < RT; ++k) split8(h[k], hi[k], lo[k]);
+      for (int k = 0; k < RT; ++k) split8(h[k], g[k]);
       load(j0 + Waves * kRows);  // (the last row again, past the end)
       ids(j0 + 2 * Waves * kRows);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        bf16x8 big, small;
-        parts<T>(y[v], big, small);
+        bf16x8 z[kOfMap<T>];
+        parts<T>(y[v], z);
 #pragma unroll
-        for (int k = 0; k < RT; ++k) {
-          mma<__bf16>(acc[k][v], hi[k], big);
-          mma<__bf16>(acc[k][v], lo[k], big);
-          if constexpr (!__is_same(T, __bf16)) mma<__bf16>(acc[k][v], hi[k], small);
-        }
+        for (int k = 0; k < RT; ++k)
+#pragma unroll
+          for (int p = 0; p < kOfMap<T>; ++p)
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) mma<__bf16>(acc[k][v], g[k][i], z[p]);
       }
     }
   }

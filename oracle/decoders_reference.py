@@ -4,10 +4,10 @@ float32 computation rounded once to its output type may be off.
 E is half a unit in the last place of float32.  A sum of n terms, in any order, each addition off by at
 most 2 E (a matrix instruction's accumulation need not round to nearest): 2 (n + 4) E sum |terms|.
 
-  adapters   hidden values h are such sums of D terms.  Where rows and maps have 16 bits, a second product
-             takes h as two 16-bit floats of 8 bits each, off by 2^-16 |h|, and the product of the two
-             smaller parts may be left out, as much again: SPLIT.  The errors of h add up through the second
-             sum at the weights of its terms.
+  adapters   hidden values h are such sums of D terms, and enter the second sum with all their bits.  Their
+             errors add up through it at the weights of its terms.  (Where a factor is the sum of several
+             16-bit floats, a matrix instruction adds many products before it rounds: a term's parts count
+             as one addition.)
   clipping   the norm's squares are exact in 64 bits; it is rounded once, the factor once, the product once.
 
 Every output is then rounded to its type: U[dtype] of its size, or half a denormal step.
@@ -20,7 +20,6 @@ import torch
 
 from .codes_reference import E, U, _rounded, check  # noqa: F401
 
-SPLIT = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -15, torch.float16: 2.0 ** -15}
 NAN = math.nan
 
 
@@ -93,7 +92,7 @@ def _product(a, da, b, db, n):
 def adapters(rows, groups, down, up, base=None, scale=1.0, by_code=False, grad=None):
     """{name: (value, bound)} of out and, with grad, of g_rows, g_down, g_up."""
     order, places, starts = groups
-    dtype, split = rows.dtype, SPLIT[rows.dtype]
+    dtype = rows.dtype
     K, r, D = down.shape
     Eo = up.shape[1]
     x = rows.reshape(-1, D).double()
@@ -118,17 +117,15 @@ def adapters(rows, groups, down, up, base=None, scale=1.0, by_code=False, grad=N
             continue
         xs, m = x[n], n.numel()
         h, dh = _product(xs, zero(m, D).double(), dn[k].t(), zero(D, r).double(), D)
-        held = dh + split * h.abs()
-        y, dy = _product(h, held, u[k].t(), zero(r, Eo).double(), r)
+        y, dy = _product(h, dh, u[k].t(), zero(r, Eo).double(), r)
         out[n], d_out[n] = scale * y, abs(scale) * (dy + 2 * E * y.abs())
         if train:
             gs = g[n]
             q, dq = _product(gs, zero(m, Eo).double(), u[k], zero(Eo, r).double(), Eo)
             q, dq = scale * q, abs(scale) * (dq + 2 * E * q.abs())
-            held_q = dq + split * q.abs()
-            gx[n], d_gx[n] = _product(q, held_q, dn[k], zero(r, D).double(), r)
-            g_down[k], d_down[k] = _product(q.t(), held_q.t(), xs, zero(m, D).double(), m)
-            a, da = _product(gs.t(), zero(Eo, m).double(), h, held, m)
+            gx[n], d_gx[n] = _product(q, dq, dn[k], zero(r, D).double(), r)
+            g_down[k], d_down[k] = _product(q.t(), dq.t(), xs, zero(m, D).double(), m)
+            a, da = _product(gs.t(), zero(Eo, m).double(), h, dh, m)
             g_up[k], d_up[k] = scale * a, abs(scale) * (da + 2 * E * a.abs())
     total = out + b
     bound = _rounded(d_out + 2 * E * (out.abs() + b.abs()).nan_to_num(0.0), total, dtype)
