@@ -6,8 +6,8 @@ has no counterpart.
 """
 from __future__ import annotations
 
-import ctypes
-from typing import Iterable, List, Optional, Sequence
+import math
+from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -23,8 +23,157 @@ def _dense(t: Tensor) -> bool:
     return torch.ops.aten.is_non_overlapping_and_dense(t)
 
 
-def _range(t: Tensor):
-    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+class _Memory(NamedTuple):
+    """Where a tensor's values lie, in bytes: pieces of `piece` adjacent ones, from `first` on, `axes` of them."""
+
+    first: int
+    piece: int
+    axes: Tuple[Tuple[int, int], ...]  # (how many, how far apart), the farthest apart first
+
+    @property
+    def end(self) -> int:
+        return self.first + self.piece + sum((n - 1) * s for n, s in self.axes)
+
+
+def _memory(t: Tensor) -> _Memory:
+    size = t.element_size()
+    if t.is_contiguous():
+        return _Memory(t.data_ptr(), t.numel() * size, ())
+    # (values that are repeated lie in one place)
+    axes = sorted(((n, s * size) for n, s in zip(t.shape, t.stride()) if n > 1 and s != 0), key=lambda a: -a[1])
+    piece = size
+    while axes and axes[-1][1] == piece:
+        piece *= axes.pop()[0]
+    return _Memory(t.data_ptr(), piece, tuple(axes))
+
+
+_MOST_STEPS = 1 << 14
+
+
+def _reaches(base: int, terms, lo: int, hi: int) -> bool:
+    """Whether base + a sum of x * s over terms (s, least x, largest x) lies in [lo, hi] for some whole numbers x.
+
+    The largest s first, since what the others can make up for leaves few x then; where the search is long all the same,
+    True."""
+    terms = sorted(terms, reverse=True)
+    rest = [(0, 0, 0)]  # of the terms from k on: the least sum, the largest, what all sums are multiples of
+    for s, a, b in reversed(terms):
+        least, most, unit = rest[-1]
+        rest.append((least + s * a, most + s * b, math.gcd(s, unit)))
+    rest.reverse()
+    steps = 0
+
+    def search(k: int, at: int) -> bool:
+        nonlocal steps
+        steps += 1
+        least, most, unit = rest[k]
+        if steps > _MOST_STEPS:
+            return True
+        if at + most < lo or at + least > hi or (unit > 0 and lo + (at - lo) % unit > hi):
+            return False
+        if k == len(terms):
+            return True
+        s, a, b = terms[k]
+        least, most, _ = rest[k + 1]
+        a, b = max(a, -((at + most - lo) // s)), min(b, (hi - at - least) // s)
+        return any(search(k + 1, at + x * s) for x in range(a, b + 1))
+
+    return search(0, base)
+
+
+def _meet(a: _Memory, b: _Memory) -> bool:
+    """Whether two tensors have a byte in common."""
+    if not a.axes and not b.axes:
+        return a.first < b.end and b.first < a.end
+    span = {}
+    for n, s in a.axes:
+        span[s] = (span.get(s, (0, 0))[0] - (n - 1), 0)
+    for n, s in b.axes:
+        least, most = span.get(s, (0, 0))
+        span[s] = (least, most + n - 1)
+    return _reaches(b.first - a.first, [(s, *x) for s, x in span.items()], 1 - b.piece, a.piece - 1)
+
+
+def _repeats(t: Tensor) -> bool:
+    """Whether two of a tensor's values have a byte in common."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        return True
+    m = _memory(t)
+    inner = m.piece
+    for n, s in reversed(m.axes):
+        if s < inner:  # (otherwise each step of an axis leaves all the inner ones behind)
+            break
+        inner += (n - 1) * s
+    else:
+        return False
+    for k, (n, s) in enumerate(m.axes):  # the farthest axis where the two differ
+        terms = [(s, 1, n - 1)] + [(t, 1 - i, i - 1) for i, t in m.axes[k + 1:]]
+        if _reaches(0, terms, 1 - m.piece, m.piece - 1):
+            return True
+    return False
+
+
+def _in_order(ranges) -> bool:
+    """Whether of (first, end, written), sorted, none that is written overlaps another."""
+    written = read = -1
+    for first, end, mine in ranges:
+        if first < max(written, read if mine else -1):
+            return False
+        if mine:
+            written = max(written, end)
+        else:
+            read = max(read, end)
+    return True
+
+
+def _check_shared(gradients: Sequence[Tensor], out: Sequence[Tensor]) -> None:
+    """What is written must be nobody else's, read or written (a tensor may be its own result)."""
+    places, apart = [], []  # (memory, which, written); those that are their own results in another layout
+    for k, (g, o) in enumerate(zip(gradients, out)):
+        if o.numel() == 0:
+            continue
+        if not o.is_contiguous() and _repeats(o):
+            raise ValueError("gradients that are written must not share memory with themselves")
+        to, source = _memory(o), _memory(g)
+        places.append((to, k, True))
+        if source != to:
+            places.append((source, k, False))
+            if source.first == to.first:
+                apart.append(k)
+    places.sort(key=lambda p: (p[0].first, p[0].end))
+    if not apart and _in_order((m.first, m.end, mine) for m, _, mine in places):
+        return
+    # Those whose extents overlap, together.
+    group, end = [], 0
+    for p in [*places, None]:
+        if group and (p is None or p[0].first >= end):
+            if not _separate(group, apart):
+                raise ValueError("gradients that are written must not share memory")
+            group, end = [], 0
+        if p is not None:
+            group.append(p)
+            end = max(end, p[0].end)
+
+
+def _separate(group, apart) -> bool:
+    first = group[0][0]
+    if all(m.axes == first.axes for m, _, _ in group) and not any(k in apart for _, k, _ in group):
+        # Columns of one tensor: steps of the axes are longer than all of them together, so that pieces at the same
+        # steps are what could overlap.
+        inner = max(m.first + m.piece for m, _, _ in group) - first.first
+        for n, s in reversed(first.axes):
+            if s < inner:
+                break
+            inner += (n - 1) * s
+        else:
+            return _in_order((m.first, m.first + m.piece, mine) for m, _, mine in group)
+    for i, (a, k, a_mine) in enumerate(group):
+        for b, j, b_mine in group[i + 1:]:
+            if b.first >= a.end:
+                break
+            if (a_mine or b_mine) and not (k == j and a.first == b.first) and _meet(a, b):
+                return False
+    return True
 
 
 def _clip(gradients: Sequence[Tensor], out: Sequence[Tensor], max_norm: float) -> Tensor:
@@ -89,23 +238,15 @@ def _check_clip(gradients: Sequence[Tensor], out: Sequence[Tensor], max_norm: fl
     _check_size("values in all", sum(g.numel() for g in gradients), _lib.MAX_VALUES)
     _check_device(**{f"gradients[{k}]": g for k, g in enumerate(gradients) if g.device != gradients[0].device},
                   gradients=gradients[0])
-    # What is written must be nobody else's, read or written (a tensor may be its own result).
-    written = sorted(_range(o) for o in out if o.numel() and _dense(o))
-    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
-        raise ValueError("gradients that are written must not share memory")
-    w = 0
-    for lo, hi in sorted(_range(g) for g, o in zip(gradients, out) if g.numel() and g.data_ptr() != o.data_ptr()):
-        while w < len(written) and written[w][1] <= lo:
-            w += 1
-        if w < len(written) and written[w][0] < hi:
-            raise ValueError("gradients that are written must not share memory")
+    _check_shared(gradients, out)
 
 
 def clip_gradients(gradients: Iterable[Tensor], max_norm: float, out: Optional[Iterable[Tensor]] = None) -> Tensor:
     """Scales gradients by min(1, max_norm / norm), norm that of all of them together, and returns it.
 
     gradients: tensors of float32, bfloat16 or float16 and of any shapes on one device (None among them is
-    left out).  out: where the results go; None: in place.  The norm is a float32 tensor without axes; its
+    left out).  out: where the results go; None: in place.  What is written shares no memory with another
+    tensor, nor with itself (as what expand makes does).  The norm is a float32 tensor without axes; its
     squares are added in 64 bits.  max_norm=inf: the norm alone.  Where the norm is not finite (or
     past float32's range) the gradients stay as they are, and the norm says so.  A captured call keeps its max_norm."""
     gradients = gradients if isinstance(gradients, (list, tuple)) else list(gradients)
