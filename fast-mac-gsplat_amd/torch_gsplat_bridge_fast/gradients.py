@@ -11,6 +11,7 @@ from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream_of
@@ -221,6 +222,12 @@ def _(gradients, out, max_norm):
     return gradients[0].new_empty((), dtype=torch.float32)
 
 
+def _check_reverse(tensors: Sequence[Tensor]) -> None:
+    """There is no forward derivative; torch would leave a dual tensor's tangent as it is."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("clipping has no derivative: its tensors must have no tangent (not in forward mode)")
+
+
 def _check_clip(gradients: Sequence[Tensor], out: Sequence[Tensor], max_norm: float) -> None:
     if not gradients:
         raise ValueError("at least one gradient is required")
@@ -258,5 +265,6 @@ def clip_gradients(gradients: Iterable[Tensor], max_norm: float, out: Optional[I
         return norm
     out = None if out is None else [o for g, o in zip(gradients, out) if g is not None]
     gradients = [g for g in gradients if g is not None]
+    _check_reverse(gradients if out is None else [*gradients, *out])
     _check_clip(gradients, gradients if out is None else out, max_norm)
     return _clip_in_place(gradients, float(max_norm)) if out is None else _clip_into(gradients, out, float(max_norm))
