@@ -620,6 +620,9 @@ __global__ __launch_bounds__(kThreads, (kRowsWaves<T, MT, RT, Fit>)) void adapte
   const int parts = Phase == 3 ? 1 : gridDim.y, part = Phase == 3 ? 0 : blockIdx.y;
   if (none) {
     rows_without_code<T, Fit>(A, lds.rows, t.count, part, parts);
+    // (the forward's are an output)
+    if (!Turned && A.hidden && part == 0)
+      for (int i = threadIdx.x; i < t.count * P.r; i += kThreads) A.hidden[t.first * P.r + i] = 0.0f;
     return;
   }
 

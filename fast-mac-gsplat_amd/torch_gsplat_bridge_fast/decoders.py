@@ -176,7 +176,7 @@ def _adapters_meta(flat: Tensor, down: Tensor, up: Tensor, scale: float, by_code
 @torch.library.custom_op(f"{_NS}::code_adapters", mutates_args=())
 def _adapters(rows: Tensor, order: Tensor, places: Tensor, starts: Tensor, down: Tensor, up: Tensor,
               base: Optional[Tensor], scale: float, by_code: bool) -> Tuple[Tensor, Tensor]:
-    """(out, hidden: float32 [rows, rank] in the order of the places)"""
+    """(out, hidden: float32 [rows, rank] in the order of the places, zeros at those without a code)"""
     _check_adapters(rows, order, places, starts, down, up, base, by_code)
     flat, o, p, s, dn, u = _rows_of(rows), *(t.contiguous() for t in (order, places, starts, down, up))
     b = None if base is None else base.contiguous()

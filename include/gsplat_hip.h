@@ -843,8 +843,8 @@ typedef struct gsplat_adapters_meta {
 } gsplat_adapters_meta;
 #define GSPLAT_MAX_RANK 128
 
-/* hidden: float [rows][rank], in the order of the places, for the backward; may
- * be NULL. */
+/* hidden: float [rows][rank], in the order of the places, zeros at those without a
+ * code, for the backward; may be NULL. */
 size_t gsplat_hip_code_adapters_workspace_bytes(const gsplat_adapters_meta* meta);
 int gsplat_hip_code_adapters_forward(const gsplat_adapters_meta* meta,
                                      const void* rows, const int32_t* order,

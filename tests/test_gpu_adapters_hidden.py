@@ -93,3 +93,29 @@ def test_gradients_of_maps(gpu, dtype, r):
     go = against(_normal(g, K, D, dtype=dtype), h[:K], h[K:])
     want, got = _gradients(gpu, codes, x, dn, _normal(g, K, D, r, dtype=dtype), go, scale)
     R.check(got["g_up"], want["g_up"], f"up r={r} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,r", [(9, 70, 5), (61, 4096, 16), (700, 33, 24), (20000, 70, 100), (33000, 59, 8)])
+def test_second_output_of_the_operator(gpu, dtype, N, D, r):
+    """The hidden values, whatever their memory held before: those of rows without a code too."""
+    K, E, g = 6, 40, _gen(N)
+    codes = torch.randint(-1, K + 1, (N,), generator=g).to(torch.int32)  # (K: out of range)
+    x, dn, up = _normal(g, N, D, dtype=dtype), _normal(g, K, r, D, dtype=dtype), _normal(g, K, E, r, dtype=dtype)
+    order, _, starts = R.group(codes, K)
+    named = int(starts[-1])
+    n = order[:named].long()
+    terms = dn.double()[codes[n].long()], x.double()[n, :, None]
+    h = torch.zeros(N, r, dtype=torch.float64)
+    size = h.clone()
+    h[:named], size[:named] = (terms[0] @ terms[1])[..., 0], (terms[0].abs() @ terms[1].abs())[..., 0]
+    groups = gs.group_codes(codes.to(gpu), K)
+    maps = dn.to(gpu), up.to(gpu)
+    for by_code in (False, True):
+        rows = (x[order.long()] if by_code else x).to(gpu)
+        for junk in (float("nan"), 7.0):
+            held = [torch.full((N, r), junk, device=gpu) for _ in range(4)]
+            del held
+            hidden = torch.ops.gsplat_hip.code_adapters(rows, *groups, *maps, None, 1.0, by_code)[1]
+            R.check(hidden, (h, 2 * (D + 4) * R.E * size), f"junk {junk}")
+            assert not hidden[named:].any()
