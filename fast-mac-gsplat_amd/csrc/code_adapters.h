@@ -483,8 +483,9 @@ __device__ __forceinline__ void second_product(const RowsArgs& A, int r, const T
   const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   const T* base = Turned ? nullptr : static_cast<const T*>(A.base);  // (no gradient has one)
   T* out = static_cast<T*>(A.out);
-  // (what is read without a base is a row of `out`, unused: no branch)
-  const T* from = base ? base : out;
+  // (what is read without a base is of the map, which has E values and more, and unused:
+  // no branch)
+  const T* from = base ? base : up;
   const int64_t from_row = base ? A.E : 0;
   const int ld = Turned ? A.E : r;
   auto place = [](int row, int chunk) {
