@@ -257,10 +257,11 @@ __global__ __launch_bounds__(kThreads) void group_finish_kernel(
 }
 
 // How choices are sorted, us of a call.  Few: one launch, 512 choices 5, 2048 12; 4096
-// would take 23, counted 13.  Counted: 65536 of 64 codes 14, 524288 of 256 codes 20
-// (by radix 45) and of 2047 codes 26 (of 2048 by radix 48), 4 million of 256 codes 54
-// (by radix 127); as long as a workgroup's LDS holds a bin a wavefront and code, and
-// the chunks' counts are less than the choices.
+// would take 23, counted 13.  Counted, as long as a workgroup's LDS holds a bin a
+// wavefront and code, and by radix: 2049 choices of 2047 codes 16 and 18, 16384 of 1024
+// codes 15 and 22, 262144 of 64 codes 14 and 42, of 2047 codes 20 and 42 (there are twice
+// as many counts as choices then), 524288 of 256 codes 20 and 48, 2 million of 2047 codes
+// 60 and 81, 4 million of 256 codes 54 and 127.
 enum class Way { kFew, kCounted, kRadix };
 Way way_of(const GroupParams& P) {
   if (P.choices <= kFew && P.K <= 16384) return Way::kFew;
