@@ -34,10 +34,12 @@
 // them, and stores and last reads past the caches (the maps' gradients 155 us
 // without, as what they read was no longer there).
 //
-// Tiles: 64 places (32 above rank 64, for their registers) once codes have 32 on
-// average and tiles fill the card; 16 below.  Measured and not kept: 32 places for
-// narrow rows (22 us for 21), three wavefronts a SIMD for the maps' gradients
-// (155 us, spilled).
+// Tiles: 64 places up to rank 64 once codes have 32 on average and tiles fill the card,
+// otherwise 16 (both sides at rows_plan).  Measured and not kept: 32 places for narrow
+// rows (22 us for 21) and above rank 64 (131072 rows, 256 a code: 416 and 446 us at
+// 1024 -> 1024, rank 128, 132 and 156 at 128 -> 59, rank 96; the rows' gradient 518 and
+// 493, 144 and 200), three wavefronts a SIMD for the maps' gradients at rank 32, which
+// spill (155 us as two took at that time).
 #pragma once
 
 #include <algorithm>
@@ -942,16 +944,25 @@ __global__ __launch_bounds__(kThreads) void adapters_join_kernel(AdapterParams P
 int rank_tiles(int r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 
 // How rows go: tiles of 16 * row_tiles places; splits > 1: hidden values and
-// results in launches of their own, each over parts of a row, for few rows of 2048
-// values and more (one row of 1024 -> 1024: 4.0 and 3.8 us so, 5.6 in one launch
-// that saves the host 3; 61 of 4096 -> 4096: 4.6 and 7.9).
+// results in launches of their own, each over parts of a row.
+//
+// Tiles, us of a forward of 131072 rows in tiles of 16 and of 64 places, by the rows a
+// code has on average: bfloat16 128 -> 59, rank 8: 16 rows 77 and 97, 32 rows 62 and 57,
+// 256 rows 44 and 34; 1024 -> 1024, rank 32: 381 and 381, 274 and 272, 194 and 181; floats
+// 128 -> 59: 70 and 108, 57 and 63, 42 and 39.  The rows' gradient gains more (bfloat16 at
+// 1024: 336 and 328, 236 and 219, 184 and 136).  Fewer rows, 256 a code: 32768 rows 14.4
+// and 11.9, 8192 rows 7.6 and 8.1.
+//
+// Splits, us of a forward at rank 16 in one launch and in two: bfloat16, one row of
+// 1024 -> 1024 6.2 and 7.6, of 2048 8.9 and 7.3, of 4096 14.3 and 7.8; 256 rows 8.0 and
+// 9.2, 12.0 and 9.0, 19.9 and 10.8; 4000 rows 9.6 and 11.9, 16.6 and 16.8, 28.5 and 26.1.
+// Floats of 1024 gain too (9.1 and 7.2), but the second launch takes the host 3 us.
 struct RowsPlan {
   int row_tiles, splits_down, splits_up;
 };
 RowsPlan rows_plan(const AdapterParams& P, int D, int E) {
-  const int big = rank_tiles(P.r) == 8 ? 2 : 4;
-  RowsPlan L{big, 1, 1};
-  if (P.rows >= 32 * (int64_t)P.K && P.rows >= 512 * 16 * big) return L;
+  RowsPlan L{4, 1, 1};
+  if (rank_tiles(P.r) < 8 && P.rows >= 32 * (int64_t)P.K && P.rows >= 512 * 64) return L;
   L.row_tiles = 1;
   const int64_t tiles = std::min<int64_t>(P.rows, P.rows / 16 + P.K);
   if (tiles < 512 && std::max(D, E) >= 2048) {
@@ -982,8 +993,9 @@ int rows_of_rank(const AdapterParams& P, RowsArgs A, const RowsPlan& L, hipStrea
     const int rc = launch_rows<T, 1, RT, 1, Turned, Fit>(P, A, L.splits_down, stream);
     return rc ? rc : launch_rows<T, 1, RT, 2, Turned, Fit>(P, A, A.out ? L.splits_up : 1, stream);
   }
-  if (L.row_tiles == 1) return launch_rows<T, 1, RT, 3, Turned, Fit>(P, A, 1, stream);
-  return launch_rows<T, RT == 8 ? 2 : 4, RT, 3, Turned, Fit>(P, A, 1, stream);
+  if constexpr (RT < 8)
+    if (L.row_tiles > 1) return launch_rows<T, 4, RT, 3, Turned, Fit>(P, A, 1, stream);
+  return launch_rows<T, 1, RT, 3, Turned, Fit>(P, A, 1, stream);
 }
 
 template <typename T, bool Turned>
@@ -1005,7 +1017,13 @@ int rows_of(const AdapterParams& P, RowsArgs A, float* parts, hipStream_t stream
 }
 
 // Places of a chunk: enough workgroups for the card, and sums that are few beside
-// the rows they come from (at 512 places, rank 32 and 16 bits an eighth of them).
+// the rows they come from (4 r / (places * bytes of a value) of them: at 512 places and
+// rank 32 in 16 bits an eighth).  Both gradients in bfloat16, us in chunks of 256, 512,
+// 1024, 2048 and 4096 places (in brackets the one taken): 131072 rows of 1024 -> 1024,
+// rank 32, 256 codes 337 267 189 (188) 187, 8 codes 362 260 218 (205) 248, one code 848
+// 516 340 (260) 236; 128 -> 128, rank 16, 256 codes 69 (65) 49 49 49, 8 codes 55 (52) 47
+// 51 70; 16384 rows of 128 -> 128, 8 codes 20 (22) 25 33 31; 65536 rows of 256 -> 256, rank
+// 128, 8 codes 260 (203) 181 205 182.
 int chunk_of(const AdapterParams& P, int dtype_bytes) {
   const int64_t blocks = (P.D + P.E) * dtype_bytes / 256 + 1;
   int L = 512;
@@ -1075,8 +1093,11 @@ int adapters_backward_of(const AdapterParams& P, const void* grad, const void* r
                    {g_down ? (P.D + W - 1) / W : 0, g_up ? (P.E + W - 1) / W : 0},
                    rank_tiles(P.r) == 8 ? 2 : 1};
   const int fit = fit_of({P.D, P.E}, kVec<T>);
-  // One wavefront a workgroup where that makes enough of them: nothing to join
-  // (201 us for 210 at 131072 x 1024 -> 1024).
+  // One wavefront a workgroup where that makes enough of them: nothing to join.  us in
+  // four and in one, by the number below, bfloat16 of rank 32: 131072 rows of 1024 -> 1024,
+  // 64 codes (2048) 219 and 253, 256 codes (5120) 195 and 187, 1024 codes (17408) 348 and
+  // 240; 128 -> 128, 256 codes (1024) 77 and 87, 4096 codes (4096) 207 and 144; floats
+  // 512 -> 512, 16384 rows: 64 codes (1536) 50 and 56, 256 codes (4096) 64 and 54.
   const bool single = std::min<int64_t>(P.rows / 64, P.K + P.rows / L.chunk) *
                           (A.blocks[0] + A.blocks[1]) * A.rank_blocks >= 4096;
   Slots S{L.chunk, false, 0};

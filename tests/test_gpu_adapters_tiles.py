@@ -1,7 +1,7 @@
-"""Low-rank maps by code with enough rows for the largest tiles (64 places, 32 above rank 64) and for the maps' gradients
+"""Low-rank maps by code with enough rows for the largest tiles (64 places, up to rank 64) and for the maps' gradients
 in one wavefront a workgroup, against the 64-bit formulas (oracle/decoders_reference.py).
 
-Tiles are that large from 32768 rows on (16384 above rank 64), with 32 rows a code on average.  A code of more than 512
+Tiles are that large from 32768 rows on, with 32 rows a code on average.  A code of more than 512
 rows has its maps' gradients from several chunks."""
 import pytest
 import torch
