@@ -23,13 +23,13 @@
 // (An infinite value of a row or a map makes what depends on it infinite or NaN.)
 //
 // What bounds it, on an MI355X: 131072 rows of 1024 -> 1024 values of bfloat16,
-// rank 32, 256 codes: the forward 176 us for 805 MB (4.6 TB/s; a large copy
-// reaches 4.9), the rows' gradient 130 us for 537 MB, the maps' gradients 115 us
-// for 537 MB and the hidden values (4.7 TB/s).  They wait on loads: two to three
+// rank 32, 256 codes: the forward 174 us for 805 MB (4.6 TB/s; a large copy
+// reaches 4.9), the rows' gradient 130 us for 537 MB, the maps' gradients 117 us
+// for 537 MB and the hidden values (4.6 TB/s).  They wait on loads: two to three
 // wavefronts a SIMD, 6 to 12 KB on their way each.  65536 rows of 128 -> 59 floats, rank 8:
 // 22, 21 and 20 us for 49 MB each: one and a half rounds of workgroups, each a
 // chain of dependent loads (starts, order, rows, maps).  What took the first case's
-// step from 785 us to 442: coalesced rows of the factors (turned in LDS), rows
+// step from 785 us to 442 (445 with all bits of the hidden values): coalesced rows of the factors (turned in LDS), rows
 // without a code in all threads, loads without a mask, a branch or a use behind
 // them, and stores and last reads past the caches (the maps' gradients 155 us
 // without, as what they read was no longer there).

@@ -42,7 +42,8 @@ from .codes import _NS, _check_codes, _check_device, _check_dtype, _check_given,
 class CodeGroups(NamedTuple):
     """What group_codes returns, all int32, for N splats of S choices each.
 
-    Places past starts[K] hold the choices without a code, in their order."""
+    Places past starts[K] hold the choices without a code, in their order.  (Groups of another making must be
+    such a sort: values out of range are met by no access, but results that order leaves out are not written.)"""
 
     order: Tensor   # [N*S]: the choice at each place (splat * S + its number), by code and then in their order
     places: Tensor  # [..., S]: the place of each choice; -1 without a code, -2 with one out of range
